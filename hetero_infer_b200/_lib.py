@@ -48,6 +48,14 @@ SIGNATURES = {
     "hq4_pick_token": (_I, [_P, _I, _P, _P, _I, _P]),
     "hq4_pick_token_next": (_I, [_P, _I, _P, _P, _P, _I, _P]),
     "hq4_advance_position": (_I, [_P, _I, _P]),
+    "hq4_paged_append": (_I, [_P, _P, _P] + [_I] * 5 + [_LL] * 3 + [_P, _P, _F, _P, _P, _I, _P, _P, _P, _I, _P, _I,
+                              _P, _P, _I, _I, _I, _LL, _P, _P]),
+    "hq4_paged_attention": (_I, [_P] + [_I] * 5 + [_LL, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _LL, _F, _P, _P,
+                                 _LL, _P]),
+    "hq4_tree_attention": (_I, [_P] + [_I] * 5 + [_LL, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _LL, _P, _I, _F, _P,
+                                _P, _LL, _P]),
+    "hq4_paged_attention_workspace_bytes": (_LL, [_I] * 8),
+    "hq4_sample_rows": (_I, [_P, _I, _I, _I, _LL, _P, _P, _P, _P, _P, _P, _P, _P]),
     "hq4_decode_plan_create": (_I, [_P] + [_I] * 7 + [_F, _F, _P, _P, _I] + [_P] * 6),
     "hq4_decode_plan_run": (_I, [_P, _P]),
     "hq4_decode_plan_info": (_I, [_P, _P]),

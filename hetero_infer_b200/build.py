@@ -17,7 +17,7 @@ INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libhq4.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
-NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-shared",
+NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
               "--expt-relaxed-constexpr", "-Xptxas", "-v"]
 
 
@@ -47,14 +47,25 @@ def build(force: bool = False, verbose: bool = False) -> str:
     """Compile every csrc/*.cu into libhq4.so (skipped when up to date)."""
     if not force and up_to_date():
         return LIB
-    cmd = [nvcc(), *ARCH_FLAGS, *NVCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-o", LIB + ".tmp",
-           *sources()]
-    out = subprocess.run(cmd, capture_output=True, text=True)
-    if out.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + out.stdout + out.stderr)
+    import concurrent.futures
+    import tempfile
+
+    def run(cmd):
+        out = subprocess.run(cmd, capture_output=True, text=True)
+        if out.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + out.stdout + out.stderr)
+        return out.stderr
+
+    with tempfile.TemporaryDirectory() as tmp:  # the files side by side, then one link
+        objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in sources()]
+        cmds = [[nvcc(), *ARCH_FLAGS, *NVCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", s, "-o", o]
+                for s, o in zip(sources(), objs)]
+        with concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+            logs = list(pool.map(run, cmds))
+        run([nvcc(), *ARCH_FLAGS, "-shared", "-o", LIB + ".tmp", *objs])
     os.replace(LIB + ".tmp", LIB)
     if verbose:
-        sys.stdout.write(out.stderr)
+        sys.stdout.write("".join(logs))
     return LIB
 
 

@@ -1,0 +1,307 @@
+// What the attention kernels over a paged cache share: the parameters, the
+// division of the work, the visibility rule and the row-wise slow path.
+//
+// The unit of work is an item: one tile of kRows query rows of one sequence
+// and one key/value head.  The G = n_heads / n_kv query heads of a key/value
+// head are rows of the same tile (row r of a sequence is head r % G of token
+// r / G), so each entry is read once for all of them.  An item's keys are cut
+// into tiles; all items' tiles, in order, are one line of `total` units, of
+// which CTA c takes the c-th equal part.  A part may begin or end inside an
+// item: then the CTA leaves the item's running maximum, sum and unnormalised
+// output of its keys in the workspace, and the combine kernel joins them in
+// key order.  A CTA has at most two such pieces (its first and its last), and
+// every CTA works the same number of key tiles whatever the lengths are.
+#pragma once
+#include "hq4_paged.cuh"
+
+namespace hq4 {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct PagedAttnParams {
+    const void* q;
+    const void *k, *v;
+    void* out;
+    long long q_stride;
+    int n_heads, n_kv, group, head_dim;
+    float scale_log2;              // softmax scale times log2(e)
+    const uint32_t* tree_mask;     // [n_rows][mask_words], or null: causal
+    int mask_words;
+    int split;                     // units are key tiles; else whole items
+    void* ws;
+    PagedBatch b;
+};
+
+struct PagedItem {
+    int s, rt, h;      // sequence, row tile, key/value head
+    int row0, n_tok;   // the sequence's first row and its tokens
+    int len, keys;     // entries before its rows; entries that the tile may see
+    int tiles;         // key tiles
+    int weight;        // units
+    int pad[3];
+    long long first;   // its first unit
+    long long total;   // units of the whole batch
+};
+
+// Rows and lengths of a sequence, clamped to what exists.
+__device__ __forceinline__ void paged_seq(const PagedAttnParams& p, int s, PagedItem& it) {
+    const int a = max(__ldg(p.b.cu_rows + s), 0), e = min(__ldg(p.b.cu_rows + s + 1), p.b.n_rows);
+    it.s = s;
+    it.row0 = a;
+    it.n_tok = max(e - a, 0);
+    it.len = __ldg(p.b.lens + s);
+}
+template <int kRows>
+__device__ __forceinline__ int paged_row_tiles(const PagedAttnParams& p, const PagedItem& it) {
+    return (it.n_tok * p.group + kRows - 1) / kRows;
+}
+// Keys and weight of row tile rt.
+template <int kRows, int kKeys>
+__device__ __forceinline__ void paged_row_tile(const PagedAttnParams& p, int rt, PagedItem& it) {
+    const int cap = p.b.pages_per_seq << p.b.page_shift;
+    const int last = min((rt + 1) * kRows, it.n_tok * p.group) - 1;
+    const int n = p.tree_mask ? it.n_tok : last / p.group + 1;
+    it.rt = rt;
+    it.keys = (int)min(max((long long)it.len + n, 0ll), (long long)cap);
+    it.tiles = max((it.keys + kKeys - 1) / kKeys, 1);  // an item without keys still writes its zeros
+    it.weight = p.split ? it.tiles : 1;
+}
+template <int kRows, int kKeys>
+__device__ __forceinline__ long long paged_seq_units(const PagedAttnParams& p, int s) {
+    PagedItem it;
+    paged_seq(p, s, it);
+    const int n = paged_row_tiles<kRows>(p, it);
+    if (!p.split) return (long long)n * p.n_kv;
+    long long w = 0;
+    for (int rt = 0; rt < n; rt++) {
+        paged_row_tile<kRows, kKeys>(p, rt, it);
+        w += it.tiles;
+    }
+    return w * p.n_kv;
+}
+
+struct PagedScan {
+    long long warp[32];
+    long long before;
+    int seq;
+};
+// Inclusive sum over the CTA's threads; *all = the CTA's sum.
+template <int kThreads>
+__device__ __forceinline__ long long cta_scan(PagedScan& sh, long long v, long long* all) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += y;
+    }
+    __syncthreads();
+    if (lane == 31) sh.warp[w] = v;
+    __syncthreads();
+    long long t = 0;
+    for (int i = 0; i < kThreads / 32; i++) {
+        if (i < w) v += sh.warp[i];
+        t += sh.warp[i];
+    }
+    *all = t;
+    return v;
+}
+
+// The CTA's part [pos, end) and the item that holds its first unit; false for
+// a CTA without work.  Parts are cut for min(gridDim.x, total) CTAs, so that
+// every one of those has some.  All threads take part and get the same.
+template <int kRows, int kKeys, int kThreads>
+__device__ __forceinline__ bool paged_part(const PagedAttnParams& p, PagedScan& sh, PagedItem& it, long long& pos,
+                                           long long& end) {
+    const int n = p.b.n_seqs;
+    long long total = 0, all;
+    long long mine = threadIdx.x < n ? paged_seq_units<kRows, kKeys>(p, threadIdx.x) : 0;
+    long long upto = cta_scan<kThreads>(sh, mine, &total);
+    const long long total0 = total;
+    for (int base = kThreads; base < n; base += kThreads) {
+        const int s = base + threadIdx.x;
+        cta_scan<kThreads>(sh, s < n ? paged_seq_units<kRows, kKeys>(p, s) : 0, &all);
+        total += all;
+    }
+    const long long parts = min((long long)gridDim.x, total);
+    if ((long long)blockIdx.x >= parts) return false;
+    pos = blockIdx.x * total / parts;
+    end = (blockIdx.x + 1) * total / parts;
+    long long run = 0, sum = total0;
+    for (int base = 0;; base += kThreads) {  // ends at the chunk that holds pos: pos < total
+        if (pos < run + sum) {
+            __syncthreads();
+            if (run + upto - mine <= pos && pos < run + upto) {
+                sh.seq = base + threadIdx.x;
+                sh.before = run + upto - mine;
+            }
+            __syncthreads();
+            break;
+        }
+        run += sum;
+        const int s = base + kThreads + threadIdx.x;
+        mine = s < n ? paged_seq_units<kRows, kKeys>(p, s) : 0;
+        upto = cta_scan<kThreads>(sh, mine, &sum);
+    }
+    paged_seq(p, sh.seq, it);
+    long long first = sh.before;
+    for (int rt = 0;; rt++) {
+        paged_row_tile<kRows, kKeys>(p, rt, it);
+        const long long w = (long long)it.weight * p.n_kv;
+        if (pos < first + w) {
+            it.h = (int)((pos - first) / it.weight);
+            it.first = first + (long long)it.h * it.weight;
+            break;
+        }
+        first += w;
+    }
+    it.total = total;
+    return true;
+}
+// The item after `it`; there is one while it.first + it.weight < it.total.
+template <int kRows, int kKeys>
+__device__ __forceinline__ void paged_next(const PagedAttnParams& p, PagedItem& it) {
+    it.first += it.weight;
+    if (++it.h < p.n_kv) return;
+    it.h = 0;
+    int rt = it.rt + 1;
+    while (rt >= paged_row_tiles<kRows>(p, it)) {
+        rt = 0;
+        paged_seq(p, it.s + 1, it);
+    }
+    paged_row_tile<kRows, kKeys>(p, rt, it);
+}
+
+// Whether token tok of the item's sequence sees entry e (0 <= e < keys).
+__device__ __forceinline__ bool paged_sees(const PagedAttnParams& p, const PagedItem& it, int tok, int e) {
+    const int j = e - it.len;  // its place among the new entries
+    if (j < 0) return true;
+    if (!p.tree_mask) return j <= tok;
+    if (j >= it.n_tok || (j >> 5) >= p.mask_words) return false;
+    return __ldg(p.tree_mask + (size_t)(it.row0 + tok) * p.mask_words + (j >> 5)) >> (j & 31) & 1;
+}
+
+// One output row, entry by entry (one warp).  The tiled kernels multiply
+// masked probabilities of zero by values that they do not look at; where such
+// a value is an infinity or a NaN, the row comes out as NaN and is computed
+// here again, from the entries that it sees alone.
+template <class A, class C>
+__device__ __noinline__ void paged_slow_row(const PagedAttnParams& p, const PagedItem& it, int r) {
+    const int lane = threadIdx.x & 31, D = p.head_dim;
+    const int tok = r / p.group, head = it.h * p.group + r % p.group;
+    const A* q = static_cast<const A*>(p.q) + (long long)(it.row0 + tok) * p.q_stride + (long long)head * D;
+    float qv[8], acc[8], m = -INFINITY, l = 0.0f;
+    const int nd = D >> 5;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        qv[i] = i < nd ? Elem<A>::to(q[lane + 32 * i]) : 0.0f;
+        acc[i] = 0.0f;
+    }
+    for (int e = 0; e < it.keys; e++) {
+        if (!paged_sees(p, it, tok, e)) continue;
+        const int page = find_page(p.b, it.s, e);
+        if (page < 0) continue;
+        const long long at = (long long)page * p.b.page_stride +
+                             (((long long)it.h << p.b.page_shift) + (e & ((1 << p.b.page_shift) - 1))) * D;
+        const C* k = static_cast<const C*>(p.k) + at;
+        const C* v = static_cast<const C*>(p.v) + at;
+        float z = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < nd) z = fmaf(qv[i], Elem<C>::to(k[lane + 32 * i]), z);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+        z *= p.scale_log2;
+        const float m1 = (z > m || z != z) ? z : m;
+        const float keep = m == m1 ? 1.0f : exp2f(m - m1), w = exp2f(z - m1);
+        m = m1;
+        l = l * keep + w;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < nd) acc[i] = acc[i] * keep + w * Elem<C>::to(v[lane + 32 * i]);
+    }
+    A* out = static_cast<A*>(p.out) + ((long long)(it.row0 + tok) * p.n_heads + head) * D;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (i < nd) out[lane + 32 * i] = Elem<A>::from(l == 0.0f ? 0.0f : acc[i] / l);
+}
+
+// The pieces of split items in the workspace: CTA c's first piece is 2c, its
+// last one 2c + 1.
+template <int kRows, int kDim>
+struct PagedWs {
+    PagedItem* info;  // of the first piece of each CTA
+    float2* ml;       // [pieces][kRows]: running maximum (of log2 scores) and sum
+    float* o;         // [pieces][kRows][kDim], not divided
+    __host__ __device__ PagedWs(void* ws, int ctas) {
+        unsigned char* p = static_cast<unsigned char*>(ws);
+        info = reinterpret_cast<PagedItem*>(p);
+        p += (size_t)ctas * sizeof(PagedItem);
+        ml = reinterpret_cast<float2*>(p);
+        p += (size_t)ctas * 2 * kRows * sizeof(float2);
+        o = reinterpret_cast<float*>(p);
+    }
+    static __host__ long long bytes(int ctas) {
+        return (long long)ctas * (sizeof(PagedItem) + 2ll * kRows * (sizeof(float2) + kDim * sizeof(float)));
+    }
+};
+static_assert(sizeof(PagedItem) % 16 == 0, "the pieces behind the items keep their alignment");
+
+// CTA (c, y): if part c begins inside an item, and c is the first part that
+// does in that item, joins the item's pieces; one warp to a row.
+constexpr int kCombineWarps = 4;
+template <class A, class C, int kRows, int kDim>
+__global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const PagedAttnParams p, int ctas) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const PagedWs<kRows, kDim> ws(p.ws, ctas);
+    const long long total = ws.info[0].total;  // CTA 0 has work whenever there is any row
+    const long long parts = min((long long)ctas, total);
+    const int c = blockIdx.x + 1;
+    if (c >= parts) return;
+    const PagedItem it = ws.info[c];
+    const long long start = c * total / parts, before = (c - 1) * total / parts;
+    if (it.first == start || it.first < before) return;
+    const int r = blockIdx.y * kCombineWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int row = it.rt * kRows + r;
+    if (r >= kRows || row >= it.n_tok * p.group) return;
+    const int first_piece = 2 * (c - 1) + (it.first == before ? 0 : 1);
+    int n = 1;  // pieces: that one, then the first ones of parts c, c + 1, ...
+    const long long stop = it.first + it.weight;
+    while (c - 1 + n < parts && (c - 1 + n) * total / parts < stop) n++;
+    auto piece = [&](int i) { return i == 0 ? first_piece : 2 * (c - 1 + i); };
+    float m = -INFINITY;
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, ws.ml[(size_t)piece(i) * kRows + r].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float mu = m == -INFINITY ? 0.0f : m;
+    constexpr int kPer = kDim / 32;
+    float acc[kPer], l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; i++) acc[i] = 0.0f;
+    const int D = p.head_dim;
+#pragma unroll 4
+    for (int i = 0; i < n; i++) {
+        const size_t at = (size_t)piece(i) * kRows + r;
+        const float2 ml = ws.ml[at];
+        const float w = exp2f(ml.x - mu);
+        l = fmaf(ml.y, w, l);
+        const float* o = ws.o + at * kDim;
+#pragma unroll
+        for (int j = 0; j < kPer; j++)
+            if (lane + 32 * j < D) acc[j] = fmaf(o[lane + 32 * j], w, acc[j]);
+    }
+    const int tok = row / p.group, head = it.h * p.group + row % p.group;
+    A* out = static_cast<A*>(p.out) + ((long long)(it.row0 + tok) * p.n_heads + head) * D;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < kPer; j++)
+        if (lane + 32 * j < D) {
+            const float y = l == 0.0f ? 0.0f : acc[j] * inv;
+            bad |= y != y;
+            out[lane + 32 * j] = Elem<A>::from(y);
+        }
+    if (__any_sync(0xffffffffu, bad)) paged_slow_row<A, C>(p, it, row);
+}
+
+}  // namespace hq4

@@ -1,0 +1,457 @@
+// Attention over a paged cache for few query rows to a key/value head (decode,
+// small trees), and for fp32 queries: warp-level matrix instructions.
+//
+// Decode is bound by the bytes of the cache.  Each warp walks its own tiles of
+// 16 keys with a running maximum and sum, from a ring of kStages tiles in
+// shared memory that it fills itself with 16-byte asynchronous copies, so
+// warps wait for nobody until the CTA's part of an item is done.  Scores are
+// computed transposed, S^T = K Q^T: 16 keys are the M of m16n8k16 and 8 rows
+// its N, so the 7 or 8 query heads of a key/value head waste nothing, and the
+// fragment of S^T turns into the operand of O^T = V^T P^T by transposing 8x8
+// blocks between lanes (movmatrix).
+//
+// fp32 queries against 16-bit entries keep fp32's precision: the entries are
+// exact in the matrix instructions, and queries and probabilities are sums of
+// 16-bit terms (three bf16 terms hold 24 bits; two fp16 terms of a row scaled
+// by a power of two hold 22).
+#pragma once
+#include "hq4_host.cuh"
+#include "hq4_paged_attn.cuh"
+
+namespace hq4 {
+
+constexpr int kPaWarps = 4;
+constexpr int kPaThreads = kPaWarps * 32;
+constexpr int kPaKeys = 16;  // keys of a tile
+
+template <int kDim>
+struct PaShape {
+    static constexpr int kStages = kDim == 64 ? 4 : 3;
+    static constexpr int kTile = kPaKeys * kDim * 2;                  // bytes of a tile of keys or of values
+    static constexpr int kRing = kStages * 2 * kTile;                 // of a warp
+};
+template <class A, class C>
+constexpr int pa_terms() { return sizeof(A) == 2 ? 1 : Elem<C>::code == HQ4_BF16 ? 3 : 2; }
+template <int kDim, int kRows, int kTerms>
+constexpr int pa_smem() { return kPaWarps * PaShape<kDim>::kRing + kTerms * kRows * kDim * 2; }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    return d;
+}
+template <class C>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    mma_f16_16816(c, a[0], a[1], a[2], a[3], b0, b1);
+}
+template <>
+__device__ __forceinline__ void mma16<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    mma_bf16_16816(c, a[0], a[1], a[2], a[3], b0, b1);
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Byte of the 16-byte chunk c of row r in a tile of rows of kDim 16-bit
+// values; the XOR spreads a column of 8 rows over all banks.
+template <int kDim>
+__device__ __forceinline__ int tile_at(int r, int c) { return r * (kDim * 2) + ((c ^ (r & 7)) << 4); }
+
+template <class A, class C, int kDim, int NT>
+__global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PagedAttnParams p) {
+    constexpr int kRows = 8 * NT, kTerms = pa_terms<A, C>(), kStages = PaShape<kDim>::kStages;
+    constexpr int kTile = PaShape<kDim>::kTile, kRing = PaShape<kDim>::kRing;
+    constexpr int kChunks = kDim / 8, kOs = kDim + 4;
+    static_assert(kRows * kOs * 4 <= kRing, "a warp's outputs fit its ring");
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ PagedScan scan;
+    __shared__ float s_m[kPaWarps][kRows], s_l[kPaWarps][kRows], s_qs[kRows];
+    __shared__ int s_bad[kRows];
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int D = p.head_dim, ksteps = D >> 4;
+    PagedItem it;
+    long long pos, end;
+    const bool busy = paged_part<kRows, kPaKeys, kPaThreads>(p, scan, it, pos, end);
+    if (!busy) {
+        pdl_launch_dependents();
+        if (p.ws && blockIdx.x == 0 && threadIdx.x == 0)  // a batch without rows: nothing to join
+            PagedWs<kRows, kDim>(p.ws, gridDim.x).info[0].total = 0;
+        return;
+    }
+    const long long start = pos;
+    const PagedWs<kRows, kDim> ws(p.ws, gridDim.x);
+    if (p.ws && threadIdx.x == 0) ws.info[blockIdx.x] = it;
+    unsigned char* ring = smem + warp * kRing;
+    const uint32_t ring_u = smem_u32(ring);
+    unsigned char* qs = smem + kPaWarps * kRing;
+    const uint32_t qs_u = smem_u32(qs);
+    const C* kc = static_cast<const C*>(p.k);
+    const C* vc = static_cast<const C*>(p.v);
+    const int in_page = (1 << p.b.page_shift) - 1;
+    float* os = reinterpret_cast<float*>(ring);
+
+    while (pos < end) {
+        const long long stop = min(end, it.first + it.weight);
+        const int t0 = p.split ? (int)(pos - it.first) : 0, t1 = p.split ? (int)(stop - it.first) : it.tiles;
+        const bool whole = t0 == 0 && t1 == it.tiles;
+        const int rows = min(kRows, it.n_tok * p.group - it.rt * kRows);
+        if (stop == end) pdl_launch_dependents();
+        if (threadIdx.x == 0 && (it.len < 0 || (long long)it.len + it.n_tok > (long long)p.b.pages_per_seq << p.b.page_shift))
+            atomicOr(p.b.status, kStatusPaged);  // rows whose entries have no place
+
+        // ---- this part's keys start to arrive ------------------------------
+        auto load_tile = [&](int t, int stage) -> uint32_t {
+            const int e = t * kPaKeys + (lane & 15);
+            int page = -1;
+            if (t < t1 && e < it.keys) {
+                page = find_page(p.b, it.s, e);
+                if (page < 0 && lane < 16) atomicOr(p.b.status, kStatusPaged);
+            }
+            const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
+            const long long at = page < 0 ? 0
+                                          : (long long)page * p.b.page_stride +
+                                                (((long long)it.h << p.b.page_shift) + (e & in_page)) * D;
+            if (t < t1) {
+                const uint32_t kd = ring_u + stage * 2 * kTile, vd = kd + kTile;
+#pragma unroll
+                for (int i = 0; i < kPaKeys * kChunks / 32; i++) {
+                    const int idx = lane + 32 * i, r = idx / kChunks, c = idx % kChunks;
+                    const long long src = __shfl_sync(0xffffffffu, at, r) + c * 8;
+                    const bool on = ok >> r & 1;
+                    if (c * 8 < D) {  // without a page: zeros, so that what lies there does not reach the products
+                        const int d = tile_at<kDim>(r, c);
+                        cp_async16(kd + d, kc + (on ? src : 0), on);
+                        cp_async16(vd + d, vc + (on ? src : 0), on);
+                    }
+                }
+            }
+            cp_async_commit();
+            return ok;
+        };
+        unsigned long long oks = 0;  // 16 bits of a stage: which of its keys have a page
+#pragma unroll
+        for (int s = 0; s < kStages - 1; s++)
+            oks |= (unsigned long long)load_tile(t0 + warp + s * kPaWarps, s) << (16 * s);
+
+        // ---- the queries, as 16-bit terms ----------------------------------
+        for (int r = warp; r < kRows; r += kPaWarps) {
+            const int row = it.rt * kRows + r;
+            const bool on = r < rows;
+            const A* src = static_cast<const A*>(p.q) + (long long)(it.row0 + (on ? row / p.group : 0)) * p.q_stride +
+                           ((long long)it.h * p.group + (on ? row % p.group : 0)) * D;
+            if constexpr (kTerms == 1) {
+                for (int c = lane; c < kChunks; c += 32) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (on && c * 8 < D) v = __ldg(reinterpret_cast<const uint4*>(src + c * 8));
+                    *reinterpret_cast<uint4*>(qs + tile_at<kDim>(r, c)) = v;
+                }
+                if (lane == 0) s_qs[r] = 1.0f;
+            } else {
+                constexpr int kN = (kChunks + 31) / 32;
+                float x[kN][8];
+                float top = 0.0f;
+#pragma unroll
+                for (int n = 0; n < kN; n++) {
+                    const int c = lane + 32 * n;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[n][i] = 0.0f;
+                    if (on && c < kChunks && c * 8 < D) load8(reinterpret_cast<const float*>(src) + c * 8, x[n]);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[n][i]));
+                }
+                // fp16 terms: the row's largest value to [2^13, 2^14), so that the second term of all
+                // but the smallest values is a normal number
+                float up = 1.0f;
+                if constexpr (kTerms == 2) {
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    if (top > 0.0f && top < INFINITY) {
+                        const int ex = (int)(__float_as_uint(top) >> 23) - 127;
+                        up = exp2i(min(max(13 - ex, -110), 110));
+                    }
+                }
+                if (lane == 0) s_qs[r] = 1.0f / up;
+#pragma unroll
+                for (int n = 0; n < kN; n++) {
+                    const int c = lane + 32 * n;
+                    if (c >= kChunks) continue;
+#pragma unroll
+                    for (int term = 0; term < kTerms; term++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float a = x[n][2 * i] * (term == 0 ? up : 1.0f), b = x[n][2 * i + 1] * (term == 0 ? up : 1.0f);
+                            w[i] = pack2<C>(a, b);
+                            const float2 f = unpack2<C>(w[i]);
+                            x[n][2 * i] = a - f.x;
+                            x[n][2 * i + 1] = b - f.y;
+                        }
+                        *reinterpret_cast<uint4*>(qs + term * (kRows * kDim * 2) + tile_at<kDim>(r, c)) =
+                            make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+        }
+        if (threadIdx.x < kRows) s_bad[threadIdx.x] = 0;
+        __syncthreads();
+
+        // ---- the keys --------------------------------------------------------
+        const int g = lane >> 2, t2 = (lane & 3) * 2;
+        float acc[kDim / 16][NT][4], m[NT][2], l[NT][2], qf[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int d = 0; d < kDim / 16; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[d][n][i] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                m[n][i] = -INFINITY;
+                l[n][i] = 0.0f;
+                qf[n][i] = s_qs[n * 8 + t2 + i] * p.scale_log2;
+            }
+        }
+        const int first_tok = it.rt * kRows / p.group;
+        int stage = 0;
+        for (int t = t0 + warp; t < t1; t += kPaWarps) {
+            int ahead = stage + kStages - 1;
+            if (ahead >= kStages) ahead -= kStages;
+            __syncwarp();  // the tile that is overwritten was read by all lanes
+            const uint32_t more = load_tile(t + (kStages - 1) * kPaWarps, ahead);
+            const uint32_t ok = (uint32_t)oks & 0xffffu;
+            oks = (oks >> 16) | (unsigned long long)more << (16 * (kStages - 2));
+            cp_async_wait<kStages - 1>();
+            __syncwarp();
+            const uint32_t kd = ring_u + stage * 2 * kTile, vd = kd + kTile;
+            float sc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) sc[n][i] = 0.0f;
+#pragma unroll
+            for (int k2 = 0; k2 < kDim / 32; k2++) {
+                if (k2 * 2 >= ksteps) break;
+                uint32_t a0[4], a1[4];
+                const int r = lane & 15, c = k2 * 4 + (lane >> 4);
+                ldsm4(kd + tile_at<kDim>(r, c), a0);
+                ldsm4(kd + tile_at<kDim>(r, c + 2), a1);
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int term = kTerms - 1; term >= 0; term--) {
+                        uint32_t b[4];
+                        ldsm4(qs_u + term * (kRows * kDim * 2) + tile_at<kDim>(n * 8 + (lane & 7), k2 * 4 + (lane >> 3)), b);
+                        mma16<C>(sc[n], a0, b[0], b[1]);
+                        mma16<C>(sc[n], a1, b[2], b[3]);
+                    }
+            }
+            const bool plain = ok == 0xffffu && (t + 1) * kPaKeys <= it.len + (p.tree_mask ? 0 : first_tok + 1);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float z = sc[n][i] * qf[n][i & 1];
+                    if (!plain) {
+                        const int kr = g + (i >> 1) * 8, row = it.rt * kRows + n * 8 + t2 + (i & 1);
+                        if (!(ok >> kr & 1) || n * 8 + t2 + (i & 1) >= rows ||
+                            !paged_sees(p, it, row / p.group, t * kPaKeys + kr))
+                            z = -INFINITY;
+                    }
+                    sc[n][i] = z;
+                }
+                float keep[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    float x = fmaxf(sc[n][i], sc[n][i + 2]);
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    const float m1 = fmaxf(m[n][i], x), mu = m1 == -INFINITY ? 0.0f : m1;
+                    keep[i] = ex2(m[n][i] - mu);
+                    m[n][i] = m1;
+                    sc[n][i] = ex2(sc[n][i] - mu);
+                    sc[n][i + 2] = ex2(sc[n][i + 2] - mu);
+                    l[n][i] = fmaf(l[n][i], keep[i], sc[n][i] + sc[n][i + 2]);
+                }
+                if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f)) {
+#pragma unroll
+                    for (int d = 0; d < kDim / 16; d++) {
+                        acc[d][n][0] *= keep[0];
+                        acc[d][n][1] *= keep[1];
+                        acc[d][n][2] *= keep[0];
+                        acc[d][n][3] *= keep[1];
+                    }
+                }
+            }
+            // the probabilities as 16-bit terms (of fp16: scaled by 2^14, which the epilogue takes back, so that
+            // those of 2^-28 of the largest are still normal numbers), transposed
+            uint32_t pb[NT][kTerms][2];
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int hh = 0; hh < 2; hh++) {
+                    float a = sc[n][2 * hh], b = sc[n][2 * hh + 1];
+                    if constexpr (kTerms == 2) {
+                        a *= 16384.0f;
+                        b *= 16384.0f;
+                    }
+#pragma unroll
+                    for (int term = 0; term < kTerms; term++) {
+                        const uint32_t w = pack2<C>(a, b);
+                        pb[n][term][hh] = transpose8(w);
+                        const float2 f = unpack2<C>(w);
+                        a -= f.x;
+                        b -= f.y;
+                    }
+                }
+#pragma unroll
+            for (int d = 0; d < kDim / 16; d++) {
+                if (d >= ksteps) break;
+                uint32_t a[4];
+                ldsm4_t(vd + tile_at<kDim>((lane & 7) + (lane >> 4) * 8, d * 2 + (lane >> 3 & 1)), a);
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int term = kTerms - 1; term >= 0; term--) mma16<C>(acc[d][n], a, pb[n][term][0], pb[n][term][1]);
+            }
+            if (++stage == kStages) stage = 0;
+        }
+        cp_async_wait<0>();
+
+        // ---- the warps' results, joined --------------------------------------
+        const float back = kTerms == 2 ? 1.0f / 16384.0f : 1.0f;
+        __syncwarp();  // the ring is the warp's own: its lanes have read their last tile
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                float x = l[n][i];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                const int r = n * 8 + t2 + i;
+                if (g == 0) {
+                    s_m[warp][r] = m[n][i];
+                    s_l[warp][r] = x;
+                }
+#pragma unroll
+                for (int d = 0; d < kDim / 16; d++) {
+                    if (d >= ksteps) break;
+                    os[r * kOs + d * 16 + g] = acc[d][n][i] * back;
+                    os[r * kOs + d * 16 + g + 8] = acc[d][n][i + 2] * back;
+                }
+            }
+        }
+        __syncthreads();
+        const int piece = 2 * blockIdx.x + (pos == start ? 0 : 1);
+        for (int r = warp; r < rows; r += kPaWarps) {
+            float mm = -INFINITY, ll = 0.0f, w[kPaWarps];
+#pragma unroll
+            for (int i = 0; i < kPaWarps; i++) mm = fmaxf(mm, s_m[i][r]);
+            const float mu = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+            for (int i = 0; i < kPaWarps; i++) {
+                w[i] = exp2f(s_m[i][r] - mu);
+                ll = fmaf(s_l[i][r], w[i], ll);
+            }
+            const int row = it.rt * kRows + r;
+            if (whole)
+#pragma unroll
+                for (int i = 0; i < kPaWarps; i++) w[i] = ll == 0.0f ? 0.0f : w[i] / ll;
+            A* out = static_cast<A*>(p.out) + ((long long)(it.row0 + row / p.group) * p.n_heads + it.h * p.group + row % p.group) * D;
+            float* part = ws.o + ((size_t)piece * kRows + r) * kDim;
+            bool bad = false;
+            for (int d = lane; d < D; d += 32) {
+                float y = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kPaWarps; i++)
+                    y = fmaf(reinterpret_cast<const float*>(smem + i * kRing)[r * kOs + d], w[i], y);
+                if (whole) {
+                    if (ll == 0.0f) y = 0.0f;
+                    bad |= y != y;
+                    out[d] = Elem<A>::from(y);
+                } else {
+                    part[d] = y;
+                }
+            }
+            if (!whole && lane == 0) ws.ml[(size_t)piece * kRows + r] = make_float2(mm, ll);
+            if (whole && __any_sync(0xffffffffu, bad)) paged_slow_row<A, C>(p, it, row);
+        }
+        __syncthreads();  // the rings and the queries are free again
+        pos = stop;
+        if (pos < end) paged_next<kRows, kPaKeys>(p, it);
+    }
+}
+
+// ---- launch ------------------------------------------------------------------
+
+struct PaPlan {
+    int nt, dim, ctas, split;
+    long long ws;
+};
+
+static inline cudaError_t launch_pdl_kernel(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStream_t st, void** args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = grid;
+    lc.blockDim = block;
+    lc.dynamicSmemBytes = smem;
+    lc.stream = st;
+    lc.attrs = attr;
+    lc.numAttrs = 1;
+    return cudaLaunchKernelExC(&lc, fn, args);
+}
+
+template <class A, class C, int kDim, int NT>
+static int launch_pa(PagedAttnParams p, const PaPlan& pl, cudaStream_t st) {
+    constexpr int smem = pa_smem<kDim, 8 * NT, pa_terms<A, C>()>();
+    auto kern = paged_attn_kernel<A, C, kDim, NT>;
+    static PerDeviceOnce once;
+    if (smem_opt_in(once, kern, smem) != cudaSuccess) return HQ4_ERR_LAUNCH;
+    void* args[] = {&p};
+    if (launch_pdl_kernel((const void*)kern, dim3(pl.ctas), dim3(kPaThreads), smem, st, args) != cudaSuccess)
+        return HQ4_ERR_LAUNCH;
+    if (!pl.split || pl.ctas < 2) return HQ4_OK;
+    int ctas = pl.ctas;
+    void* cargs[] = {&p, &ctas};
+    return launch_pdl_kernel((const void*)paged_combine_kernel<A, C, 8 * NT, kDim>,
+                             dim3(pl.ctas - 1, (8 * NT + kCombineWarps - 1) / kCombineWarps), dim3(kCombineWarps * 32),
+                             0, st, cargs) == cudaSuccess
+               ? HQ4_OK
+               : HQ4_ERR_LAUNCH;
+}
+template <class A, class C, int kDim>
+static int launch_pa_nt(const PagedAttnParams& p, const PaPlan& pl, cudaStream_t st) {
+    if constexpr (kDim <= 128) {
+        if (pl.nt == 4) return launch_pa<A, C, kDim, 4>(p, pl, st);
+    }
+    return pl.nt == 1 ? launch_pa<A, C, kDim, 1>(p, pl, st) : launch_pa<A, C, kDim, 2>(p, pl, st);
+}
+template <class A, class C>
+static int launch_pa_dim(const PagedAttnParams& p, const PaPlan& pl, cudaStream_t st) {
+    return pl.dim == 64 ? launch_pa_nt<A, C, 64>(p, pl, st)
+         : pl.dim == 128 ? launch_pa_nt<A, C, 128>(p, pl, st) : launch_pa_nt<A, C, 256>(p, pl, st);
+}
+
+}  // namespace hq4

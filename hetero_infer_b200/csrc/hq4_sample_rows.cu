@@ -1,0 +1,528 @@
+// Sampling a token for each row of a batch: temperature, top-k, top-p, min-p
+// and the draw for given random numbers.
+//
+// With the entries in descending order (equal values by index), each filter
+// keeps a beginning of that order, so the kept set is what the shortest one
+// keeps, and the draw walks it in index order.  Nothing is sorted: a cluster of
+// CTAs holds a row in shared memory (read from memory once), and the value at
+// which a filter ends is found by a radix search.  Its keys are the distances
+// below the maximum in 2^15 equal steps over the 44 octaves that have mass --
+// a monotone function of the value whose digits, unlike the float's own, split
+// a row evenly -- five bits at a time; the few entries of the last step are
+// compared with one another.
+//
+// Masses are integers: w = floor(2^44 * 2^((x - max) / T * log2 e)) from fp64
+// arithmetic, at least 1, and 0 below 2^-44 of the maximum.  Their sums are
+// exact, so the token does not depend on how the work is divided, and the
+// cumulative bounds are off by less than 2^-40 of the whole, where fp32 sums
+// over 1.5e5 entries would be off by 1e-6 and move tokens.
+//
+// A digit's 32 sums are taken in columns of shared memory, one to a thread
+// (no atomics), then over the threads and the cluster.
+#include <algorithm>
+
+#include "hq4_host.cuh"
+#include "hq4_paged.cuh"
+
+namespace hq4 {
+
+int check_device_cap();
+int* status_word();
+
+constexpr int kSrBins = 32;
+constexpr float kSrSteps = 32768.0f;   // of the search's keys
+constexpr double kSrOctaves = 44.0;    // that have mass
+constexpr int kSrList = 512;           // entries of one step that are compared directly
+constexpr int kSrMaxCluster = 8;
+constexpr int kSrMaxSlice = 36864;     // entries of a CTA
+
+struct SampleRowsParams {
+    const void* x;
+    long long stride;
+    int n, chunk;  // chunk: entries of a CTA
+    const float* temperature;
+    const int* top_k;
+    const float *top_p, *min_p;
+    const double* u;
+    int* tok;
+    float* logp;
+    int* status;
+};
+
+typedef unsigned long long u64;
+
+__device__ __forceinline__ void st_cluster_u64(uint32_t addr, u64 v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ u64 ld_cluster_u64(uint32_t addr) {
+    u64 v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t atom_add_cluster(uint32_t addr, uint32_t v) {
+    uint32_t r;
+    asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(r) : "r"(addr), "r"(v) : "memory");
+    return r;
+}
+// Bits that order as the floats do, and back.
+__device__ __forceinline__ uint32_t order_bits(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float order_value(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+template <int T>
+struct SampleRowsShared {
+    u64 all[2][kSrMaxCluster][kSrBins];  // the CTAs' sums of a digit, by turns
+    u64 sums[kSrBins];
+    u64 warp[T / 32];
+    u64 pair[2][kSrMaxCluster];          // a number of each CTA, by turns
+    uint32_t list[kSrList];              // rank 0's: keys of one step's entries
+    uint32_t n_list, best;
+    u64 best_above;
+    u64 bin_before;
+    int bin;
+};
+
+template <int T>
+struct SampleRow {
+    SampleRowsShared<T>& sh;
+    u64* hist;         // [kSrBins][T]
+    const float* xs;   // this CTA's slice
+    int cnt, rank, nr, turn, pturn;
+    float top, steps;  // the maximum; steps of the search's keys for a unit of x
+    double oct;        // octaves for a unit of x
+
+    // Sum over the cluster; every thread gets it, and the sum of lower ranks.
+    __device__ u64 cluster_sum(u64 v, u64* lower = nullptr) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = v;
+        __syncthreads();
+        if ((int)threadIdx.x < nr) {
+            u64 t = 0;
+            for (int w = 0; w < T / 32; w++) t += sh.warp[w];
+            st_cluster_u64(map_to_rank(smem_u32(&sh.pair[pturn][rank]), threadIdx.x), t);
+        }
+        cluster_sync();
+        u64 t = 0, lo = 0;
+        for (int r = 0; r < nr; r++) {
+            if (r < rank) lo += sh.pair[pturn][r];
+            t += sh.pair[pturn][r];
+        }
+        pturn ^= 1;
+        if (lower) *lower = lo;
+        return t;
+    }
+    __device__ uint32_t cluster_max(uint32_t v) {  // of 32-bit numbers
+        v = __reduce_max_sync(0xffffffffu, v);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = v;
+        __syncthreads();
+        if ((int)threadIdx.x < nr) {
+            u64 t = 0;
+            for (int w = 0; w < T / 32; w++) t = max(t, sh.warp[w]);
+            st_cluster_u64(map_to_rank(smem_u32(&sh.pair[pturn][rank]), threadIdx.x), t);
+        }
+        cluster_sync();
+        u64 t = 0;
+        for (int r = 0; r < nr; r++) t = max(t, sh.pair[pturn][r]);
+        pturn ^= 1;
+        return (uint32_t)t;
+    }
+    // The search's key of x, at least kSrSteps for an entry without mass.
+    __device__ __forceinline__ float key(float x) const { return (top - x) * steps; }
+    __device__ __forceinline__ bool has_mass(float x) const { return key(x) < kSrSteps; }
+    // The mass of an entry that has some.  2^-f for f in [0, 1) by its Taylor
+    // series about 1/2: the term left out is below 2e-10.
+    __device__ u64 mass(float x) const {
+        const double z = ((double)top - (double)x) * oct;
+        const int e = (int)z;
+        const double t = (0.5 - (z - e)) * 0.6931471805599453094;  // ln(2^(1/2 - f))
+        double s = 1.0 / 40320.0;
+        s = fma(s, t, 1.0 / 5040.0);
+        s = fma(s, t, 1.0 / 720.0);
+        s = fma(s, t, 1.0 / 120.0);
+        s = fma(s, t, 1.0 / 24.0);
+        s = fma(s, t, 1.0 / 6.0);
+        s = fma(s, t, 0.5);
+        s = fma(s, t, 1.0);
+        s = fma(s, t, 1.0);
+        s *= 0.70710678118654752440 * 17592186044416.0;  // 2^-1/2 * 2^44
+        const u64 w = (u64)s >> min(e, 63);
+        return w ? w : 1;
+    }
+    __device__ __forceinline__ u64 weight(float x, bool counting) const { return counting ? 1 : mass(x); }
+
+    // The smallest value v >= floor_key's of an entry with mass such that the
+    // entries above it weigh less than `target` (each its mass, or one), and
+    // what those weigh.  There is one when target >= 1.
+    __device__ uint32_t find_end(bool counting, u64 target, uint32_t floor_key, u64& above) {
+        u64 before = 0;  // weight of the entries above the searched range
+        int prefix = 0;  // the key's digits so far
+        for (int shift = 10; shift >= 0; shift -= 5) {
+            for (int b = 0; b < kSrBins; b++) hist[b * T + threadIdx.x] = 0;
+            for (int i = threadIdx.x; i < cnt; i += T) {
+                const float x = xs[i], k = key(x);
+                if (!(k < kSrSteps) || order_bits(x) < floor_key) continue;
+                const int f = (int)k >> shift;
+                if (f >> 5 == prefix) hist[(f & 31) * T + threadIdx.x] += weight(x, counting);
+            }
+            __syncthreads();
+            const int lane = threadIdx.x & 31;
+            for (int b = threadIdx.x >> 5; b < kSrBins; b += T / 32) {
+                u64 v = 0;
+#pragma unroll 8
+                for (int j = 0; j < T / 32; j++) v += hist[b * T + j * 32 + lane];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                if (lane == 0) sh.sums[b] = v;
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < nr * kSrBins; i += T)
+                st_cluster_u64(map_to_rank(smem_u32(&sh.all[turn][rank][i & 31]), i >> 5), sh.sums[i & 31]);
+            cluster_sync();
+            if (threadIdx.x < 32) {  // a bin to a lane
+                u64 v = 0;
+                for (int r = 0; r < nr; r++) v += sh.all[turn][r][lane];
+                u64 upto = v;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += y;
+                }
+                const u64 excl = before + upto - v;
+                const uint32_t ok = __ballot_sync(0xffffffffu, v != 0 && excl < target);
+                const int b = ok ? 31 - __clz(ok) : 0;  // the last step that begins below the target
+                if (lane == b) {
+                    sh.bin = b;
+                    sh.bin_before = excl;
+                }
+            }
+            __syncthreads();
+            turn ^= 1;
+            before = sh.bin_before;
+            prefix = prefix << 5 | sh.bin;
+        }
+        // the entries of the last step
+        if (threadIdx.x == 0) {
+            sh.n_list = 0;
+            sh.best = 0xffffffffu;
+        }
+        cluster_sync();
+        const uint32_t head = map_to_rank(smem_u32(&sh.n_list), 0);
+        uint32_t low = 0xffffffffu, high = 0;
+        for (int i = threadIdx.x; i < cnt; i += T) {
+            const float x = xs[i], k = key(x);
+            const uint32_t ob = order_bits(x);
+            if (!(k < kSrSteps) || (int)k != prefix || ob < floor_key) continue;
+            low = min(low, ob);
+            high = max(high, ob);
+            const uint32_t at = atom_add_cluster(head, 1);
+            if (at < kSrList) st_cluster_u32(map_to_rank(smem_u32(&sh.list[at]), 0), ob);
+        }
+        cluster_sync();
+        const uint32_t n = (uint32_t)ld_cluster_u32(head);
+        if (n <= kSrList) {
+            if (rank == 0) {
+                for (uint32_t i = threadIdx.x; i < n; i += T) {
+                    const uint32_t mine = sh.list[i];
+                    u64 a = before;
+                    for (uint32_t j = 0; j < n; j++) {
+                        const uint32_t o = sh.list[j];
+                        if (o > mine) a += weight(order_value(o), counting);
+                    }
+                    if (a < target) atomicMin(&sh.best, mine);
+                }
+                __syncthreads();
+                const uint32_t v = sh.best;
+                u64 a = 0;
+                for (uint32_t i = threadIdx.x; i < n; i += T)
+                    if (sh.list[i] > v) a += weight(order_value(sh.list[i]), counting);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+                if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = a;
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    a = before;
+                    for (int w = 0; w < T / 32; w++) a += sh.warp[w];
+                    sh.best_above = a;
+                }
+            }
+            cluster_sync();
+            const uint32_t v = ld_cluster_u32(map_to_rank(smem_u32(&sh.best), 0));
+            above = ld_cluster_u64(map_to_rank(smem_u32(&sh.best_above), 0));
+            cluster_sync();  // rank 0 may begin another search
+            return v;
+        }
+        // many entries within one step (equal ones, or a high temperature): bisection over their order
+        uint32_t lo = ~cluster_max(~low), hi = cluster_max(high);  // lo <= the end <= hi
+        above = before;
+        while (lo < hi) {
+            const uint32_t mid = lo + ((hi - lo) >> 1);
+            u64 a = 0;
+            for (int i = threadIdx.x; i < cnt; i += T) {
+                const float x = xs[i], k = key(x);
+                if (k < kSrSteps && (int)k == prefix && order_bits(x) > mid) a += weight(x, counting);
+            }
+            a = before + cluster_sum(a);
+            if (a < target) {
+                hi = mid;
+                above = a;
+            } else {
+                lo = mid + 1;
+            }
+        }
+        return lo;
+    }
+    static __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+        uint32_t v;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+        return v;
+    }
+};
+
+template <class E>
+__device__ __forceinline__ float as_logit(E v) { return Elem<E>::to(v) + 0.0f; }  // -0 counts as 0
+
+template <class E, int T>
+__global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ SampleRowsShared<T> sh;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int rank = (int)cluster_ctarank(), nr = (int)cluster_nctarank();
+    const int row = blockIdx.x / nr;
+    const int lo = min(p.n, rank * p.chunk), cnt = min(p.n, lo + p.chunk) - lo;
+    u64* hist = reinterpret_cast<u64*>(smem);
+    const E* src = static_cast<const E*>(p.x) + (long long)row * p.stride + lo;
+    constexpr int kV = 16 / sizeof(E);
+    const int off = (int)((uintptr_t)src & 15) / (int)sizeof(E);  // the slice keeps the row's alignment
+    float* xs = reinterpret_cast<float*>(smem + sizeof(u64) * kSrBins * T) + off;
+
+    // ---- the slice; its largest entry, the first of its equals; NaN ------------
+    const int head = min(cnt, (kV - off) % kV), vecs = (cnt - head) / kV;
+    for (int i = threadIdx.x; i < head; i += T) xs[i] = as_logit(src[i]);
+    for (int i = head + vecs * kV + threadIdx.x; i < cnt; i += T) xs[i] = as_logit(src[i]);
+    const uint4* vsrc = reinterpret_cast<const uint4*>(src + head);
+    auto put = [&](int v, uint4 w) {
+        float4* d = reinterpret_cast<float4*>(xs + head + v * kV);
+        if constexpr (sizeof(E) == 4) {
+            d[0] = make_float4(__uint_as_float(w.x) + 0.0f, __uint_as_float(w.y) + 0.0f, __uint_as_float(w.z) + 0.0f,
+                               __uint_as_float(w.w) + 0.0f);
+        } else {
+            const float2 a = unpack2<E>(w.x), b = unpack2<E>(w.y), c = unpack2<E>(w.z), e = unpack2<E>(w.w);
+            d[0] = make_float4(a.x + 0.0f, a.y + 0.0f, b.x + 0.0f, b.y + 0.0f);
+            d[1] = make_float4(c.x + 0.0f, c.y + 0.0f, e.x + 0.0f, e.y + 0.0f);
+        }
+    };
+    int v = threadIdx.x;
+    for (; v + 3 * T < vecs; v += 4 * T) {  // four loads in flight
+        uint4 w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = __ldg(vsrc + v + j * T);
+#pragma unroll
+        for (int j = 0; j < 4; j++) put(v + j * T, w[j]);
+    }
+    for (; v < vecs; v += T) put(v, __ldg(vsrc + v));
+    cluster_sync();  // the slice is there, and the cluster's other CTAs run: their shared memory can be written
+    uint32_t best = 0, at = 0x7fffffffu;  // order bits (of a NaN: all ones), index in the row
+    for (int i = threadIdx.x; i < cnt; i += T) {
+        const float x = xs[i];
+        const uint32_t ob = x != x ? 0xffffffffu : order_bits(x);
+        if (ob > best) {
+            best = ob;
+            at = lo + i;
+        }
+    }
+    SampleRow<T> s{sh, hist, xs, cnt, rank, nr, 0, 0, 0.0f, 0.0f, 0.0};
+    const uint32_t top_bits = s.cluster_max(best);
+    const float temp = p.temperature ? p.temperature[row] : 1.0f;
+    if (!(temp > 0.0f)) {
+        const uint32_t first = ~s.cluster_max(best == top_bits ? ~at : 0u);
+        if (rank == 0 && threadIdx.x == 0) {
+            p.tok[row] = (int)first;
+            if (p.logp) p.logp[row] = 0.0f;
+        }
+        return;
+    }
+    const float top = top_bits == 0xffffffffu ? NAN : order_value(top_bits);
+    if (!(fabsf(top) < INFINITY)) {  // NaN, +inf, or nothing above -inf
+        if (rank == 0 && threadIdx.x == 0) {
+            p.tok[row] = p.n - 1;
+            if (p.logp) p.logp[row] = NAN;
+            if (p.status) atomicOr(p.status, 8);
+        }
+        return;
+    }
+    s.top = top;
+    s.oct = 1.4426950408889634074 / (double)temp;
+    s.steps = fminf((float)(s.oct * (kSrSteps / kSrOctaves)), 1e30f);
+
+    // ---- where the filters end ---------------------------------------------------
+    uint32_t floor_key = 0;   // entries below are out
+    int ties = 0x7fffffff;    // of the entries equal to tie_key, how many stay
+    uint32_t tie_key = 0;
+    const int k = p.top_k ? p.top_k[row] : 0;
+    const float tp = p.top_p ? p.top_p[row] : 1.0f;
+    const float mp = p.min_p ? p.min_p[row] : 0.0f;
+    if (k > 0 && k < p.n) {
+        u64 above;
+        floor_key = tie_key = s.find_end(true, (u64)k, 0, above);
+        ties = k - (int)above;
+    }
+    if (tp < 1.0f) {
+        u64 m = 0;
+        for (int i = threadIdx.x; i < cnt; i += T) {
+            const float x = xs[i];
+            const uint32_t ob = order_bits(x);
+            if (s.has_mass(x) && (ob > tie_key || (ob == tie_key && ties == 0x7fffffff))) m += s.mass(x);
+        }
+        m = s.cluster_sum(m);
+        if (ties != 0x7fffffff) {  // those that stay of the entries equal to the last
+            u64 equal = 0;
+            for (int i = threadIdx.x; i < cnt; i += T) equal += order_bits(xs[i]) == tie_key ? 1 : 0;
+            equal = s.cluster_sum(equal);
+            if ((u64)ties > equal) ties = (int)equal;  // all entries with mass stay
+            m += (u64)ties * s.mass(order_value(tie_key));
+        }
+        const double want = ceil((double)tp * (double)m);
+        u64 above;
+        floor_key = s.find_end(false, want >= 1.0 ? (u64)want : 1, floor_key, above);
+    }
+    const double oct_max = mp > 0.0f ? -log2((double)fminf(mp, 1.0f)) : 1e300;
+
+    // ---- the draw: runs of the slice in index order, one to a thread -----------
+    const int E_ = ((cnt + T - 1) / T) | 1;  // odd: no bank twice in a warp
+    const int a = min(cnt, (int)threadIdx.x * E_), b = min(cnt, a + E_);
+    int tie_before = 0;  // entries equal to tie_key before this run
+    if (ties != 0x7fffffff && floor_key == tie_key) {
+        u64 mine = 0, lower;
+        for (int i = a; i < b; i++) mine += order_bits(xs[i]) == tie_key ? 1 : 0;
+        s.cluster_sum(mine, &lower);
+        u64 inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
+            if ((threadIdx.x & 31) >= o) inc += y;
+        }
+        __syncthreads();
+        if ((threadIdx.x & 31) == 31) sh.warp[threadIdx.x >> 5] = inc;
+        __syncthreads();
+        u64 before = lower + inc - mine;
+        for (int w = 0; w < (int)(threadIdx.x >> 5); w++) before += sh.warp[w];
+        tie_before = (int)before;
+    }
+    auto kept = [&](int i, int& seen) -> u64 {  // the mass of entry i if it stays
+        const float x = xs[i];
+        const uint32_t ob = order_bits(x);
+        if (ob < floor_key || !s.has_mass(x)) return 0;
+        if (ob == tie_key && ties != 0x7fffffff && seen++ >= ties) return 0;
+        if (((double)top - (double)x) * s.oct > oct_max) return 0;
+        return s.mass(x);
+    };
+    u64 mine = 0;
+    int seen = tie_before;
+    for (int i = a; i < b; i++) mine += kept(i, seen);
+    u64 lower;
+    const u64 total = s.cluster_sum(mine, &lower);
+    u64 inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
+        if ((threadIdx.x & 31) >= o) inc += y;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 31) sh.warp[threadIdx.x >> 5] = inc;
+    __syncthreads();
+    u64 c = lower + inc - mine;
+    for (int w = 0; w < (int)(threadIdx.x >> 5); w++) c += sh.warp[w];
+    const double u = p.u[row];
+    const double want = (u > 0.0 ? u : 0.0) * (double)total;
+    const u64 goal = want >= (double)total ? total - 1 : (u64)want;
+    if (goal >= c && goal < c + mine) {  // one thread of the cluster
+        seen = tie_before;
+        for (int i = a; i < b; i++) {
+            c += kept(i, seen);
+            if (c > goal) {
+                p.tok[row] = lo + i;
+                if (p.logp)
+                    p.logp[row] = (float)(-((double)top - (double)xs[i]) * s.oct * 0.6931471805599453094 -
+                                          log((double)total / 17592186044416.0));
+                break;
+            }
+        }
+    }
+}
+
+template <class E, int T>
+static int launch_sample_rows(const SampleRowsParams& p, int rows, int cluster, size_t smem, cudaStream_t st) {
+    auto kern = sample_rows_kernel<E, T>;
+    static PerDeviceOnce once;
+    if (smem_opt_in(once, kern, 216 * 1024) != cudaSuccess) return HQ4_ERR_LAUNCH;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)rows * cluster);
+    lc.blockDim = dim3(T);
+    lc.dynamicSmemBytes = smem;
+    lc.stream = st;
+    lc.attrs = attr;
+    lc.numAttrs = 2;
+    return cudaLaunchKernelEx(&lc, kern, p) == cudaSuccess ? HQ4_OK : HQ4_ERR_LAUNCH;
+}
+
+template <class E>
+static int sample_rows(SampleRowsParams p, int rows, cudaStream_t st) {
+    int cluster = kSrMaxCluster;
+    while (cluster > 1 && p.n / cluster < 2048) cluster >>= 1;
+    p.chunk = (p.n + cluster - 1) / cluster;
+    const size_t slice = (size_t)(p.chunk + 16) * sizeof(float);
+    if (slice + sizeof(u64) * kSrBins * 512 <= 216 * 1024)
+        return launch_sample_rows<E, 512>(p, rows, cluster, slice + sizeof(u64) * kSrBins * 512, st);
+    return launch_sample_rows<E, 256>(p, rows, cluster, slice + sizeof(u64) * kSrBins * 256, st);
+}
+
+}  // namespace hq4
+
+using namespace hq4;
+
+extern "C" int hq4_sample_rows(const void* logits, int act_type, int n_rows, int n, long long row_stride,
+                               const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                               const double* u, int* tok, float* logprob, void* stream) {
+    if (n_rows <= 0 || n <= 0 || n > kSrMaxCluster * kSrMaxSlice || row_stride < n || !logits || !u || !tok)
+        return HQ4_ERR_SHAPE;
+    if (n_rows > (1 << 27)) return HQ4_ERR_SHAPE;
+    if (act_type != HQ4_F32 && act_type != HQ4_BF16 && act_type != HQ4_F16) return HQ4_ERR_SHAPE;
+    if (((uintptr_t)logits & (act_type == HQ4_F32 ? 3 : 1)) || ((uintptr_t)u & 7) ||
+        (((uintptr_t)temperature | (uintptr_t)top_k | (uintptr_t)top_p | (uintptr_t)min_p | (uintptr_t)tok |
+          (uintptr_t)logprob) & 3))
+        return HQ4_ERR_ALIGN;
+    if (int rc = check_device_cap()) return rc;
+    SampleRowsParams p = {};
+    p.x = logits;
+    p.stride = row_stride;
+    p.n = n;
+    p.temperature = temperature;
+    p.top_k = top_k;
+    p.top_p = top_p;
+    p.min_p = min_p;
+    p.u = u;
+    p.tok = tok;
+    p.logp = logprob;
+    p.status = status_word();
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return act_type == HQ4_F32 ? sample_rows<float>(p, n_rows, st)
+         : act_type == HQ4_BF16 ? sample_rows<__nv_bfloat16>(p, n_rows, st) : sample_rows<__half>(p, n_rows, st);
+}

@@ -39,7 +39,8 @@ int hq4_version(void);
  * that kernel's output is not valid; bit 1 when hq4_embed_f16 met a token id
  * outside [0, vocab) -- that row was written as zeros; bit 2 when
  * hq4_gemm_w4a16 met an activation outside fp16 range; bit 3 when hq4_sample
- * met logits without a usable distribution (NaN).  Non-zero `clear`
+ * met logits without a usable distribution (NaN); bit 4 when a paged call met
+ * an entry without a page (or a position outside the rotation tables).  Non-zero `clear`
  * resets it.  No counterpart in the reference: its CPU kernel cannot stall,
  * its table indexing raises IndexError on a bad id, and it computes in fp32. */
 int hq4_device_status(int clear);
@@ -276,6 +277,105 @@ int hq4_pick_token_next(const int* pairs, int world, int* tok, int* history, int
 
 /* *pos += delta on the device (advances the decode position inside a graph). */
 int hq4_advance_position(int* pos, int delta, void* stream);
+
+/* ---- many streams over a paged cache ---------------------------------------
+ * Key/value caches of pages [n_pages][n_kv][page_size][head_dim] in bf16 or
+ * fp16, shared by sequences of any length, and the batch sampler.  No
+ * reference counterpart (the reference keeps one growing fp32 cache to a
+ * request, hetero/cpu_model.py:207-230, and serves one request at a time);
+ * hq4_qkv_rope, hq4_attention and hq4_sample are the one-request forms.
+ *
+ * A batch is n_seqs sequences: sequence s owns rows [cu_rows[s], cu_rows[s+1])
+ * of the n_rows rows of q, k and v, its cache holds lens[s] entries before
+ * them, and its i-th row is entry lens[s] + i.  Entry e lies at place
+ * e % page_size of page pages[s][e / page_size]; pages is
+ * [n_seqs][pages_per_seq].  cu_rows ([n_seqs + 1], ascending), lens and pages
+ * are device ints, so a captured step can be replayed while the sequences
+ * grow.  Rows outside every sequence are left alone; sequences without rows
+ * are allowed.  An entry without a page in [0, n_pages) is not written and not
+ * attended to, and sets status bit 4.  Two sequences may share pages that
+ * neither of them writes.
+ *
+ * Types: activations are HQ4_F32, or the cache's type HQ4_BF16 / HQ4_F16;
+ * outputs have the activations' type, sums and softmax are fp32.  n_heads a
+ * multiple of n_kv, head_dim a multiple of 32 up to 256, page_size a power of
+ * two from 8 to 4096.  page_stride: elements from a page to the next (at least
+ * n_kv * page_size * head_dim, a multiple of 8), so that the two caches can be
+ * views of one tensor.  q_stride, k_stride, v_stride: elements from a row to
+ * the next (16-byte multiples), so that they can be views of one projection's
+ * output.  Pointers are 16-byte aligned, ints 4-byte. */
+#define HQ4_F32 0
+#define HQ4_BF16 1
+#define HQ4_F16 2
+
+/* Appends the rows of k (rotated) and v to their pages and writes the rotated
+ * queries to q_out [n_rows][n_heads][head_dim] (which must not overlap q).
+ * Rotation as hq4_qkv_rope: half-split, cos/sin tables [max_pos][head_dim/2];
+ * a row's position is its entry's number, or positions[row] where positions
+ * is not NULL (the nodes of a drafted tree: entries one after another,
+ * positions by depth).  q_norm / k_norm ([head_dim], each may be NULL): an RMS
+ * norm of each query / key head before the rotation, x / sqrt(mean(x^2) + eps)
+ * * w.  A row without a page, or whose position is outside [0, max_pos), writes
+ * nothing and sets status bit 4. */
+int hq4_paged_append(const void* q, const void* k, const void* v, int act_type, int n_rows, int n_heads,
+                     int n_kv, int head_dim, long long q_stride, long long k_stride, long long v_stride,
+                     const float* q_norm, const float* k_norm, float eps, const int* cu_rows, const int* lens,
+                     int n_seqs, const int* positions, const float* rope_cos, const float* rope_sin, int max_pos,
+                     const int* pages, int pages_per_seq, void* k_cache, void* v_cache, int cache_type, int n_pages,
+                     int page_size, long long page_stride, void* q_out, void* stream);
+
+/* Grouped-query attention of the batch's rows over the cache: row i of
+ * sequence s attends to entries [0, lens[s] + i], its own among them
+ * (hq4_paged_append first).  out [n_rows][n_heads][head_dim]; a row that sees
+ * nothing is zeros.  What lies in entries that a row does not see (stale
+ * pages, NaN, infinities) does not reach it.  The workspace
+ * (hq4_paged_attention_workspace_bytes, 128-byte aligned; may be NULL where
+ * that is 0) is written and read by one call: calls that can run at the same
+ * time must not share it.  Deterministic; allocates nothing. */
+int hq4_paged_attention(const void* q, int act_type, int n_rows, int n_heads, int n_kv, int head_dim,
+                        long long q_stride, const int* cu_rows, const int* lens, int n_seqs, const int* pages,
+                        int pages_per_seq, const void* k_cache, const void* v_cache, int cache_type, int n_pages,
+                        int page_size, long long page_stride, float scale, void* out, void* workspace,
+                        long long workspace_bytes, void* stream);
+
+/* The same for trees of drafted tokens: a sequence's rows are the nodes of its
+ * tree, appended as entries lens[s] + 0, 1, ...; row i sees all entries before
+ * lens[s], and entry lens[s] + j where bit j % 32 of word j / 32 of its row of
+ * tree_mask [n_rows][mask_words] is set (its ancestors and itself).  Bits of
+ * nodes that the sequence does not have are ignored; nodes beyond the mask's
+ * words are not seen. */
+int hq4_tree_attention(const void* q, int act_type, int n_rows, int n_heads, int n_kv, int head_dim,
+                       long long q_stride, const int* cu_rows, const int* lens, int n_seqs, const int* pages,
+                       int pages_per_seq, const void* k_cache, const void* v_cache, int cache_type, int n_pages,
+                       int page_size, long long page_stride, const uint32_t* tree_mask, int mask_words, float scale,
+                       void* out, void* workspace, long long workspace_bytes, void* stream);
+
+/* Workspace bytes of hq4_paged_attention and hq4_tree_attention for a shape on
+ * the current device (host only; -1 for a bad shape). */
+long long hq4_paged_attention_workspace_bytes(int act_type, int n_rows, int n_heads, int n_kv, int head_dim,
+                                              int n_seqs, int pages_per_seq, int page_size);
+
+/* A token for each of n_rows rows of logits [n_rows][n] (act_type HQ4_F32,
+ * HQ4_BF16 or HQ4_F16; row_stride elements from a row to the next): the batch
+ * form of hq4_sample with top-k and min-p.  Each parameter is a device array
+ * of n_rows values or NULL (off).  With z = x / temperature, the entries in
+ * descending order, equal ones by index:
+ *   top_k  > 0: the first top_k of them stay;
+ *   top_p  < 1: of those, each whose strictly larger ones hold less than top_p
+ *               of their mass (the most likely ones always stay);
+ *   min_p  > 0: of those, each with at least min_p (at most 1) times the
+ *               largest probability.
+ * The token is the first entry, by index, at which the cumulative mass of
+ * those that stay exceeds u[row] of their whole (u in [0, 1), as hq4_sample).
+ * temperature NULL: 1; a row's temperature <= 0: its greedy token, as
+ * hq4_argmax.  logprob (may be NULL): the log of the token's probability among
+ * those that stay (0 for a greedy one).  Masses are 44-bit fixed point, so the
+ * draw does not depend on an order of summation.  -inf logits have no mass; a
+ * row with a NaN, a +inf or -inf alone gets token n - 1 and log probability
+ * NaN, and sets status bit 3.  n up to 8 x 36864. */
+int hq4_sample_rows(const void* logits, int act_type, int n_rows, int n, long long row_stride,
+                    const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                    const double* u, int* tok, float* logprob, void* stream);
 
 /* ---- persistent decode ----------------------------------------------------
  * One token through n_layers qwen2 decoder layers (hetero/cpu_model.py:280-310
