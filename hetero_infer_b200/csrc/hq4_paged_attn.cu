@@ -12,25 +12,33 @@ int paged_batch(PagedBatch& b, int n_rows, int n_heads, int n_kv, int head_dim, 
                 int cache_type, int act_type, int n_pages, int page_size, long long page_stride);
 int paged_rows_bf16(bool f32, const PagedAttnParams& p, const PaPlan& pl, cudaStream_t st);
 int paged_rows_f16(bool f32, const PagedAttnParams& p, const PaPlan& pl, cudaStream_t st);
+int paged_tc_bf16(const PagedAttnParams& p, const PaPlan& pl, cudaStream_t st);
+int paged_tc_f16(const PagedAttnParams& p, const PaPlan& pl, cudaStream_t st);
 
-// Tiles of 8, 16 or 32 rows (16 at most for wide heads, whose outputs fill the
-// registers), by the rows that a sequence has on average; split
-// over keys when a sequence may be longer than kPaWhole entries (shorter ones
-// are a CTA's work whole, and need no second kernel).
+// More than kPaTcRows rows to a sequence and key/value head on average: the
+// tensor-memory kernel, whose tile of 128 rows is then worth filling (16-bit
+// activations only). Else tiles of 8, 16 or 32 rows (16 at most for wide
+// heads, whose outputs fill the registers). Split over keys when a sequence
+// may be longer than kPaWhole entries (shorter ones are a CTA's work whole,
+// and need no second kernel).
+constexpr int kPaTcRows = 32;
 constexpr int kPaWhole = 512;
-static PaPlan pa_plan(int n_rows, int n_heads, int n_kv, int head_dim, int n_seqs, int pages_per_seq, int page_size,
-                      int sms) {
+static PaPlan pa_plan(int act_type, int n_rows, int n_heads, int n_kv, int head_dim, int n_seqs, int pages_per_seq,
+                      int page_size, int sms) {
     PaPlan r;
     const long long group = n_heads / n_kv;
     const long long avg = ((long long)n_rows + n_seqs - 1) / n_seqs * group;
+    r.tc = act_type != HQ4_F32 && avg > kPaTcRows;
     r.dim = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
     r.nt = avg <= 8 ? 1 : avg <= 16 || r.dim == 256 ? 2 : 4;
+    const int rows = !r.tc ? 8 * r.nt : r.dim == 256 ? 128 : 256;
+    const int keys = !r.tc ? kPaKeys : r.dim == 256 ? 64 : 128;
+    const int per_sm = r.tc || r.dim == 256 ? 1 : r.dim == 128 ? 2 : 3;
     const long long cap = (long long)pages_per_seq * page_size;
-    const long long items = ((long long)n_rows * group / (8 * r.nt) + n_seqs) * n_kv;
+    const long long items = ((long long)n_rows * group / rows + n_seqs) * n_kv;  // at most
     r.split = cap > kPaWhole;
-    const long long units = r.split ? items * ((cap + kPaKeys - 1) / kPaKeys) : items;
-    r.ctas = (int)std::min<long long>(units, (long long)sms * (r.dim == 64 ? 3 : r.dim == 128 ? 2 : 1));
-    const int rows = 8 * r.nt;
+    const long long units = r.split ? items * ((cap + keys - 1) / keys) : items;
+    r.ctas = (int)std::min<long long>(units, (long long)sms * per_sm);
     r.ws = r.split ? (long long)r.ctas * (sizeof(PagedItem) + 2ll * rows * (sizeof(float2) + r.dim * sizeof(float))) : 0;
     return r;
 }
@@ -64,7 +72,7 @@ static int paged_attention(const void* q, int act_type, int n_rows, int n_heads,
     p.b.status = status_word();
     const int sms = sm_count();
     if (!p.b.status || sms <= 0) return HQ4_ERR_LAUNCH;
-    const PaPlan pl = pa_plan(n_rows, n_heads, n_kv, head_dim, n_seqs, pages_per_seq, page_size, sms);
+    const PaPlan pl = pa_plan(act_type, n_rows, n_heads, n_kv, head_dim, n_seqs, pages_per_seq, page_size, sms);
     if (pl.ws) {
         if (!workspace || workspace_bytes < pl.ws) return HQ4_ERR_SHAPE;
         if ((uintptr_t)workspace & 127) return HQ4_ERR_ALIGN;
@@ -84,6 +92,7 @@ static int paged_attention(const void* q, int act_type, int n_rows, int n_heads,
     p.split = pl.split;
     p.ws = pl.ws ? workspace : nullptr;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (pl.tc) return cache_type == HQ4_BF16 ? paged_tc_bf16(p, pl, st) : paged_tc_f16(p, pl, st);
     return cache_type == HQ4_BF16 ? paged_rows_bf16(act_type == HQ4_F32, p, pl, st)
                                   : paged_rows_f16(act_type == HQ4_F32, p, pl, st);
 }
@@ -100,7 +109,7 @@ extern "C" long long hq4_paged_attention_workspace_bytes(int act_type, int n_row
         return -1;
     const int sms = sm_count();
     if (sms <= 0) return -1;
-    return pa_plan(n_rows, n_heads, n_kv, head_dim, n_seqs, pages_per_seq, page_size, sms).ws;
+    return pa_plan(act_type, n_rows, n_heads, n_kv, head_dim, n_seqs, pages_per_seq, page_size, sms).ws;
 }
 
 extern "C" int hq4_paged_attention(const void* q, int act_type, int n_rows, int n_heads, int n_kv, int head_dim,

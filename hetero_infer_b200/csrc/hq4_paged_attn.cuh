@@ -250,7 +250,7 @@ static_assert(sizeof(PagedItem) % 16 == 0, "the pieces behind the items keep the
 // does in that item, joins the item's pieces; one warp to a row.
 constexpr int kCombineWarps = 4;
 template <class A, class C, int kRows, int kDim>
-__global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const PagedAttnParams p, int ctas) {
+__global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const __grid_constant__ PagedAttnParams p, int ctas) {
     pdl_launch_dependents();
     pdl_wait();
     const PagedWs<kRows, kDim> ws(p.ws, ctas);
@@ -303,5 +303,14 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
         }
     if (__any_sync(0xffffffffu, bad)) paged_slow_row<A, C>(p, it, row);
 }
+
+// How a call is run (host).
+struct PaPlan {
+    int tc;     // tensor-memory kernel (hq4_paged_tc.cuh), else the warp-level one (hq4_paged_rows.cuh)
+    int nt;     // 8-row tiles of the latter
+    int dim;    // head_dim rounded up to what the kernels are built for
+    int ctas, split;
+    long long ws;
+};
 
 }  // namespace hq4

@@ -76,7 +76,7 @@ template <int kDim>
 __device__ __forceinline__ int tile_at(int r, int c) { return r * (kDim * 2) + ((c ^ (r & 7)) << 4); }
 
 template <class A, class C, int kDim, int NT>
-__global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
     constexpr int kRows = 8 * NT, kTerms = pa_terms<A, C>(), kStages = PaShape<kDim>::kStages;
     constexpr int kTile = PaShape<kDim>::kTile, kRing = PaShape<kDim>::kRing;
     constexpr int kChunks = kDim / 8, kOs = kDim + 4;
@@ -403,11 +403,6 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const PagedAttnP
 }
 
 // ---- launch ------------------------------------------------------------------
-
-struct PaPlan {
-    int nt, dim, ctas, split;
-    long long ws;
-};
 
 static inline cudaError_t launch_pdl_kernel(const void* fn, dim3 grid, dim3 block, size_t smem, cudaStream_t st, void** args) {
     cudaLaunchAttribute attr[1];
