@@ -126,4 +126,10 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
                                               pack2<T>(v[6], v[7]));
 }
 
+__device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
+template <class T>
+__device__ __forceinline__ void store4(T* p, float4 v) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+}
+
 }  // namespace hq4

@@ -16,6 +16,14 @@
 
 namespace hq4 {
 
+// 16 bytes to shared memory; zeros where `on` is not set (nothing is read then).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct PagedAttnParams {
@@ -247,61 +255,74 @@ struct PagedWs {
 static_assert(sizeof(PagedItem) % 16 == 0, "the pieces behind the items keep their alignment");
 
 // CTA (c, y): if part c begins inside an item, and c is the first part that
-// does in that item, joins the item's pieces; one warp to a row.
+// does in that item, joins kCombineRows rows of the item's pieces in key order;
+// a warp takes a row, a lane 4 consecutive values of each 128.
 constexpr int kCombineWarps = 4;
+constexpr int kCombineRows = 8;  // of a CTA
 template <class A, class C, int kRows, int kDim>
-__global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const __grid_constant__ PagedAttnParams p, int ctas) {
+__global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const __grid_constant__ PagedAttnParams p,
+                                                                           int ctas) {
     pdl_launch_dependents();
     pdl_wait();
     const PagedWs<kRows, kDim> ws(p.ws, ctas);
+    const int c = blockIdx.x + 1;
     const long long total = ws.info[0].total;  // CTA 0 has work whenever there is any row
     const long long parts = min((long long)ctas, total);
-    const int c = blockIdx.x + 1;
     if (c >= parts) return;
     const PagedItem it = ws.info[c];
     const long long start = c * total / parts, before = (c - 1) * total / parts;
     if (it.first == start || it.first < before) return;
-    const int r = blockIdx.y * kCombineWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int row = it.rt * kRows + r;
-    if (r >= kRows || row >= it.n_tok * p.group) return;
+    const int rows = min(kRows, it.n_tok * p.group - it.rt * kRows);
     const int first_piece = 2 * (c - 1) + (it.first == before ? 0 : 1);
-    int n = 1;  // pieces: that one, then the first ones of parts c, c + 1, ...
-    const long long stop = it.first + it.weight;
-    while (c - 1 + n < parts && (c - 1 + n) * total / parts < stop) n++;
-    auto piece = [&](int i) { return i == 0 ? first_piece : 2 * (c - 1 + i); };
-    float m = -INFINITY;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, ws.ml[(size_t)piece(i) * kRows + r].x);
+    // pieces: that one, then the first ones of parts c, c + 1, ... up to the one with the item's last unit
+    const long long last = it.first + it.weight - 1;
+    long long owner = last * parts / total;  // or the one after it, by rounding
+    while ((owner + 1) * total / parts <= last) owner++;
+    const int n = (int)(owner - (c - 1)) + 1;
+    const int lane = threadIdx.x & 31, D = p.head_dim;
+    constexpr int kPer = (kDim + 127) / 128;
+    for (int r = blockIdx.y * kCombineRows + (threadIdx.x >> 5); r < min(rows, (int)(blockIdx.y + 1) * kCombineRows);
+         r += kCombineWarps) {
+        auto at = [&](int i) { return (size_t)(i == 0 ? first_piece : 2 * (c - 1 + i)) * kRows + r; };
+        float m = -INFINITY;
+        for (int i = lane; i < n; i += 32) m = fmaxf(m, ws.ml[at(i)].x);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float mu = m == -INFINITY ? 0.0f : m;
-    constexpr int kPer = kDim / 32;
-    float acc[kPer], l = 0.0f;
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float mu = m == -INFINITY ? 0.0f : m;
+        float4 acc[kPer];
+        float l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kPer; i++) acc[i] = 0.0f;
-    const int D = p.head_dim;
+        for (int j = 0; j < kPer; j++) acc[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-    for (int i = 0; i < n; i++) {
-        const size_t at = (size_t)piece(i) * kRows + r;
-        const float2 ml = ws.ml[at];
-        const float w = exp2f(ml.x - mu);
-        l = fmaf(ml.y, w, l);
-        const float* o = ws.o + at * kDim;
+        for (int i = 0; i < n; i++) {
+            const float2 ml = ws.ml[at(i)];
+            const float w = exp2f(ml.x - mu);
+            l = fmaf(ml.y, w, l);
+            const float* o = ws.o + at(i) * kDim;
+#pragma unroll
+            for (int j = 0; j < kPer; j++)
+                if (lane * 4 + 128 * j < D) {
+                    const float4 v = *reinterpret_cast<const float4*>(o + lane * 4 + 128 * j);
+                    acc[j].x = fmaf(v.x, w, acc[j].x);
+                    acc[j].y = fmaf(v.y, w, acc[j].y);
+                    acc[j].z = fmaf(v.z, w, acc[j].z);
+                    acc[j].w = fmaf(v.w, w, acc[j].w);
+                }
+        }
+        const int row = it.rt * kRows + r, tok = row / p.group, head = it.h * p.group + row % p.group;
+        A* out = static_cast<A*>(p.out) + ((long long)(it.row0 + tok) * p.n_heads + head) * D;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        bool bad = false;
 #pragma unroll
         for (int j = 0; j < kPer; j++)
-            if (lane + 32 * j < D) acc[j] = fmaf(o[lane + 32 * j], w, acc[j]);
+            if (lane * 4 + 128 * j < D) {
+                const float4 y = l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                           : make_float4(acc[j].x * inv, acc[j].y * inv, acc[j].z * inv, acc[j].w * inv);
+                bad |= y.x != y.x || y.y != y.y || y.z != y.z || y.w != y.w;
+                store4(out + lane * 4 + 128 * j, y);
+            }
+        if (__any_sync(0xffffffffu, bad)) paged_slow_row<A, C>(p, it, row);
     }
-    const int tok = row / p.group, head = it.h * p.group + row % p.group;
-    A* out = static_cast<A*>(p.out) + ((long long)(it.row0 + tok) * p.n_heads + head) * D;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < kPer; j++)
-        if (lane + 32 * j < D) {
-            const float y = l == 0.0f ? 0.0f : acc[j] * inv;
-            bad |= y != y;
-            out[lane + 32 * j] = Elem<A>::from(y);
-        }
-    if (__any_sync(0xffffffffu, bad)) paged_slow_row<A, C>(p, it, row);
 }
 
 // How a call is run (host).

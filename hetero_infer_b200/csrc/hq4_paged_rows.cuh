@@ -35,12 +35,6 @@ constexpr int pa_terms() { return sizeof(A) == 2 ? 1 : Elem<C>::code == HQ4_BF16
 template <int kDim, int kRows, int kTerms>
 constexpr int pa_smem() { return kPaWarps * PaShape<kDim>::kRing + kTerms * kRows * kDim * 2; }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -431,7 +425,7 @@ static int launch_pa(PagedAttnParams p, const PaPlan& pl, cudaStream_t st) {
     int ctas = pl.ctas;
     void* cargs[] = {&p, &ctas};
     return launch_pdl_kernel((const void*)paged_combine_kernel<A, C, 8 * NT, kDim>,
-                             dim3(pl.ctas - 1, (8 * NT + kCombineWarps - 1) / kCombineWarps), dim3(kCombineWarps * 32),
+                             dim3(pl.ctas - 1, (8 * NT + kCombineRows - 1) / kCombineRows), dim3(kCombineWarps * 32),
                              0, st, cargs) == cudaSuccess
                ? HQ4_OK
                : HQ4_ERR_LAUNCH;

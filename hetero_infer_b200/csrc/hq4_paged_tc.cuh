@@ -45,14 +45,24 @@ struct PtShape {
     static constexpr int kOCol = kGroups * kKeys;         // TMEM column of the first group's O
 };
 
-// D[tmem] (+)= A[smem] . B[smem]^T, 16-bit operands, fp32 accumulator.
-__device__ __forceinline__ void umma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
-    const uint32_t z = 0;
+// D[tmem] (+)= A . B^T, 16-bit operands, fp32 accumulator; A in shared memory or
+// in TMEM.  The whole warp comes here and `issue` picks the lane: computing the
+// operands outside of any branch lets them be in uniform registers, where a
+// loop within a one-lane branch took 128 cycles to an instruction.
+__device__ __forceinline__ void pt_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate, uint32_t issue) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(z), "r"(z), "r"(z), "r"(z)
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issue)
+        : "memory");
+}
+__device__ __forceinline__ void pt_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate, uint32_t issue) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issue)
         : "memory");
 }
 // Descriptor of a tile whose rows are the contraction's (values: keys x dims,
@@ -82,6 +92,45 @@ __device__ __forceinline__ float pt_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two fp32 values to an instruction.
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 pair(float a, float b) {
+    u64 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ u64 pair(uint32_t a, uint32_t b) {
+    u64 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ float2 unpair(u64 v) {
+    float2 d;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+    return d;
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+    u64 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+    u64 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// -inf where a bit of `see` is not set.
+__device__ __forceinline__ void pt_hide(uint32_t (&s)[32], uint32_t see) {
+#pragma unroll
+    for (int j = 0; j < 32; j++)
+        if (!(see >> j & 1)) s[j] = 0xff800000u;
 }
 
 // Which of the 32 entries from e0 on token tok of the item sees, a bit each.
@@ -164,10 +213,11 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
     pdl_launch_dependents();
     const int D = p.head_dim, ksteps = D >> 4;
     bool fail = false;
-    // A warp's wait, which ends: after its limit, or once another warp's has run out.
+    // A warp's wait, which ends: after so many tries (each may sleep up to a millisecond; reading a
+    // timer instead costs more than most waits), or once another warp's has run out.
     auto wait = [&](uint32_t bar, uint32_t parity) -> bool {
         for (int i = 0; i < 10; i++) {
-            const bool ok = mbar_wait_ns(bar, parity & 1u, kPtWaitNs / 10);
+            const bool ok = mbar_wait_tries(bar, parity & 1u, 1000000u, 1000);
             if (__all_sync(0xffffffffu, ok)) return true;
             if (__any_sync(0xffffffffu, s_dead)) break;
         }
@@ -190,24 +240,30 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_col = tmem + lanes + g * kKeys, o_col = tmem + lanes + S::kOCol + g * kDim;
         const int in_group = (warp & 3) * 32 + lane;
-        auto load_q = [&]() {  // the group's rows of item `it`, a warp its own 32
-            const int chunks = D >> 3;
-            for (int i = lane; i < 32 * chunks; i += 32) {
-                const int r = i / chunks, c = i - r * chunks;
-                const int gr = (warp & 3) * 32 + r, row = it.rt * kRows + g * 128 + gr;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (row < it.n_tok * p.group) {
-                    const C* src = static_cast<const C*>(p.q) + (long long)(it.row0 + row / p.group) * p.q_stride +
-                                   ((long long)it.h * p.group + row % p.group) * D;
-                    v = __ldg(reinterpret_cast<const uint4*>(src) + c);
-                    if (p.scale_log2 < 0.0f) {  // a negative scale: the rows' signs instead
-                        v.x ^= 0x80008000u;
-                        v.y ^= 0x80008000u;
-                        v.z ^= 0x80008000u;
-                        v.w ^= 0x80008000u;
-                    }
+        auto load_q = [&]() {  // the group's rows of item `it`, a warp its own 32, all copies in flight at once
+            const int row = it.rt * kRows + g * 128 + in_group;
+            const bool there = row < it.n_tok * p.group;
+            const C* src = static_cast<const C*>(p.q);
+            if (there)
+                src += (long long)(it.row0 + row / p.group) * p.q_stride + ((long long)it.h * p.group + row % p.group) * D;
+            const uint32_t q0 = base + g * S::kQBytes;
+            constexpr int kChunks = kDim / 8;  // of 16 bytes
+#pragma unroll
+            for (int i = 0; i < kChunks; i++) {
+                const int r = (lane + 32 * i) / kChunks, c = (lane + 32 * i) % kChunks, gr = (warp & 3) * 32 + r;
+                const C* from = reinterpret_cast<const C*>(__shfl_sync(0xffffffffu, (u64)src, r));
+                const int ok = __shfl_sync(0xffffffffu, (int)there, r);
+                if (c * 8 < D) cp_async16(q0 + (c >> 3) * (128 * 128) + sw128_off(gr, c & 7), from + c * 8, ok);
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            if (p.scale_log2 < 0.0f) {  // a negative scale: the rows' signs instead
+#pragma unroll 1
+                for (int i = 0; i < kChunks; i++) {
+                    const int r = (lane + 32 * i) / kChunks, c = (lane + 32 * i) % kChunks, gr = (warp & 3) * 32 + r;
+                    uint4* v = reinterpret_cast<uint4*>(sm + g * S::kQBytes + (c >> 3) * (128 * 128) + sw128_off(gr, c & 7));
+                    if (c * 8 < D) *v = make_uint4(v->x ^ 0x80008000u, v->y ^ 0x80008000u, v->z ^ 0x80008000u, v->w ^ 0x80008000u);
                 }
-                *reinterpret_cast<uint4*>(sm + g * S::kQBytes + (c >> 3) * (128 * 128) + sw128_off(gr, c & 7)) = v;
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -241,32 +297,31 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                         bool plain = (t + 1) * kKeys <= mine.len + (p.tree_mask ? 0 : mine.rt * kRows / p.group + 1);
 #pragma unroll
                         for (int i = 0; i < kParts; i++) plain = plain && valid[i] == 0xffffffffu;
+                        plain = __all_sync(0xffffffffu, plain);
                         if (!plain)
 #pragma unroll
                             for (int i = 0; i < kParts; i++)
                                 see[i] = on ? valid[i] & paged_sees32(p, mine, tok, t * kKeys + i * 32) : 0u;
-                        uint32_t s[2][32];
                         float x = -INFINITY;
-                        tmem_ld32(s_col, s[0]);
-#pragma unroll
-                        for (int i = 0; i < kParts; i++) {
+#pragma unroll 1
+                        for (int h = 0; h < kParts; h += 2) {
+                            uint32_t s[2][32];
+                            tmem_ld32(s_col + h * 32, s[0]);
+                            tmem_ld32(s_col + h * 32 + 32, s[1]);
                             tmem_wait_ld();
-                            if (i + 1 < kParts) tmem_ld32(s_col + (i + 1) * 32, s[(i + 1) & 1]);
-                            uint32_t (&v)[32] = s[i & 1];
-                            if (!plain)
-#pragma unroll
-                                for (int j = 0; j < 32; j++)
-                                    if (!(see[i] >> j & 1)) v[j] = 0xff800000u;  // -inf
-                            float a = __uint_as_float(v[0]), b = __uint_as_float(v[1]);
-#pragma unroll
-                            for (int j = 2; j < 32; j += 2) {
-                                a = fmaxf(a, __uint_as_float(v[j]));
-                                b = fmaxf(b, __uint_as_float(v[j + 1]));
+                            if (!plain) {
+                                pt_hide(s[0], h ? see[kParts - 2] : see[0]);
+                                pt_hide(s[1], h ? see[kParts - 1] : see[1]);
                             }
-                            x = fmaxf(x, fmaxf(a, b));
+                            float a = x, b = -INFINITY;
+#pragma unroll
+                            for (int j = 0; j < 32; j += 2) {
+                                a = max3(a, __uint_as_float(s[0][j]), __uint_as_float(s[0][j + 1]));
+                                b = max3(b, __uint_as_float(s[1][j]), __uint_as_float(s[1][j + 1]));
+                            }
+                            x = fmaxf(a, b);
                         }
                         x *= c2;
-                        tmem_ld32(s_col, s[0]);
                         // m follows when it is 2^8 behind (or has seen nothing yet)
                         const bool move = x > m + 8.0f;
                         const float m1 = move ? x : m;
@@ -274,6 +329,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                             const float keep = move ? pt_ex2(m - m1) : 1.0f;  // 0 from -inf
                             l *= keep;
                             if (t > t0) {
+#pragma unroll 1
                                 for (int c = 0; c < D; c += 16) {
                                     uint32_t o[16];
                                     tmem_ld16(o_col + c, o);
@@ -286,28 +342,34 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                             m = m1;
                         }
                         const float mu = m == -INFINITY ? 0.0f : m;
-                        float add0 = 0.0f, add1 = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < kParts; i++) {
+                        const u64 cc = pair(c2, c2), mm = pair(-mu, -mu);
+                        u64 add0 = 0, add1 = 0;
+#pragma unroll 1
+                        for (int h = 0; h < kParts; h += 2) {
+                            uint32_t s[2][32];
+                            tmem_ld32(s_col + h * 32, s[0]);
+                            tmem_ld32(s_col + h * 32 + 32, s[1]);
                             tmem_wait_ld();
-                            if (i + 1 < kParts) tmem_ld32(s_col + (i + 1) * 32, s[(i + 1) & 1]);
-                            uint32_t (&v)[32] = s[i & 1];
-                            uint32_t w[16];
-#pragma unroll
-                            for (int j = 0; j < 16; j++) {
-                                float a = pt_ex2(fmaf(__uint_as_float(v[2 * j]), c2, -mu));
-                                float b = pt_ex2(fmaf(__uint_as_float(v[2 * j + 1]), c2, -mu));
-                                if (!plain) {
-                                    if (!(see[i] >> (2 * j) & 1)) a = 0.0f;
-                                    if (!(see[i] >> (2 * j + 1) & 1)) b = 0.0f;
-                                }
-                                add0 += a;
-                                add1 += b;
-                                w[j] = pack2<C>(a, b);
+                            if (!plain) {
+                                pt_hide(s[0], h ? see[kParts - 2] : see[0]);
+                                pt_hide(s[1], h ? see[kParts - 1] : see[1]);
                             }
-                            tmem_st16(s_col + i * 16, w);  // columns whose scores have been read
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                uint32_t w[16];
+#pragma unroll
+                                for (int j = 0; j < 16; j++) {
+                                    const float2 z = unpair(fma2(pair(s[i][2 * j], s[i][2 * j + 1]), cc, mm));
+                                    const float a = pt_ex2(z.x), b = pt_ex2(z.y);
+                                    if (j & 1) add1 = add2(add1, pair(a, b));
+                                    else add0 = add2(add0, pair(a, b));
+                                    w[j] = pack2<C>(a, b);
+                                }
+                                tmem_st16(s_col + (h + i) * 16, w);  // columns whose scores have been read
+                            }
                         }
-                        l += add0 + add1;
+                        const float2 add = unpair(add2(add0, add1));
+                        l += add.x + add.y;
                         tmem_wait_st();
                     }
                     tc_fence_before();
@@ -373,14 +435,19 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
         for (int g = 0; g < kGroups; g++) n_q[g] = n_p[g] = 0;
         auto slot_at = [&](uint32_t n) { return ring + (n % S::kSlots) * S::kSlot; };
         auto full = [&](uint32_t n) { return wait(full_bar(n % S::kSlots), n / S::kSlots); };
+        const uint32_t issue = lane == 0;
         auto scores = [&](int g, uint32_t slot) {
-            if (lane == 0) {
-                for (int k = 0; k < ksteps; k++)
-                    umma_f16_ss(tmem + g * kKeys,
-                                sw128_desc(base + g * S::kQBytes + (k >> 2) * (128 * 128)) + 2u * (k & 3),
-                                sw128_desc(slot + (k >> 2) * (kKeys * 128)) + 2u * (k & 3), id_s, k ? 1u : 0u);
-                umma_commit(s_bar(g));
+            const uint64_t a = sw128_desc(base + g * S::kQBytes), b = sw128_desc(slot);
+            const uint32_t d = tmem + g * kKeys;
+#pragma unroll
+            for (int k = 0; k < kDim / 16; k++) {
+                if (k >= ksteps) break;
+                // 16 dims: 32 bytes on within a 128-byte row, then the next block of 64 dims
+                pt_mma_ss(d, a + ((k >> 2) * (128 * 128 / 16) + 2 * (k & 3)),
+                          b + ((k >> 2) * (kKeys * 128 / 16) + 2 * (k & 3)), id_s, k ? 1u : 0u, issue);
             }
+            if (lane == 0) umma_commit(s_bar(g));
+            __syncwarp();
         };
         while (pos < end && !fail) {
             int t0, t1;
@@ -413,13 +480,13 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                     if (!wait(p_bar(g), n_p[g])) break;
                     n_p[g]++;
                     tc_fence_after();
-                    if (lane == 0) {
-                        for (int k = 0; k < kKeys / 16; k++)
-                            umma_f16_ts(tmem + S::kOCol + g * kDim, tmem + g * kKeys + 8u * k,
-                                        sw128_mn_desc(slot_at(nv) + k * 2048, kKeys * 128), id_o,
-                                        t > t0 || k ? 1u : 0u);
-                        if (!more) umma_commit(o_bar(g));
-                    }
+                    const uint64_t b = sw128_mn_desc(slot_at(nv), kKeys * 128);
+                    const uint32_t d = tmem + S::kOCol + g * kDim, a = tmem + g * kKeys;
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; k++)  // 16 keys: 2048 bytes on
+                        pt_mma_ts(d, a + 8 * k, b + k * (2048 / 16), id_o, k || t > t0 ? 1u : 0u, issue);
+                    if (!more && lane == 0) umma_commit(o_bar(g));
+                    __syncwarp();
                     if (more) {
                         if (g == 0 && !full(nk)) break;
                         tc_fence_after();
@@ -535,7 +602,7 @@ static int launch_pt(const PagedAttnParams& p, const PaPlan& pl, cudaStream_t st
     lc.numAttrs = 1;
     if (cudaLaunchKernelEx(&lc, kern, tk, tv, p) != cudaSuccess) return HQ4_ERR_LAUNCH;
     if (!p.split || pl.ctas < 2) return HQ4_OK;
-    lc.gridDim = dim3(pl.ctas - 1, S::kRows / kCombineWarps);
+    lc.gridDim = dim3(pl.ctas - 1, (S::kRows + kCombineRows - 1) / kCombineRows);
     lc.blockDim = dim3(kCombineWarps * 32);
     lc.dynamicSmemBytes = 0;
     return cudaLaunchKernelEx(&lc, paged_combine_kernel<C, C, S::kRows, kDim>, p, pl.ctas) == cudaSuccess
