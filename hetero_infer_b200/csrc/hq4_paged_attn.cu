@@ -39,7 +39,7 @@ static PaPlan pa_plan(int act_type, int n_rows, int n_heads, int n_kv, int head_
     r.split = cap > kPaWhole;
     const long long units = r.split ? items * ((cap + keys - 1) / keys) : items;
     r.ctas = (int)std::min<long long>(units, (long long)sms * per_sm);
-    r.ws = r.split ? (long long)r.ctas * (sizeof(PagedItem) + 2ll * rows * (sizeof(float2) + r.dim * sizeof(float))) : 0;
+    r.ws = r.split ? (long long)r.ctas * (sizeof(PagedStart) + 2ll * rows * (sizeof(float2) + r.dim * sizeof(float))) : 0;
     return r;
 }
 

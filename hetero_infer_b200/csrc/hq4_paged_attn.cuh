@@ -46,9 +46,13 @@ struct PagedItem {
     int len, keys;     // entries before its rows; entries that the tile may see
     int tiles;         // key tiles
     int weight;        // units
+};
+// Where a CTA's part begins.
+struct PagedStart {
+    PagedItem it;
     int pad[3];
-    long long first;   // its first unit
-    long long total;   // units of the whole batch
+    long long first;  // the item's first unit
+    long long total;  // units of the whole batch
 };
 
 // Rows and lengths of a sequence, clamped to what exists.
@@ -114,12 +118,14 @@ __device__ __forceinline__ long long cta_scan(PagedScan& sh, long long v, long l
     return v;
 }
 
-// The CTA's part [pos, end) and the item that holds its first unit; false for
-// a CTA without work.  Parts are cut for min(gridDim.x, total) CTAs, so that
+// The CTA's part [pos, end) and the item that holds its first unit; pos == end
+// for a CTA without work.  Parts are cut for min(gridDim.x, total) CTAs, so that
 // every one of those has some.  All threads take part and get the same.
 template <int kRows, int kKeys, int kThreads>
-__device__ __forceinline__ bool paged_part(const PagedAttnParams& p, PagedScan& sh, PagedItem& it, long long& pos,
-                                           long long& end) {
+__device__ __forceinline__ PagedStart paged_part(const PagedAttnParams& p, PagedScan& sh, long long& pos,
+                                                 long long& end) {
+    PagedStart st = {};
+    PagedItem& it = st.it;
     const int n = p.b.n_seqs;
     long long total = 0, all;
     long long mine = threadIdx.x < n ? paged_seq_units<kRows, kKeys>(p, threadIdx.x) : 0;
@@ -131,7 +137,9 @@ __device__ __forceinline__ bool paged_part(const PagedAttnParams& p, PagedScan& 
         total += all;
     }
     const long long parts = min((long long)gridDim.x, total);
-    if ((long long)blockIdx.x >= parts) return false;
+    pos = end = 0;
+    st.total = total;
+    if ((long long)blockIdx.x >= parts) return st;
     pos = blockIdx.x * total / parts;
     end = (blockIdx.x + 1) * total / parts;
     long long run = 0, sum = total0;
@@ -157,18 +165,16 @@ __device__ __forceinline__ bool paged_part(const PagedAttnParams& p, PagedScan& 
         const long long w = (long long)it.weight * p.n_kv;
         if (pos < first + w) {
             it.h = (int)((pos - first) / it.weight);
-            it.first = first + (long long)it.h * it.weight;
+            st.first = first + (long long)it.h * it.weight;
             break;
         }
         first += w;
     }
-    it.total = total;
-    return true;
+    return st;
 }
-// The item after `it`; there is one while it.first + it.weight < it.total.
+// The item after `it`, if there is one.
 template <int kRows, int kKeys>
 __device__ __forceinline__ void paged_next(const PagedAttnParams& p, PagedItem& it) {
-    it.first += it.weight;
     if (++it.h < p.n_kv) return;
     it.h = 0;
     int rt = it.rt + 1;
@@ -237,22 +243,19 @@ __device__ __noinline__ void paged_slow_row(const PagedAttnParams& p, const Page
 // last one 2c + 1.
 template <int kRows, int kDim>
 struct PagedWs {
-    PagedItem* info;  // of the first piece of each CTA
+    PagedStart* info;  // of each CTA's part; without any work at all, of CTA 0 alone
     float2* ml;       // [pieces][kRows]: running maximum (of log2 scores) and sum
     float* o;         // [pieces][kRows][kDim], not divided
     __host__ __device__ PagedWs(void* ws, int ctas) {
         unsigned char* p = static_cast<unsigned char*>(ws);
-        info = reinterpret_cast<PagedItem*>(p);
-        p += (size_t)ctas * sizeof(PagedItem);
+        info = reinterpret_cast<PagedStart*>(p);
+        p += (size_t)ctas * sizeof(PagedStart);
         ml = reinterpret_cast<float2*>(p);
         p += (size_t)ctas * 2 * kRows * sizeof(float2);
         o = reinterpret_cast<float*>(p);
     }
-    static __host__ long long bytes(int ctas) {
-        return (long long)ctas * (sizeof(PagedItem) + 2ll * kRows * (sizeof(float2) + kDim * sizeof(float)));
-    }
 };
-static_assert(sizeof(PagedItem) % 16 == 0, "the pieces behind the items keep their alignment");
+static_assert(sizeof(PagedStart) % 16 == 0, "the pieces behind the items keep their alignment");
 
 // CTA (c, y): if part c begins inside an item, and c is the first part that
 // does in that item, joins kCombineRows rows of the item's pieces in key order;
@@ -266,16 +269,17 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
     pdl_wait();
     const PagedWs<kRows, kDim> ws(p.ws, ctas);
     const int c = blockIdx.x + 1;
-    const long long total = ws.info[0].total;  // CTA 0 has work whenever there is any row
+    const long long total = ws.info[0].total;
     const long long parts = min((long long)ctas, total);
     if (c >= parts) return;
-    const PagedItem it = ws.info[c];
+    const PagedStart st = ws.info[c];
+    const PagedItem& it = st.it;
     const long long start = c * total / parts, before = (c - 1) * total / parts;
-    if (it.first == start || it.first < before) return;
+    if (st.first == start || st.first < before) return;
     const int rows = min(kRows, it.n_tok * p.group - it.rt * kRows);
-    const int first_piece = 2 * (c - 1) + (it.first == before ? 0 : 1);
+    const int first_piece = 2 * (c - 1) + (st.first == before ? 0 : 1);
     // pieces: that one, then the first ones of parts c, c + 1, ... up to the one with the item's last unit
-    const long long last = it.first + it.weight - 1;
+    const long long last = st.first + it.weight - 1;
     long long owner = last * parts / total;  // or the one after it, by rounding
     while ((owner + 1) * total / parts <= last) owner++;
     const int n = (int)(owner - (c - 1)) + 1;

@@ -82,18 +82,17 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int D = p.head_dim, ksteps = D >> 4;
-    PagedItem it;
     long long pos, end;
-    const bool busy = paged_part<kRows, kPaKeys, kPaThreads>(p, scan, it, pos, end);
-    if (!busy) {
+    const PagedStart begin = paged_part<kRows, kPaKeys, kPaThreads>(p, scan, pos, end);
+    const PagedWs<kRows, kDim> ws(p.ws, gridDim.x);
+    if (p.ws && threadIdx.x == 0 && (pos < end || blockIdx.x == 0)) ws.info[blockIdx.x] = begin;
+    if (pos >= end) {
         pdl_launch_dependents();
-        if (p.ws && blockIdx.x == 0 && threadIdx.x == 0)  // a batch without rows: nothing to join
-            PagedWs<kRows, kDim>(p.ws, gridDim.x).info[0].total = 0;
         return;
     }
-    const long long start = pos;
-    const PagedWs<kRows, kDim> ws(p.ws, gridDim.x);
-    if (p.ws && threadIdx.x == 0) ws.info[blockIdx.x] = it;
+    PagedItem it = begin.it;
+    int left = (int)(end - pos), from = (int)(pos - begin.first);  // units still to do; the first of them in the item
+    int pieces = 0;
     unsigned char* ring = smem + warp * kRing;
     const uint32_t ring_u = smem_u32(ring);
     unsigned char* qs = smem + kPaWarps * kRing;
@@ -103,12 +102,12 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     const int in_page = (1 << p.b.page_shift) - 1;
     float* os = reinterpret_cast<float*>(ring);
 
-    while (pos < end) {
-        const long long stop = min(end, it.first + it.weight);
-        const int t0 = p.split ? (int)(pos - it.first) : 0, t1 = p.split ? (int)(stop - it.first) : it.tiles;
+    while (left > 0) {
+        const int units = min(left, it.weight - from);
+        const int t0 = p.split ? from : 0, t1 = p.split ? from + units : it.tiles;
         const bool whole = t0 == 0 && t1 == it.tiles;
         const int rows = min(kRows, it.n_tok * p.group - it.rt * kRows);
-        if (stop == end) pdl_launch_dependents();
+        if (units == left) pdl_launch_dependents();
         if (threadIdx.x == 0 && (it.len < 0 || (long long)it.len + it.n_tok > (long long)p.b.pages_per_seq << p.b.page_shift))
             atomicOr(p.b.status, kStatusPaged);  // rows whose entries have no place
 
@@ -356,7 +355,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
             }
         }
         __syncthreads();
-        const int piece = 2 * blockIdx.x + (pos == start ? 0 : 1);
+        const int piece = 2 * blockIdx.x + (pieces++ ? 1 : 0);
         for (int r = warp; r < rows; r += kPaWarps) {
             float mm = -INFINITY, ll = 0.0f, w[kPaWarps];
 #pragma unroll
@@ -391,8 +390,9 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
             if (whole && __any_sync(0xffffffffu, bad)) paged_slow_row<A, C>(p, it, row);
         }
         __syncthreads();  // the rings and the queries are free again
-        pos = stop;
-        if (pos < end) paged_next<kRows, kPaKeys>(p, it);
+        left -= units;
+        from = 0;
+        if (left > 0) paged_next<kRows, kPaKeys>(p, it);
     }
 }
 

@@ -40,29 +40,29 @@ struct PtShape {
     static constexpr int kQBytes = 128 * kDim * 2;        // of a group
     static constexpr int kSlot = kKeys * kDim * 2;        // a tile of keys or of values
     static constexpr int kSlots = kDim == 64 ? 8 : 5;
-    static constexpr int kThreads = (4 * kGroups + 2) * 32;
+    // Two groups: whole warpgroups, which share out the registers: at launch 168 a thread, of which
+    // the third keeps 88 and the two of the rows take 208 (168 x 3 = 88 + 208 x 2).
+    static constexpr int kThreads = kGroups == 2 ? 384 : 192;
     static constexpr int kSmem = kGroups * kQBytes + kSlots * kSlot + 1024;
     static constexpr int kOCol = kGroups * kKeys;         // TMEM column of the first group's O
 };
 
 // D[tmem] (+)= A . B^T, 16-bit operands, fp32 accumulator; A in shared memory or
-// in TMEM.  The whole warp comes here and `issue` picks the lane: computing the
-// operands outside of any branch lets them be in uniform registers, where a
-// loop within a one-lane branch took 128 cycles to an instruction.
+// in TMEM.
 __device__ __forceinline__ void pt_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                          uint32_t accumulate, uint32_t issue) {
+                                          uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
-        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issue)
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 __device__ __forceinline__ void pt_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                          uint32_t accumulate, uint32_t issue) {
+                                          uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
-        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issue)
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 // Descriptor of a tile whose rows are the contraction's (values: keys x dims,
@@ -73,6 +73,11 @@ __device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t smem_addr, uint32_t b
     const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
     return ((uint64_t)hi << 32) | lo;
 }
+__device__ __forceinline__ bool pt_elect() {  // one lane of the converged warp, always the same
+    uint32_t on;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(on));
+    return on != 0;
+}
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tm, int x, int y, int z, int w,
                                             uint32_t bar, uint64_t policy) {
     asm volatile(
@@ -81,12 +86,15 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tm,
         "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar), "l"(policy)
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 __device__ __forceinline__ float pt_ex2(float x) {
     float y;
@@ -163,6 +171,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
     __shared__ uint32_t s_valid[8][kKeys / 32];
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_dead;
+    __shared__ PagedItem s_items[4 * kGroups + 2][2];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     unsigned char* sm = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t ring = base + kGroups * S::kQBytes;
@@ -201,16 +210,26 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
     const uint32_t tmem = s_tmem;
     pdl_wait();
 
-    PagedItem it;
-    long long pos, end;
-    const bool busy = paged_part<kRows, kKeys, S::kThreads>(p, scan, it, pos, end);
-    const long long start = pos;
+    // each warp walks the part's items by itself; its item lies in shared memory, not in registers
+    const PagedItem* it = &s_items[min(warp, 4 * kGroups + 1)][0];  // the item at hand; the other place takes the next one
+    int left;   // units of the part that are still to do
+    int from;   // the first of them within the item
+    bool busy;
     const PagedWs<kRows, kDim> ws(p.ws, gridDim.x);
-    if (p.ws && threadIdx.x == 0) {
-        if (busy) ws.info[blockIdx.x] = it;
-        else if (blockIdx.x == 0) ws.info[0].total = 0;  // a batch without rows: nothing to join
+    {
+        long long pos, end;
+        const PagedStart begin = paged_part<kRows, kKeys, S::kThreads>(p, scan, pos, end);
+        busy = pos < end;
+        if (p.ws && threadIdx.x == 0 && (busy || blockIdx.x == 0)) ws.info[blockIdx.x] = begin;
+        left = (int)(end - pos);
+        from = (int)(pos - begin.first);
+        if (lane == 0 && warp < 4 * kGroups + 2) s_items[warp][0] = begin.it;
+        __syncwarp();
     }
     pdl_launch_dependents();
+    auto fewer_registers = [] {
+        if constexpr (kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    };
     const int D = p.head_dim, ksteps = D >> 4;
     bool fail = false;
     // A warp's wait, which ends: after so many tries (each may sleep up to a millisecond; reading a
@@ -225,27 +244,43 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
         fail = true;
         return false;
     };
-    // The key tiles of the part's piece of item `it`.
-    auto piece = [&](int& t0, int& t1) -> long long {
-        const long long stop = min(end, it.first + it.weight);
-        t0 = p.split ? (int)(pos - it.first) : 0;
-        t1 = p.split ? (int)(stop - it.first) : it.tiles;
-        return stop;
+    // The key tiles of the part's piece of the item, and the units that it takes; then the next item.
+    auto piece = [&](int& t0, int& t1) -> int {
+        const int units = min(left, it->weight - from);
+        t0 = p.split ? from : 0;
+        t1 = p.split ? from + units : it->tiles;
+        return units;
     };
-    auto groups_of = [&]() { return it.n_tok * p.group - it.rt * kRows > 128 ? kGroups : 1; };
+    auto next = [&](int units) {
+        left -= units;
+        from = 0;
+        if (left > 0) {
+            PagedItem* n = it == &s_items[warp][0] ? &s_items[warp][1] : &s_items[warp][0];
+            __syncwarp();
+            if (lane == 0) {
+                PagedItem i = *it;
+                paged_next<kRows, kKeys>(p, i);
+                *n = i;
+            }
+            __syncwarp();
+            it = n;
+        }
+    };
+    auto groups_of = [&]() { return it->n_tok * p.group - it->rt * kRows > 128 ? kGroups : 1; };
 
     if (busy && warp < 4 * kGroups) {
         // ---- rows ------------------------------------------------------------------
+        if constexpr (kGroups == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int g = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t s_col = tmem + lanes + g * kKeys, o_col = tmem + lanes + S::kOCol + g * kDim;
         const int in_group = (warp & 3) * 32 + lane;
         auto load_q = [&]() {  // the group's rows of item `it`, a warp its own 32, all copies in flight at once
-            const int row = it.rt * kRows + g * 128 + in_group;
-            const bool there = row < it.n_tok * p.group;
+            const int row = it->rt * kRows + g * 128 + in_group;
+            const bool there = row < it->n_tok * p.group;
             const C* src = static_cast<const C*>(p.q);
             if (there)
-                src += (long long)(it.row0 + row / p.group) * p.q_stride + ((long long)it.h * p.group + row % p.group) * D;
+                src += (long long)(it->row0 + row / p.group) * p.q_stride + ((long long)it->h * p.group + row % p.group) * D;
             const uint32_t q0 = base + g * S::kQBytes;
             constexpr int kChunks = kDim / 8;  // of 16 bytes
 #pragma unroll
@@ -271,17 +306,18 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
         };
         uint32_t n_s = 0, n_o = 0, tile_no = 0;  // tiles of this group, pieces of it, tiles of the CTA so far
         if (g < groups_of()) load_q();
-        while (pos < end && !fail) {
+        int pieces = 0;
+        while (left > 0 && !fail) {
             int t0, t1;
-            const long long stop = piece(t0, t1);
-            const bool whole = t0 == 0 && t1 == it.tiles;
-            const PagedItem mine = it;
+            const int units = piece(t0, t1);
+            const bool whole = t0 == 0 && t1 == it->tiles;
             const bool in = g < groups_of();
-            const int row = it.rt * kRows + g * 128 + in_group, rows = it.n_tok * p.group;
+            const int row = it->rt * kRows + g * 128 + in_group, rows = it->n_tok * p.group;
             const bool on = in && row < rows;
-            const bool warp_on = in && it.rt * kRows + g * 128 + (warp & 3) * 32 < rows;
+            const bool warp_on = in && it->rt * kRows + g * 128 + (warp & 3) * 32 < rows;
             const int tok = on ? row / p.group : 0;
             float m = -INFINITY, l = 0.0f;  // of scaled scores (log2), and the row's sum
+            const int t_plain = (it->len + (p.tree_mask ? 0 : it->rt * kRows / p.group + 1)) / kKeys;  // before: all seen
             const float c2 = fmaxf(fabsf(p.scale_log2), 1e-30f);  // not 0: masked scores stay -inf
             if (in) {
                 for (int t = t0; t < t1; t++, n_s++) {
@@ -289,87 +325,71 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                     __syncwarp();
                     tc_fence_after();
                     if (warp_on) {
-                        // the row twice, 32 scores at a time: for its maximum, then for P (a second
-                        // read of TMEM costs less than 128 registers of scores)
                         constexpr int kParts = kKeys / 32;
-                        uint32_t see[kParts];
+                        uint32_t s[kParts][32];
+#pragma unroll
+                        for (int i = 0; i < kParts; i++) tmem_ld32(s_col + i * 32, s[i]);
+                        tmem_wait_ld();
                         const uint32_t* valid = s_valid[(tile_no + (t - t0)) & 7];
-                        bool plain = (t + 1) * kKeys <= mine.len + (p.tree_mask ? 0 : mine.rt * kRows / p.group + 1);
+                        bool plain = t < t_plain;
 #pragma unroll
                         for (int i = 0; i < kParts; i++) plain = plain && valid[i] == 0xffffffffu;
-                        plain = __all_sync(0xffffffffu, plain);
-                        if (!plain)
+                        if (!__all_sync(0xffffffffu, plain)) {
 #pragma unroll
-                            for (int i = 0; i < kParts; i++)
-                                see[i] = on ? valid[i] & paged_sees32(p, mine, tok, t * kKeys + i * 32) : 0u;
-                        float x = -INFINITY;
-#pragma unroll 1
-                        for (int h = 0; h < kParts; h += 2) {
-                            uint32_t s[2][32];
-                            tmem_ld32(s_col + h * 32, s[0]);
-                            tmem_ld32(s_col + h * 32 + 32, s[1]);
-                            tmem_wait_ld();
-                            if (!plain) {
-                                pt_hide(s[0], h ? see[kParts - 2] : see[0]);
-                                pt_hide(s[1], h ? see[kParts - 1] : see[1]);
-                            }
-                            float a = x, b = -INFINITY;
+                            for (int i = 0; i < kParts; i++) {
+                                const uint32_t see = on ? valid[i] & paged_sees32(p, *it, tok, t * kKeys + i * 32) : 0u;
 #pragma unroll
-                            for (int j = 0; j < 32; j += 2) {
-                                a = max3(a, __uint_as_float(s[0][j]), __uint_as_float(s[0][j + 1]));
-                                b = max3(b, __uint_as_float(s[1][j]), __uint_as_float(s[1][j + 1]));
+                                for (int j = 0; j < 32; j++)
+                                    if (!(see >> j & 1)) s[i][j] = 0xff800000u;  // -inf
                             }
-                            x = fmaxf(a, b);
                         }
-                        x *= c2;
+                        float top[kParts];
+#pragma unroll
+                        for (int i = 0; i < kParts; i++) {
+                            top[i] = fmaxf(__uint_as_float(s[i][0]), __uint_as_float(s[i][1]));
+#pragma unroll
+                            for (int j = 2; j < 32; j += 2)
+                                top[i] = max3(top[i], __uint_as_float(s[i][j]), __uint_as_float(s[i][j + 1]));
+                        }
+#pragma unroll
+                        for (int i = 1; i < kParts; i++) top[0] = fmaxf(top[0], top[i]);
+                        const float x = top[0] * c2;
                         // m follows when it is 2^8 behind (or has seen nothing yet)
                         const bool move = x > m + 8.0f;
-                        const float m1 = move ? x : m;
                         if (__any_sync(0xffffffffu, move)) {
+                            const float m1 = move ? x : m;
                             const float keep = move ? pt_ex2(m - m1) : 1.0f;  // 0 from -inf
                             l *= keep;
+                            m = m1;
                             if (t > t0) {
 #pragma unroll 1
-                                for (int c = 0; c < D; c += 16) {
-                                    uint32_t o[16];
-                                    tmem_ld16(o_col + c, o);
+                                for (int c = 0; c < D; c += 8) {
+                                    uint32_t o[8];
+                                    tmem_ld8(o_col + c, o);
                                     tmem_wait_ld();
 #pragma unroll
-                                    for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-                                    tmem_st16(o_col + c, o);
+                                    for (int j = 0; j < 8; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                                    tmem_st8(o_col + c, o);
                                 }
                             }
-                            m = m1;
                         }
                         const float mu = m == -INFINITY ? 0.0f : m;
                         const u64 cc = pair(c2, c2), mm = pair(-mu, -mu);
-                        u64 add0 = 0, add1 = 0;
-#pragma unroll 1
-                        for (int h = 0; h < kParts; h += 2) {
-                            uint32_t s[2][32];
-                            tmem_ld32(s_col + h * 32, s[0]);
-                            tmem_ld32(s_col + h * 32 + 32, s[1]);
-                            tmem_wait_ld();
-                            if (!plain) {
-                                pt_hide(s[0], h ? see[kParts - 2] : see[0]);
-                                pt_hide(s[1], h ? see[kParts - 1] : see[1]);
-                            }
+                        u64 add[2] = {0, 0};
 #pragma unroll
-                            for (int i = 0; i < 2; i++) {
-                                uint32_t w[16];
+                        for (int i = 0; i < kParts; i++) {
+                            uint32_t w[16];
 #pragma unroll
-                                for (int j = 0; j < 16; j++) {
-                                    const float2 z = unpair(fma2(pair(s[i][2 * j], s[i][2 * j + 1]), cc, mm));
-                                    const float a = pt_ex2(z.x), b = pt_ex2(z.y);
-                                    if (j & 1) add1 = add2(add1, pair(a, b));
-                                    else add0 = add2(add0, pair(a, b));
-                                    w[j] = pack2<C>(a, b);
-                                }
-                                tmem_st16(s_col + (h + i) * 16, w);  // columns whose scores have been read
+                            for (int j = 0; j < 16; j++) {
+                                const float2 z = unpair(fma2(pair(s[i][2 * j], s[i][2 * j + 1]), cc, mm));
+                                const float a = pt_ex2(z.x), b = pt_ex2(z.y);
+                                add[j & 1] = add2(add[j & 1], pair(a, b));
+                                w[j] = pack2<C>(a, b);
                             }
+                            tmem_st16(s_col + i * 16, w);  // over scores that are in registers
                         }
-                        const float2 add = unpair(add2(add0, add1));
-                        l += add.x + add.y;
+                        const float2 sum = unpair(add2(add[0], add[1]));
+                        l += sum.x + sum.y;
                         tmem_wait_st();
                     }
                     tc_fence_before();
@@ -378,12 +398,12 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                 }
             }
             tile_no += t1 - t0;
-            // ---- the next item's rows, then this one's output ------------------------
-            const long long was = pos;
-            pos = stop;
-            if (pos < end) paged_next<kRows, kKeys>(p, it);
+            // ---- the next item's rows (S of the last tile is done: Q is free), then this one's output ----
             if (fail) break;
-            if (pos < end && g < groups_of()) load_q();  // S of the last tile is done: Q is free
+            const PagedItem* const mine = it;
+            const int piece_no = 2 * blockIdx.x + (pieces++ ? 1 : 0);
+            next(units);
+            if (left > 0 && g < groups_of()) load_q();
             if (!in) continue;
             if (!wait(o_bar(g), n_o)) break;
             n_o++;
@@ -393,8 +413,8 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 const int r = g * 128 + in_group;
                 C* out = static_cast<C*>(p.out) +
-                         ((long long)(mine.row0 + tok) * p.n_heads + mine.h * p.group + row % p.group) * D;
-                const size_t at = (size_t)(2 * blockIdx.x + (was == start ? 0 : 1)) * kRows + r;
+                         ((long long)(mine->row0 + tok) * p.n_heads + mine->h * p.group + row % p.group) * D;
+                const size_t at = (size_t)piece_no * kRows + r;
                 bool bad = false;
                 for (int c = 0; c < D; c += 32) {
                     uint32_t o[32];
@@ -421,13 +441,14 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                 while (again) {
                     const int i = __ffs(again) - 1;
                     again &= again - 1;
-                    paged_slow_row<C, C>(p, mine, __shfl_sync(0xffffffffu, row, i));
+                    paged_slow_row<C, C>(p, *mine, __shfl_sync(0xffffffffu, row, i));
                 }
             }
             tc_fence_before();
         }
     } else if (busy && warp == 4 * kGroups) {
         // ---- matrix instructions -------------------------------------------------------
+        fewer_registers();
         constexpr uint32_t kType = Elem<C>::code == HQ4_BF16 ? 1u : 0u;
         const uint32_t id_s = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(kKeys >> 3) << 17) | (8u << 24);
         const uint32_t id_o = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
@@ -435,23 +456,24 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
         for (int g = 0; g < kGroups; g++) n_q[g] = n_p[g] = 0;
         auto slot_at = [&](uint32_t n) { return ring + (n % S::kSlots) * S::kSlot; };
         auto full = [&](uint32_t n) { return wait(full_bar(n % S::kSlots), n / S::kSlots); };
-        const uint32_t issue = lane == 0;
         auto scores = [&](int g, uint32_t slot) {
             const uint64_t a = sw128_desc(base + g * S::kQBytes), b = sw128_desc(slot);
             const uint32_t d = tmem + g * kKeys;
+            if (pt_elect()) {
 #pragma unroll
-            for (int k = 0; k < kDim / 16; k++) {
-                if (k >= ksteps) break;
-                // 16 dims: 32 bytes on within a 128-byte row, then the next block of 64 dims
-                pt_mma_ss(d, a + ((k >> 2) * (128 * 128 / 16) + 2 * (k & 3)),
-                          b + ((k >> 2) * (kKeys * 128 / 16) + 2 * (k & 3)), id_s, k ? 1u : 0u, issue);
+                for (int k = 0; k < kDim / 16; k++) {
+                    if (k >= ksteps) break;
+                    // 16 dims: 32 bytes on within a 128-byte row, then the next block of 64 dims
+                    pt_mma_ss(d, a + ((k >> 2) * (128 * 128 / 16) + 2 * (k & 3)),
+                              b + ((k >> 2) * (kKeys * 128 / 16) + 2 * (k & 3)), id_s, k ? 1u : 0u);
+                }
+                umma_commit(s_bar(g));
             }
-            if (lane == 0) umma_commit(s_bar(g));
             __syncwarp();
         };
-        while (pos < end && !fail) {
+        while (left > 0 && !fail) {
             int t0, t1;
-            const long long stop = piece(t0, t1);
+            const int units = piece(t0, t1);
             const int ng = groups_of();
             if (!full(n_slot)) break;
             for (int g = 0; g < ng && !fail; g++) {
@@ -466,7 +488,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                 const uint32_t nv = n_slot + 1, nk = n_slot + 2;  // this tile's values, the next one's keys
                 const bool more = t + 1 < t1;
                 if (!full(nv)) break;
-                const int past = it.keys - t * kKeys;  // values that no row sees may be anything: zeros instead
+                const int past = it->keys - t * kKeys;  // values that no row sees may be anything: zeros instead
                 if (past < kKeys) {
                     for (int i = lane; i < (kKeys - max(past, 0)) * (kDim / 8); i += 32) {
                         const int r = max(past, 0) + i / (kDim / 8), c = i % (kDim / 8);
@@ -482,10 +504,12 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                     tc_fence_after();
                     const uint64_t b = sw128_mn_desc(slot_at(nv), kKeys * 128);
                     const uint32_t d = tmem + S::kOCol + g * kDim, a = tmem + g * kKeys;
+                    if (pt_elect()) {
 #pragma unroll
-                    for (int k = 0; k < kKeys / 16; k++)  // 16 keys: 2048 bytes on
-                        pt_mma_ts(d, a + 8 * k, b + k * (2048 / 16), id_o, k || t > t0 ? 1u : 0u, issue);
-                    if (!more && lane == 0) umma_commit(o_bar(g));
+                        for (int k = 0; k < kKeys / 16; k++)  // 16 keys: 2048 bytes on
+                            pt_mma_ts(d, a + 8 * k, b + k * (2048 / 16), id_o, k || t > t0 ? 1u : 0u);
+                        if (!more) umma_commit(o_bar(g));
+                    }
                     __syncwarp();
                     if (more) {
                         if (g == 0 && !full(nk)) break;
@@ -500,28 +524,28 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                 }
                 n_slot += 2;
             }
-            pos = stop;
-            if (pos < end) paged_next<kRows, kKeys>(p, it);
+            next(units);
         }
         if (lane == 0) umma_commit(end_bar);
         __syncwarp();
         // all products are done before the memory goes (a limit of its own: the others may have failed)
         mbar_wait_ns(end_bar, 0, kPtWaitNs);
-    } else if (busy) {
+    } else if (busy && warp == 4 * kGroups + 1) {
         // ---- keys and values -------------------------------------------------------------
+        fewer_registers();
         const uint64_t policy = l2_policy_evict_last();
         const int box = min(1 << p.b.page_shift, kKeys), boxes = kKeys / box;
         uint32_t n = 0, tile_no = 0;
-        while (pos < end && !fail) {
+        while (left > 0 && !fail) {
             int t0, t1;
-            const long long stop = piece(t0, t1);
-            if (lane == 0 && (it.len < 0 || (long long)it.len + it.n_tok > (long long)p.b.pages_per_seq << p.b.page_shift))
+            const int units = piece(t0, t1);
+            if (lane == 0 && (it->len < 0 || (long long)it->len + it->n_tok > (long long)p.b.pages_per_seq << p.b.page_shift))
                 atomicOr(p.b.status, kStatusPaged);  // rows whose entries have no place
             for (int t = t0; t < t1 && !fail; t++, tile_no++) {
                 const int e = t * kKeys + lane * box;
                 int page = -1;
-                if (lane < boxes && e < it.keys) {
-                    page = find_page(p.b, it.s, e);
+                if (lane < boxes && e < it->keys) {
+                    page = find_page(p.b, it->s, e);
                     if (page < 0) atomicOr(p.b.status, kStatusPaged);
                 }
                 const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
@@ -542,17 +566,17 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                         const int y = e & ((1 << p.b.page_shift) - 1), w = page >= 0 ? page : p.b.n_pages;
                         for (int b = 0; b < S::kBlocks; b++)
                             tma_load_4d(ring + slot * S::kSlot + b * (kKeys * 128) + lane * box * 128,
-                                        kv ? &tm_v : &tm_k, b * 64, y, it.h, w, full_bar(slot), policy);
+                                        kv ? &tm_v : &tm_k, b * 64, y, it->h, w, full_bar(slot), policy);
                     }
                 }
             }
-            pos = stop;
-            if (pos < end) paged_next<kRows, kKeys>(p, it);
+            next(units);
         }
         // no copy is left behind: each slot's last one has arrived
         for (uint32_t i = n > S::kSlots ? n - S::kSlots : 0; i < n; i++)
             mbar_wait_ns(full_bar(i % S::kSlots), (i / S::kSlots) & 1u, kPtWaitNs);
     }
+    if (busy && warp > 4 * kGroups + 1) fewer_registers();  // the rest of the third warpgroup
     if (fail && lane == 0) atomicOr(p.b.status, 1);
     __syncwarp();
     tc_fence_before();
