@@ -41,6 +41,17 @@ inline cudaError_t smem_opt_in(PerDeviceOnce& once, Kern kern, int bytes) {
     return once.run([&](int) { return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
 }
 
+// SMs of the current device (0: the query failed).
+inline int device_sms() {
+    static PerDeviceOnce once;
+    static int n[kMaxDevices] = {0};
+    int dev = 0;
+    if (once.run([&](int d) { return cudaDeviceGetAttribute(&n[d], cudaDevAttrMultiProcessorCount, d); }) != cudaSuccess ||
+        cudaGetDevice(&dev) != cudaSuccess)
+        return 0;
+    return n[dev];
+}
+
 // Split-K factor for `tiles` output tiles of `kern` (one CTA per tile and
 // split, the splits of a tile launched as one 1 x ks x 1 cluster): the ks in
 // [1, kmax] with the most splits per wave, the fewer splits on a tie.  A

@@ -43,17 +43,6 @@ static PaPlan pa_plan(int act_type, int n_rows, int n_heads, int n_kv, int head_
     return r;
 }
 
-// SMs of the current device (0: the query failed).
-static int sm_count() {
-    static PerDeviceOnce once;
-    static int n[kMaxDevices] = {0};
-    int dev = 0;
-    if (once.run([&](int d) { return cudaDeviceGetAttribute(&n[d], cudaDevAttrMultiProcessorCount, d); }) != cudaSuccess ||
-        cudaGetDevice(&dev) != cudaSuccess)
-        return 0;
-    return n[dev];
-}
-
 static int paged_attention(const void* q, int act_type, int n_rows, int n_heads, int n_kv, int head_dim,
                            long long q_stride, const int* cu_rows, const int* lens, int n_seqs, const int* pages,
                            int pages_per_seq, const void* k_cache, const void* v_cache, int cache_type, int n_pages,
@@ -70,7 +59,7 @@ static int paged_attention(const void* q, int act_type, int n_rows, int n_heads,
         return HQ4_ERR_ALIGN;
     if (int rc = check_device_cap()) return rc;
     p.b.status = status_word();
-    const int sms = sm_count();
+    const int sms = device_sms();
     if (!p.b.status || sms <= 0) return HQ4_ERR_LAUNCH;
     const PaPlan pl = pa_plan(act_type, n_rows, n_heads, n_kv, head_dim, n_seqs, pages_per_seq, page_size, sms);
     if (pl.ws) {
@@ -107,7 +96,7 @@ extern "C" long long hq4_paged_attention_workspace_bytes(int act_type, int n_row
         head_dim > 256 || n_seqs <= 0 || pages_per_seq <= 0 || page_size <= 0 || act_type < HQ4_F32 ||
         act_type > HQ4_F16)
         return -1;
-    const int sms = sm_count();
+    const int sms = device_sms();
     if (sms <= 0) return -1;
     return pa_plan(act_type, n_rows, n_heads, n_kv, head_dim, n_seqs, pages_per_seq, page_size, sms).ws;
 }

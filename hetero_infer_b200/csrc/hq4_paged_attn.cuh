@@ -16,14 +16,6 @@
 
 namespace hq4 {
 
-// 16 bytes to shared memory; zeros where `on` is not set (nothing is read then).
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct PagedAttnParams {

@@ -6,9 +6,9 @@
 // keeps, and the draw walks it in index order.  Nothing is sorted: a cluster of
 // CTAs holds a row in shared memory (read from memory once), and the value at
 // which a filter ends is found by a radix search.  Its keys are the distances
-// below the maximum in 2^15 equal steps over the 44 octaves that have mass --
+// below the maximum in 2^12 equal steps over the 44 octaves that have mass --
 // a monotone function of the value whose digits, unlike the float's own, split
-// a row evenly -- five bits at a time; the few entries of the last step are
+// a row evenly -- four bits at a time; the few entries of the last step are
 // compared with one another.
 //
 // Masses are integers: w = floor(2^44 * 2^((x - max) / T * log2 e)) from fp64
@@ -17,8 +17,12 @@
 // cumulative bounds are off by less than 2^-40 of the whole, where fp32 sums
 // over 1.5e5 entries would be off by 1e-6 and move tokens.
 //
-// A digit's 32 sums are taken in columns of shared memory, one to a thread
-// (no atomics), then over the threads and the cluster.
+// A digit's 16 sums are taken in columns of shared memory, one to a thread
+// (no atomics: equal addresses within a warp would queue), then over the
+// threads and the cluster.  A thread owns a run of consecutive entries, so its
+// columns above the end that is found add up to what its run contributes to
+// the draw, and only the thread in whose run the draw falls looks at single
+// entries again.
 #include <algorithm>
 
 #include "hq4_host.cuh"
@@ -29,12 +33,14 @@ namespace hq4 {
 int check_device_cap();
 int* status_word();
 
-constexpr int kSrBins = 32;
-constexpr float kSrSteps = 32768.0f;   // of the search's keys
+constexpr int kSrDigit = 4;             // bits
+constexpr int kSrBins = 1 << kSrDigit;
+constexpr float kSrSteps = 4096.0f;    // of the search's keys
 constexpr double kSrOctaves = 44.0;    // that have mass
-constexpr int kSrList = 512;           // entries of one step that are compared directly
+constexpr int kSrList = 512;            // entries of one step that are compared directly
 constexpr int kSrMaxCluster = 8;
 constexpr int kSrMaxSlice = 36864;     // entries of a CTA
+constexpr size_t kSrSmem = 212 * 1024;
 
 struct SampleRowsParams {
     const void* x;
@@ -82,22 +88,26 @@ struct SampleRowsShared {
     u64 sums[kSrBins];
     u64 warp[T / 32];
     u64 pair[2][kSrMaxCluster];          // a number of each CTA, by turns
-    uint32_t list[kSrList];              // rank 0's: keys of one step's entries
+    uint32_t list[kSrList];              // rank 0's: keys of one step's entries, and their weights
+    u64 list_w[kSrList];
+    u64 target;
     uint32_t n_list, best;
     u64 best_above;
     u64 bin_before;
     int bin;
 };
 
-template <int T>
+template <class E, int T>
 struct SampleRow {
     SampleRowsShared<T>& sh;
     u64* hist;         // [kSrBins][T]
-    const float* xs;   // this CTA's slice
-    int cnt, rank, nr, turn, pturn;
+    const E* xs;       // this CTA's slice
+    int a, b;          // the thread's run in it
+    int rank, nr, turn, pturn;
     float top, steps;  // the maximum; steps of the search's keys for a unit of x
     double oct;        // octaves for a unit of x
 
+    __device__ __forceinline__ float at(int i) const { return Elem<E>::to(xs[i]) + 0.0f; }  // -0 counts as 0
     // Sum over the cluster; every thread gets it, and the sum of lower ranks.
     __device__ u64 cluster_sum(u64 v, u64* lower = nullptr) {
 #pragma unroll
@@ -119,6 +129,21 @@ struct SampleRow {
         pturn ^= 1;
         if (lower) *lower = lo;
         return t;
+    }
+    // Sum over the CTA's threads before this one.
+    __device__ u64 cta_before(u64 v) {
+        u64 inc = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
+            if ((threadIdx.x & 31) >= o) inc += y;
+        }
+        __syncthreads();
+        if ((threadIdx.x & 31) == 31) sh.warp[threadIdx.x >> 5] = inc;
+        __syncthreads();
+        u64 before = inc - v;
+        for (int w = 0; w < (int)(threadIdx.x >> 5); w++) before += sh.warp[w];
+        return before;
     }
     __device__ uint32_t cluster_max(uint32_t v) {  // of 32-bit numbers
         v = __reduce_max_sync(0xffffffffu, v);
@@ -161,55 +186,72 @@ struct SampleRow {
     __device__ __forceinline__ u64 weight(float x, bool counting) const { return counting ? 1 : mass(x); }
 
     // The smallest value v >= floor_key's of an entry with mass such that the
-    // entries above it weigh less than `target` (each its mass, or one), and
-    // what those weigh.  There is one when target >= 1.
-    __device__ uint32_t find_end(bool counting, u64 target, uint32_t floor_key, u64& above) {
+    // entries above it weigh less than the target (each its mass, or one), and
+    // what those weigh.  The target is `count`, or, of the masses, share times
+    // `whole` (of all masses where that is 0), at least 1, so that there is
+    // such a value.  `mine` gets the masses of the thread's run above v's step;
+    // `step` is that step.
+    __device__ uint32_t find_end(bool counting, u64 count, double share, u64 whole, uint32_t floor_key, u64& above,
+                                 u64& mine, int& step) {
+        u64 target = count;
         u64 before = 0;  // weight of the entries above the searched range
         int prefix = 0;  // the key's digits so far
-        for (int shift = 10; shift >= 0; shift -= 5) {
-            for (int b = 0; b < kSrBins; b++) hist[b * T + threadIdx.x] = 0;
-            for (int i = threadIdx.x; i < cnt; i += T) {
-                const float x = xs[i], k = key(x);
+        mine = 0;
+        for (int shift = 2 * kSrDigit; shift >= 0; shift -= kSrDigit) {
+#pragma unroll
+            for (int i = 0; i < kSrBins; i++) hist[i * T + threadIdx.x] = 0;
+#pragma unroll 2
+            for (int i = a; i < b; i++) {
+                const float x = at(i), k = key(x);
                 if (!(k < kSrSteps) || order_bits(x) < floor_key) continue;
                 const int f = (int)k >> shift;
-                if (f >> 5 == prefix) hist[(f & 31) * T + threadIdx.x] += weight(x, counting);
+                if (f >> kSrDigit == prefix) hist[(f & (kSrBins - 1)) * T + threadIdx.x] += weight(x, counting);
             }
             __syncthreads();
             const int lane = threadIdx.x & 31;
-            for (int b = threadIdx.x >> 5; b < kSrBins; b += T / 32) {
+            for (int i = threadIdx.x >> 5; i < kSrBins; i += T / 32) {
                 u64 v = 0;
-#pragma unroll 8
-                for (int j = 0; j < T / 32; j++) v += hist[b * T + j * 32 + lane];
+#pragma unroll
+                for (int j = 0; j < T / 32; j++) v += hist[i * T + j * 32 + lane];
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                if (lane == 0) sh.sums[b] = v;
+                if (lane < nr) st_cluster_u64(map_to_rank(smem_u32(&sh.all[turn][rank][i]), lane), v);
             }
-            __syncthreads();
-            for (int i = threadIdx.x; i < nr * kSrBins; i += T)
-                st_cluster_u64(map_to_rank(smem_u32(&sh.all[turn][rank][i & 31]), i >> 5), sh.sums[i & 31]);
             cluster_sync();
             if (threadIdx.x < 32) {  // a bin to a lane
                 u64 v = 0;
-                for (int r = 0; r < nr; r++) v += sh.all[turn][r][lane];
+                if (lane < kSrBins)
+                    for (int r = 0; r < nr; r++) v += sh.all[turn][r][lane];
                 u64 upto = v;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
+                for (int o = 1; o < kSrBins; o <<= 1) {
                     const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
                     if (lane >= o) upto += y;
                 }
+                if (!counting && shift == 2 * kSrDigit) {
+                    const u64 all = whole ? whole : __shfl_sync(0xffffffffu, upto, kSrBins - 1);
+                    const double want = ceil(share * (double)all);
+                    target = want >= 1.0 ? (u64)want : 1;
+                    if (lane == 0) sh.target = target;
+                }
                 const u64 excl = before + upto - v;
                 const uint32_t ok = __ballot_sync(0xffffffffu, v != 0 && excl < target);
-                const int b = ok ? 31 - __clz(ok) : 0;  // the last step that begins below the target
-                if (lane == b) {
-                    sh.bin = b;
+                const int i = ok ? 31 - __clz(ok) : 0;  // the last step that begins below the target
+                if (lane == i) {
+                    sh.bin = i;
                     sh.bin_before = excl;
                 }
             }
             __syncthreads();
             turn ^= 1;
+            if (!counting) target = sh.target;
             before = sh.bin_before;
-            prefix = prefix << 5 | sh.bin;
+            const int bin = sh.bin;
+            if (!counting)
+                for (int i = 0; i < bin; i++) mine += hist[i * T + threadIdx.x];
+            prefix = prefix << kSrDigit | bin;
         }
+        step = prefix;
         // the entries of the last step
         if (threadIdx.x == 0) {
             sh.n_list = 0;
@@ -218,41 +260,42 @@ struct SampleRow {
         cluster_sync();
         const uint32_t head = map_to_rank(smem_u32(&sh.n_list), 0);
         uint32_t low = 0xffffffffu, high = 0;
-        for (int i = threadIdx.x; i < cnt; i += T) {
-            const float x = xs[i], k = key(x);
+        for (int i = a; i < b; i++) {
+            const float x = at(i), k = key(x);
+            if (!(k < kSrSteps) || (int)k != prefix) continue;
             const uint32_t ob = order_bits(x);
-            if (!(k < kSrSteps) || (int)k != prefix || ob < floor_key) continue;
+            if (ob < floor_key) continue;
             low = min(low, ob);
             high = max(high, ob);
-            const uint32_t at = atom_add_cluster(head, 1);
-            if (at < kSrList) st_cluster_u32(map_to_rank(smem_u32(&sh.list[at]), 0), ob);
+            const uint32_t place = atom_add_cluster(head, 1);
+            if (place < kSrList) st_cluster_u32(map_to_rank(smem_u32(&sh.list[place]), 0), ob);
         }
         cluster_sync();
         const uint32_t n = (uint32_t)ld_cluster_u32(head);
         if (n <= kSrList) {
             if (rank == 0) {
+                for (uint32_t i = threadIdx.x; i < n; i += T) sh.list_w[i] = weight(order_value(sh.list[i]), counting);
+                __syncthreads();
                 for (uint32_t i = threadIdx.x; i < n; i += T) {
-                    const uint32_t mine = sh.list[i];
-                    u64 a = before;
-                    for (uint32_t j = 0; j < n; j++) {
-                        const uint32_t o = sh.list[j];
-                        if (o > mine) a += weight(order_value(o), counting);
-                    }
-                    if (a < target) atomicMin(&sh.best, mine);
+                    const uint32_t key_i = sh.list[i];
+                    u64 w = before;
+                    for (uint32_t j = 0; j < n; j++)
+                        if (sh.list[j] > key_i) w += sh.list_w[j];
+                    if (w < target) atomicMin(&sh.best, key_i);
                 }
                 __syncthreads();
                 const uint32_t v = sh.best;
-                u64 a = 0;
+                u64 w = 0;
                 for (uint32_t i = threadIdx.x; i < n; i += T)
-                    if (sh.list[i] > v) a += weight(order_value(sh.list[i]), counting);
+                    if (sh.list[i] > v) w += sh.list_w[i];
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-                if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = a;
+                for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+                if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = w;
                 __syncthreads();
                 if (threadIdx.x == 0) {
-                    a = before;
-                    for (int w = 0; w < T / 32; w++) a += sh.warp[w];
-                    sh.best_above = a;
+                    w = before;
+                    for (int i = 0; i < T / 32; i++) w += sh.warp[i];
+                    sh.best_above = w;
                 }
             }
             cluster_sync();
@@ -266,15 +309,15 @@ struct SampleRow {
         above = before;
         while (lo < hi) {
             const uint32_t mid = lo + ((hi - lo) >> 1);
-            u64 a = 0;
-            for (int i = threadIdx.x; i < cnt; i += T) {
-                const float x = xs[i], k = key(x);
-                if (k < kSrSteps && (int)k == prefix && order_bits(x) > mid) a += weight(x, counting);
+            u64 w = 0;
+            for (int i = a; i < b; i++) {
+                const float x = at(i), k = key(x);
+                if (k < kSrSteps && (int)k == prefix && order_bits(x) > mid) w += weight(x, counting);
             }
-            a = before + cluster_sum(a);
-            if (a < target) {
+            w = before + cluster_sum(w);
+            if (w < target) {
                 hi = mid;
-                above = a;
+                above = w;
             } else {
                 lo = mid + 1;
             }
@@ -288,9 +331,6 @@ struct SampleRow {
     }
 };
 
-template <class E>
-__device__ __forceinline__ float as_logit(E v) { return Elem<E>::to(v) + 0.0f; }  // -0 counts as 0
-
 template <class E, int T>
 __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p) {
     extern __shared__ __align__(128) unsigned char smem[];
@@ -300,52 +340,41 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
     const int rank = (int)cluster_ctarank(), nr = (int)cluster_nctarank();
     const int row = blockIdx.x / nr;
     const int lo = min(p.n, rank * p.chunk), cnt = min(p.n, lo + p.chunk) - lo;
-    u64* hist = reinterpret_cast<u64*>(smem);
     const E* src = static_cast<const E*>(p.x) + (long long)row * p.stride + lo;
     constexpr int kV = 16 / sizeof(E);
     const int off = (int)((uintptr_t)src & 15) / (int)sizeof(E);  // the slice keeps the row's alignment
-    float* xs = reinterpret_cast<float*>(smem + sizeof(u64) * kSrBins * T) + off;
+    E* xs = reinterpret_cast<E*>(smem + sizeof(u64) * kSrBins * T) + off;
 
-    // ---- the slice; its largest entry, the first of its equals; NaN ------------
+    // ---- the slice, all copies in flight at once ---------------------------------
     const int head = min(cnt, (kV - off) % kV), vecs = (cnt - head) / kV;
-    for (int i = threadIdx.x; i < head; i += T) xs[i] = as_logit(src[i]);
-    for (int i = head + vecs * kV + threadIdx.x; i < cnt; i += T) xs[i] = as_logit(src[i]);
-    const uint4* vsrc = reinterpret_cast<const uint4*>(src + head);
-    auto put = [&](int v, uint4 w) {
-        float4* d = reinterpret_cast<float4*>(xs + head + v * kV);
-        if constexpr (sizeof(E) == 4) {
-            d[0] = make_float4(__uint_as_float(w.x) + 0.0f, __uint_as_float(w.y) + 0.0f, __uint_as_float(w.z) + 0.0f,
-                               __uint_as_float(w.w) + 0.0f);
-        } else {
-            const float2 a = unpack2<E>(w.x), b = unpack2<E>(w.y), c = unpack2<E>(w.z), e = unpack2<E>(w.w);
-            d[0] = make_float4(a.x + 0.0f, a.y + 0.0f, b.x + 0.0f, b.y + 0.0f);
-            d[1] = make_float4(c.x + 0.0f, c.y + 0.0f, e.x + 0.0f, e.y + 0.0f);
-        }
-    };
-    int v = threadIdx.x;
-    for (; v + 3 * T < vecs; v += 4 * T) {  // four loads in flight
-        uint4 w[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = __ldg(vsrc + v + j * T);
-#pragma unroll
-        for (int j = 0; j < 4; j++) put(v + j * T, w[j]);
-    }
-    for (; v < vecs; v += T) put(v, __ldg(vsrc + v));
+    for (int i = threadIdx.x; i < vecs; i += T) cp_async16(smem_u32(xs + head + i * kV), src + head + i * kV, true);
+    cp_async_commit();
+    for (int i = threadIdx.x; i < head; i += T) xs[i] = src[i];
+    for (int i = head + vecs * kV + threadIdx.x; i < cnt; i += T) xs[i] = src[i];
+    const float temp = p.temperature ? p.temperature[row] : 1.0f;
+    const int top_k = p.top_k ? p.top_k[row] : 0;
+    const float top_p = p.top_p ? p.top_p[row] : 1.0f;
+    const float min_p = p.min_p ? p.min_p[row] : 0.0f;
+    const double u = p.u[row];
+    cp_async_wait<0>();
     cluster_sync();  // the slice is there, and the cluster's other CTAs run: their shared memory can be written
-    uint32_t best = 0, at = 0x7fffffffu;  // order bits (of a NaN: all ones), index in the row
-    for (int i = threadIdx.x; i < cnt; i += T) {
-        const float x = xs[i];
+
+    // ---- its largest entry, the first of its equals; NaN ---------------------------
+    const int run = ((cnt + T - 1) / T) | 1;  // entries of a thread: odd, which spreads a warp over the banks
+    SampleRow<E, T> s{sh, reinterpret_cast<u64*>(smem), xs, min(cnt, (int)threadIdx.x * run), 0, rank, nr, 0, 0, 0.0f, 0.0f, 0.0};
+    s.b = min(cnt, s.a + run);
+    uint32_t best = 0, first = 0x7fffffffu;  // order bits (of a NaN: all ones), index in the row
+    for (int i = s.a; i < s.b; i++) {
+        const float x = s.at(i);
         const uint32_t ob = x != x ? 0xffffffffu : order_bits(x);
         if (ob > best) {
             best = ob;
-            at = lo + i;
+            first = lo + i;
         }
     }
-    SampleRow<T> s{sh, hist, xs, cnt, rank, nr, 0, 0, 0.0f, 0.0f, 0.0};
     const uint32_t top_bits = s.cluster_max(best);
-    const float temp = p.temperature ? p.temperature[row] : 1.0f;
     if (!(temp > 0.0f)) {
-        const uint32_t first = ~s.cluster_max(best == top_bits ? ~at : 0u);
+        first = ~s.cluster_max(best == top_bits ? ~first : 0u);
         if (rank == 0 && threadIdx.x == 0) {
             p.tok[row] = (int)first;
             if (p.logp) p.logp[row] = 0.0f;
@@ -369,91 +398,72 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
     uint32_t floor_key = 0;   // entries below are out
     int ties = 0x7fffffff;    // of the entries equal to tie_key, how many stay
     uint32_t tie_key = 0;
-    const int k = p.top_k ? p.top_k[row] : 0;
-    const float tp = p.top_p ? p.top_p[row] : 1.0f;
-    const float mp = p.min_p ? p.min_p[row] : 0.0f;
-    if (k > 0 && k < p.n) {
+    u64 mine = 0;             // mass that stays of the thread's run, as far as it is known:
+    int step = -1;            // that above this step
+    if (top_k > 0 && top_k < p.n) {
         u64 above;
-        floor_key = tie_key = s.find_end(true, (u64)k, 0, above);
-        ties = k - (int)above;
+        floor_key = tie_key = s.find_end(true, (u64)top_k, 0.0, 0, 0, above, mine, step);
+        ties = top_k - (int)above;
+        step = -1;
     }
-    if (tp < 1.0f) {
-        u64 m = 0;
-        for (int i = threadIdx.x; i < cnt; i += T) {
-            const float x = xs[i];
-            const uint32_t ob = order_bits(x);
-            if (s.has_mass(x) && (ob > tie_key || (ob == tie_key && ties == 0x7fffffff))) m += s.mass(x);
-        }
-        m = s.cluster_sum(m);
-        if (ties != 0x7fffffff) {  // those that stay of the entries equal to the last
-            u64 equal = 0;
-            for (int i = threadIdx.x; i < cnt; i += T) equal += order_bits(xs[i]) == tie_key ? 1 : 0;
+    if (top_p < 1.0f) {
+        u64 whole = 0;
+        if (ties != 0x7fffffff) {  // the mass of those top_k: few, with of the equal last ones those that stay
+            u64 m = 0, equal = 0;
+            for (int i = s.a; i < s.b; i++) {
+                const float x = s.at(i);
+                const uint32_t ob = order_bits(x);
+                if (ob > tie_key) m += s.mass(x);
+                equal += ob == tie_key ? 1 : 0;
+            }
             equal = s.cluster_sum(equal);
             if ((u64)ties > equal) ties = (int)equal;  // all entries with mass stay
-            m += (u64)ties * s.mass(order_value(tie_key));
+            whole = s.cluster_sum(m) + (u64)ties * s.mass(order_value(tie_key));
         }
-        const double want = ceil((double)tp * (double)m);
         u64 above;
-        floor_key = s.find_end(false, want >= 1.0 ? (u64)want : 1, floor_key, above);
+        floor_key = s.find_end(false, 0, (double)top_p, whole, floor_key, above, mine, step);
     }
-    const double oct_max = mp > 0.0f ? -log2((double)fminf(mp, 1.0f)) : 1e300;
+    const double oct_max = min_p > 0.0f ? -log2((double)fminf(min_p, 1.0f)) : 1e300;
+    const bool cut = ((double)top - (double)order_value(floor_key)) * s.oct > oct_max;  // min_p ends before
 
-    // ---- the draw: runs of the slice in index order, one to a thread -----------
-    const int E_ = ((cnt + T - 1) / T) | 1;  // odd: no bank twice in a warp
-    const int a = min(cnt, (int)threadIdx.x * E_), b = min(cnt, a + E_);
+    // ---- the draw, in index order --------------------------------------------------
     int tie_before = 0;  // entries equal to tie_key before this run
-    if (ties != 0x7fffffff && floor_key == tie_key) {
-        u64 mine = 0, lower;
-        for (int i = a; i < b; i++) mine += order_bits(xs[i]) == tie_key ? 1 : 0;
-        s.cluster_sum(mine, &lower);
-        u64 inc = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
-            if ((threadIdx.x & 31) >= o) inc += y;
-        }
-        __syncthreads();
-        if ((threadIdx.x & 31) == 31) sh.warp[threadIdx.x >> 5] = inc;
-        __syncthreads();
-        u64 before = lower + inc - mine;
-        for (int w = 0; w < (int)(threadIdx.x >> 5); w++) before += sh.warp[w];
-        tie_before = (int)before;
+    const bool few = ties != 0x7fffffff && floor_key == tie_key;
+    if (few) {
+        u64 eq = 0, lower;
+        for (int i = s.a; i < s.b; i++) eq += order_bits(s.at(i)) == tie_key ? 1 : 0;
+        s.cluster_sum(eq, &lower);
+        tie_before = (int)(lower + s.cta_before(eq));
     }
     auto kept = [&](int i, int& seen) -> u64 {  // the mass of entry i if it stays
-        const float x = xs[i];
+        const float x = s.at(i);
         const uint32_t ob = order_bits(x);
         if (ob < floor_key || !s.has_mass(x)) return 0;
-        if (ob == tie_key && ties != 0x7fffffff && seen++ >= ties) return 0;
+        if (few && ob == tie_key && seen++ >= ties) return 0;
         if (((double)top - (double)x) * s.oct > oct_max) return 0;
         return s.mass(x);
     };
-    u64 mine = 0;
     int seen = tie_before;
-    for (int i = a; i < b; i++) mine += kept(i, seen);
+    if (step < 0 || cut) {
+        mine = 0;
+        for (int i = s.a; i < s.b; i++) mine += kept(i, seen);
+    } else {  // what lies above the last search's step has been added up
+        for (int i = s.a; i < s.b; i++)
+            if ((int)s.key(s.at(i)) == step) mine += kept(i, seen);
+    }
     u64 lower;
     const u64 total = s.cluster_sum(mine, &lower);
-    u64 inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
-        if ((threadIdx.x & 31) >= o) inc += y;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 31) sh.warp[threadIdx.x >> 5] = inc;
-    __syncthreads();
-    u64 c = lower + inc - mine;
-    for (int w = 0; w < (int)(threadIdx.x >> 5); w++) c += sh.warp[w];
-    const double u = p.u[row];
+    u64 c = lower + s.cta_before(mine);
     const double want = (u > 0.0 ? u : 0.0) * (double)total;
     const u64 goal = want >= (double)total ? total - 1 : (u64)want;
     if (goal >= c && goal < c + mine) {  // one thread of the cluster
         seen = tie_before;
-        for (int i = a; i < b; i++) {
+        for (int i = s.a; i < s.b; i++) {
             c += kept(i, seen);
             if (c > goal) {
                 p.tok[row] = lo + i;
                 if (p.logp)
-                    p.logp[row] = (float)(-((double)top - (double)xs[i]) * s.oct * 0.6931471805599453094 -
+                    p.logp[row] = (float)(-((double)top - (double)s.at(i)) * s.oct * 0.6931471805599453094 -
                                           log((double)total / 17592186044416.0));
                 break;
             }
@@ -465,7 +475,7 @@ template <class E, int T>
 static int launch_sample_rows(const SampleRowsParams& p, int rows, int cluster, size_t smem, cudaStream_t st) {
     auto kern = sample_rows_kernel<E, T>;
     static PerDeviceOnce once;
-    if (smem_opt_in(once, kern, 216 * 1024) != cudaSuccess) return HQ4_ERR_LAUNCH;
+    if (smem_opt_in(once, kern, (int)kSrSmem) != cudaSuccess) return HQ4_ERR_LAUNCH;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -483,15 +493,41 @@ static int launch_sample_rows(const SampleRowsParams& p, int rows, int cluster, 
     return cudaLaunchKernelEx(&lc, kern, p) == cudaSuccess ? HQ4_OK : HQ4_ERR_LAUNCH;
 }
 
+// Shared memory of a CTA (without its static part).
+static size_t sr_smem(int n, int cluster, int threads, size_t elem) {
+    return (size_t)((n + cluster - 1) / cluster + 16) * elem + sizeof(u64) * kSrBins * threads;
+}
+
+// The largest cluster whose CTAs all fit the device at once (a row then takes
+// the least time), else the one with the fewest CTAs that holds a row; 512
+// threads, or 256 where that lets more CTAs share an SM or a slice fit.
 template <class E>
-static int sample_rows(SampleRowsParams p, int rows, cudaStream_t st) {
-    int cluster = kSrMaxCluster;
-    while (cluster > 1 && p.n / cluster < 2048) cluster >>= 1;
-    p.chunk = (p.n + cluster - 1) / cluster;
-    const size_t slice = (size_t)(p.chunk + 16) * sizeof(float);
-    if (slice + sizeof(u64) * kSrBins * 512 <= 216 * 1024)
-        return launch_sample_rows<E, 512>(p, rows, cluster, slice + sizeof(u64) * kSrBins * 512, st);
-    return launch_sample_rows<E, 256>(p, rows, cluster, slice + sizeof(u64) * kSrBins * 256, st);
+static int sample_rows(SampleRowsParams p, int rows, int sms, cudaStream_t st) {
+    int best_cluster = 0, best_threads = 0;
+    double best = 0.0;
+    for (int cluster = kSrMaxCluster; cluster >= 1; cluster >>= 1) {
+        if (cluster > 1 && p.n / cluster < 2048) continue;
+        for (int threads = 512; threads >= 256; threads >>= 1) {
+            const size_t smem = sr_smem(p.n, cluster, threads, sizeof(E));
+            if (smem > kSrSmem) continue;
+            const int per_sm = std::min<int>(2048 / threads, (int)(kSrSmem / (smem + 8 * 1024)) < 1 ? 1 : (int)(kSrSmem / (smem + 8 * 1024)));
+            const int at_once = std::max(1, sms * per_sm / cluster);  // rows
+            const double waves = (rows + at_once - 1) / at_once;
+            // a row's time: passes over its entries (shared by the CTAs of an SM), and the cluster's barriers
+            const double each = (double)p.n / cluster / threads * std::max(1.0, (double)std::min(per_sm, (rows * cluster + sms - 1) / sms) * threads / 512.0);
+            const double cost = waves * (each + 40.0 + 4.0 * cluster);
+            if (!best_cluster || cost < best) {
+                best = cost;
+                best_cluster = cluster;
+                best_threads = threads;
+            }
+        }
+    }
+    if (!best_cluster) return HQ4_ERR_SHAPE;
+    p.chunk = (p.n + best_cluster - 1) / best_cluster;
+    const size_t smem = sr_smem(p.n, best_cluster, best_threads, sizeof(E));
+    return best_threads == 512 ? launch_sample_rows<E, 512>(p, rows, best_cluster, smem, st)
+                               : launch_sample_rows<E, 256>(p, rows, best_cluster, smem, st);
 }
 
 }  // namespace hq4
@@ -522,7 +558,9 @@ extern "C" int hq4_sample_rows(const void* logits, int act_type, int n_rows, int
     p.tok = tok;
     p.logp = logprob;
     p.status = status_word();
+    const int sms = device_sms();
+    if (sms <= 0) return HQ4_ERR_LAUNCH;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return act_type == HQ4_F32 ? sample_rows<float>(p, n_rows, st)
-         : act_type == HQ4_BF16 ? sample_rows<__nv_bfloat16>(p, n_rows, st) : sample_rows<__half>(p, n_rows, st);
+    return act_type == HQ4_F32 ? sample_rows<float>(p, n_rows, sms, st)
+         : act_type == HQ4_BF16 ? sample_rows<__nv_bfloat16>(p, n_rows, sms, st) : sample_rows<__half>(p, n_rows, sms, st);
 }
