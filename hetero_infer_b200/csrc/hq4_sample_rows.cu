@@ -11,7 +11,7 @@
 // a row evenly -- four bits at a time; the few entries of the last step are
 // compared with one another.
 //
-// Masses are integers: w = floor(2^44 * 2^((x - max) / T * log2 e)) from fp64
+// Masses are integers: w = 2^44 * 2^((x - max) / T * log2 e) rounded, from fp64
 // arithmetic, at least 1, and 0 below 2^-44 of the maximum.  Their sums are
 // exact, so the token does not depend on how the work is divided, and the
 // cumulative bounds are off by less than 2^-40 of the whole, where fp32 sums
@@ -106,6 +106,7 @@ struct SampleRow {
     int rank, nr, turn, pturn;
     float top, steps;  // the maximum; steps of the search's keys for a unit of x
     double oct;        // octaves for a unit of x
+    double top_wide;   // the maximum
 
     __device__ __forceinline__ float at(int i) const { return Elem<E>::to(xs[i]) + 0.0f; }  // -0 counts as 0
     // Sum over the cluster; every thread gets it, and the sum of lower ranks.
@@ -164,34 +165,66 @@ struct SampleRow {
     // The search's key of x, at least kSrSteps for an entry without mass.
     __device__ __forceinline__ float key(float x) const { return (top - x) * steps; }
     __device__ __forceinline__ bool has_mass(float x) const { return key(x) < kSrSteps; }
-    // The mass of an entry that has some.  2^-f for f in [0, 1) by its Taylor
-    // series about 1/2: the term left out is below 2e-10.
-    __device__ u64 mass(float x) const {
-        const double z = ((double)top - (double)x) * oct;
-        const int e = (int)z;
-        const double t = (0.5 - (z - e)) * 0.6931471805599453094;  // ln(2^(1/2 - f))
-        double s = 1.0 / 40320.0;
-        s = fma(s, t, 1.0 / 5040.0);
-        s = fma(s, t, 1.0 / 720.0);
-        s = fma(s, t, 1.0 / 120.0);
-        s = fma(s, t, 1.0 / 24.0);
-        s = fma(s, t, 1.0 / 6.0);
-        s = fma(s, t, 0.5);
-        s = fma(s, t, 1.0);
-        s = fma(s, t, 1.0);
-        s *= 0.70710678118654752440 * 17592186044416.0;  // 2^-1/2 * 2^44
-        const u64 w = (u64)s >> min(e, 63);
+    static __device__ __forceinline__ double widen(float x) {
+        const uint32_t b = __float_as_uint(x);
+        return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
+    }
+    // The mass of an entry that has some: 2^-z = 2^-n 2^-f with n the nearest
+    // integer (left in the low bits by adding 1.5 * 2^52) and f in [-1/2, 1/2],
+    // whose power is its Taylor series (the term left out is below 2e-10); the
+    // last step scales it and rounds it to an integer in the low bits of 2^52.
+    // Conversions between types would be slower than all of this: the fp64
+    // value of x is put together from its bits (of a subnormal's or zero's,
+    // 2^-127 or less, something as small).
+    __device__ __forceinline__ u64 mass(float x) const {
+        const double z = (top_wide - widen(x)) * oct;
+        const double r = z + 6755399441055744.0;
+        const double f = z - (r - 6755399441055744.0);
+        const int n = __double2loint(r);
+        // (-ln 2)^k / k!
+        double s = 1.3215486790144307e-6;
+        s = fma(s, f, -1.5252733804059841e-5);
+        s = fma(s, f, 1.5403530393381609e-4);
+        s = fma(s, f, -1.3333558146428443e-3);
+        s = fma(s, f, 9.6181291076284772e-3);
+        s = fma(s, f, -5.5504108664821580e-2);
+        s = fma(s, f, 2.4022650695910071e-1);
+        s = fma(s, f, -6.9314718055994531e-1);
+        s = fma(s, f, 1.0);
+        const double m = fma(s, __hiloint2double((1023 + 44 - n) << 20, 0), 4503599627370496.0);
+        const u64 w = (u64)__double_as_longlong(m) & 0xfffffffffffffull;
         return w ? w : 1;
+    }
+    // f(x, i) of the run's entries four at a time, so that their arithmetic
+    // overlaps: first `pick` chooses, then the masses of the four are worked
+    // out, then `use` gets those of the chosen ones in order.
+    template <class Pick, class Use>
+    __device__ __forceinline__ void masses(bool counting, Pick pick, Use use) const {
+        for (int i = a; i < b; i += 4) {
+            float x[4];
+            bool on[4];
+            u64 w[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = i + j < b ? at(i + j) : -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; j++) on[j] = pick(x[j]);
+            if (!(on[0] || on[1] || on[2] || on[3])) continue;
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[j] = counting ? 1 : mass(x[j]);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (on[j]) use(x[j], w[j]);
+        }
     }
     __device__ __forceinline__ u64 weight(float x, bool counting) const { return counting ? 1 : mass(x); }
 
-    // The smallest value v >= floor_key's of an entry with mass such that the
+    // The order bits of the smallest value v >= floor of an entry with mass such that the
     // entries above it weigh less than the target (each its mass, or one), and
     // what those weigh.  The target is `count`, or, of the masses, share times
     // `whole` (of all masses where that is 0), at least 1, so that there is
     // such a value.  `mine` gets the masses of the thread's run above v's step;
     // `step` is that step.
-    __device__ uint32_t find_end(bool counting, u64 count, double share, u64 whole, uint32_t floor_key, u64& above,
+    __device__ uint32_t find_end(bool counting, u64 count, double share, u64 whole, float floor, u64& above,
                                  u64& mine, int& step) {
         u64 target = count;
         u64 before = 0;  // weight of the entries above the searched range
@@ -200,13 +233,12 @@ struct SampleRow {
         for (int shift = 2 * kSrDigit; shift >= 0; shift -= kSrDigit) {
 #pragma unroll
             for (int i = 0; i < kSrBins; i++) hist[i * T + threadIdx.x] = 0;
-#pragma unroll 2
-            for (int i = a; i < b; i++) {
-                const float x = at(i), k = key(x);
-                if (!(k < kSrSteps) || order_bits(x) < floor_key) continue;
-                const int f = (int)k >> shift;
-                if (f >> kSrDigit == prefix) hist[(f & (kSrBins - 1)) * T + threadIdx.x] += weight(x, counting);
-            }
+            masses(counting,
+                   [&](float x) {
+                       const float k = key(x);
+                       return k < kSrSteps && x >= floor && (int)k >> (shift + kSrDigit) == prefix;
+                   },
+                   [&](float x, u64 w) { hist[((int)key(x) >> shift & (kSrBins - 1)) * T + threadIdx.x] += w; });
             __syncthreads();
             const int lane = threadIdx.x & 31;
             for (int i = threadIdx.x >> 5; i < kSrBins; i += T / 32) {
@@ -262,9 +294,8 @@ struct SampleRow {
         uint32_t low = 0xffffffffu, high = 0;
         for (int i = a; i < b; i++) {
             const float x = at(i), k = key(x);
-            if (!(k < kSrSteps) || (int)k != prefix) continue;
+            if (!(k < kSrSteps) || (int)k != prefix || x < floor) continue;
             const uint32_t ob = order_bits(x);
-            if (ob < floor_key) continue;
             low = min(low, ob);
             high = max(high, ob);
             const uint32_t place = atom_add_cluster(head, 1);
@@ -361,7 +392,7 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
 
     // ---- its largest entry, the first of its equals; NaN ---------------------------
     const int run = ((cnt + T - 1) / T) | 1;  // entries of a thread: odd, which spreads a warp over the banks
-    SampleRow<E, T> s{sh, reinterpret_cast<u64*>(smem), xs, min(cnt, (int)threadIdx.x * run), 0, rank, nr, 0, 0, 0.0f, 0.0f, 0.0};
+    SampleRow<E, T> s{sh, reinterpret_cast<u64*>(smem), xs, min(cnt, (int)threadIdx.x * run), 0, rank, nr, 0, 0, 0.0f, 0.0f, 0.0, 0.0};
     s.b = min(cnt, s.a + run);
     uint32_t best = 0, first = 0x7fffffffu;  // order bits (of a NaN: all ones), index in the row
     for (int i = s.a; i < s.b; i++) {
@@ -392,17 +423,18 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
     }
     s.top = top;
     s.oct = 1.4426950408889634074 / (double)temp;
+    s.top_wide = s.widen(top);
     s.steps = fminf((float)(s.oct * (kSrSteps / kSrOctaves)), 1e30f);
 
     // ---- where the filters end ---------------------------------------------------
-    uint32_t floor_key = 0;   // entries below are out
-    int ties = 0x7fffffff;    // of the entries equal to tie_key, how many stay
-    uint32_t tie_key = 0;
+    float floor = -INFINITY;  // entries below are out
+    int ties = 0x7fffffff;    // of the entries equal to tie, how many stay
+    float tie = 0.0f;
     u64 mine = 0;             // mass that stays of the thread's run, as far as it is known:
     int step = -1;            // that above this step
     if (top_k > 0 && top_k < p.n) {
         u64 above;
-        floor_key = tie_key = s.find_end(true, (u64)top_k, 0.0, 0, 0, above, mine, step);
+        floor = tie = order_value(s.find_end(true, (u64)top_k, 0.0, 0, floor, above, mine, step));
         ties = top_k - (int)above;
         step = -1;
     }
@@ -410,46 +442,54 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
         u64 whole = 0;
         if (ties != 0x7fffffff) {  // the mass of those top_k: few, with of the equal last ones those that stay
             u64 m = 0, equal = 0;
-            for (int i = s.a; i < s.b; i++) {
-                const float x = s.at(i);
-                const uint32_t ob = order_bits(x);
-                if (ob > tie_key) m += s.mass(x);
-                equal += ob == tie_key ? 1 : 0;
-            }
+            s.masses(false, [&](float x) { return x >= tie; },
+                     [&](float x, u64 w) {
+                         if (x == tie) equal++;
+                         else m += w;
+                     });
             equal = s.cluster_sum(equal);
             if ((u64)ties > equal) ties = (int)equal;  // all entries with mass stay
-            whole = s.cluster_sum(m) + (u64)ties * s.mass(order_value(tie_key));
+            whole = s.cluster_sum(m) + (u64)ties * s.mass(tie);
         }
         u64 above;
-        floor_key = s.find_end(false, 0, (double)top_p, whole, floor_key, above, mine, step);
+        floor = order_value(s.find_end(false, 0, (double)top_p, whole, floor, above, mine, step));
     }
-    const double oct_max = min_p > 0.0f ? -log2((double)fminf(min_p, 1.0f)) : 1e300;
-    const bool cut = ((double)top - (double)order_value(floor_key)) * s.oct > oct_max;  // min_p ends before
+    if (min_p > 0.0f) {  // the smallest value that it keeps
+        const double most = -log2((double)fminf(min_p, 1.0f));
+        auto stays = [&](float x) { return ((double)top - (double)x) * s.oct <= most; };
+        const float guess = (float)((double)top - most / s.oct);
+        uint32_t k = order_bits(fminf(guess == guess ? guess : top, top) + 0.0f);
+        const uint32_t last = order_bits(top);
+        while (k < last && !stays(order_value(k))) k++;  // a rounding or two
+        while (k > 0x00800000u && stays(order_value(k - 1))) k--;
+        const float end = order_value(k) + 0.0f;
+        if (end > floor) {
+            floor = end;
+            step = -1;
+        }
+    }
 
     // ---- the draw, in index order --------------------------------------------------
-    int tie_before = 0;  // entries equal to tie_key before this run
-    const bool few = ties != 0x7fffffff && floor_key == tie_key;
+    const bool few = ties != 0x7fffffff && floor == tie;
+    int tie_before = 0;  // entries equal to the tie before this run
     if (few) {
         u64 eq = 0, lower;
-        for (int i = s.a; i < s.b; i++) eq += order_bits(s.at(i)) == tie_key ? 1 : 0;
+        for (int i = s.a; i < s.b; i++) eq += s.at(i) == tie ? 1 : 0;
         s.cluster_sum(eq, &lower);
         tie_before = (int)(lower + s.cta_before(eq));
     }
-    auto kept = [&](int i, int& seen) -> u64 {  // the mass of entry i if it stays
-        const float x = s.at(i);
-        const uint32_t ob = order_bits(x);
-        if (ob < floor_key || !s.has_mass(x)) return 0;
-        if (few && ob == tie_key && seen++ >= ties) return 0;
-        if (((double)top - (double)x) * s.oct > oct_max) return 0;
-        return s.mass(x);
-    };
     int seen = tie_before;
-    if (step < 0 || cut) {
+    // whether the next entry of the run stays (it is asked once for each, in order)
+    auto stays = [&](float x) {
+        if (x < floor || !s.has_mass(x)) return false;
+        return !(few && x == tie && seen++ >= ties);
+    };
+    if (step < 0) {
         mine = 0;
-        for (int i = s.a; i < s.b; i++) mine += kept(i, seen);
+        s.masses(false, stays, [&](float, u64 w) { mine += w; });
     } else {  // what lies above the last search's step has been added up
-        for (int i = s.a; i < s.b; i++)
-            if ((int)s.key(s.at(i)) == step) mine += kept(i, seen);
+        s.masses(false, [&](float x) { return s.has_mass(x) && (int)s.key(x) == step && stays(x); },
+                 [&](float, u64 w) { mine += w; });
     }
     u64 lower;
     const u64 total = s.cluster_sum(mine, &lower);
@@ -459,11 +499,12 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
     if (goal >= c && goal < c + mine) {  // one thread of the cluster
         seen = tie_before;
         for (int i = s.a; i < s.b; i++) {
-            c += kept(i, seen);
+            const float x = s.at(i);
+            if (stays(x)) c += s.mass(x);
             if (c > goal) {
                 p.tok[row] = lo + i;
                 if (p.logp)
-                    p.logp[row] = (float)(-((double)top - (double)s.at(i)) * s.oct * 0.6931471805599453094 -
+                    p.logp[row] = (float)(-((double)top - (double)x) * s.oct * 0.6931471805599453094 -
                                           log((double)total / 17592186044416.0));
                 break;
             }
