@@ -6,23 +6,23 @@
 // keeps, and the draw walks it in index order.  Nothing is sorted: a cluster of
 // CTAs holds a row in shared memory (read from memory once), and the value at
 // which a filter ends is found by a radix search.  Its keys are the distances
-// below the maximum in 2^12 equal steps over the 44 octaves that have mass --
-// a monotone function of the value whose digits, unlike the float's own, split
-// a row evenly -- four bits at a time; the few entries of the last step are
-// compared with one another.
+// below the maximum in 2^12 equal steps over the 44 octaves that have mass -- a
+// monotone function of the value whose digits, unlike the float's own, split a
+// row evenly.  A first digit's sums are taken in columns of shared memory, one
+// to a thread; the second's, of the few entries that the first leaves, by
+// shared-memory atomics; the entries of the last step are compared with one
+// another.  Where top-k keeps few entries, those alone are compared, and all
+// the rest of the work is theirs.
 //
-// Masses are integers: w = 2^44 * 2^((x - max) / T * log2 e) rounded, from fp64
-// arithmetic, at least 1, and 0 below 2^-44 of the maximum.  Their sums are
-// exact, so the token does not depend on how the work is divided, and the
-// cumulative bounds are off by less than 2^-40 of the whole, where fp32 sums
-// over 1.5e5 entries would be off by 1e-6 and move tokens.
+// Masses are integers of 2^-44 of the maximum's or so, at least 1, and 0 below
+// that, each good to 2e-9 of itself (see mass()).  Their
+// sums are exact, so the token does not depend on how the work is divided, and
+// rounding errors of fp32 sums over 1.5e5 entries, 1e-6 of the whole, which
+// would move tokens, do not arise.
 //
-// A digit's 16 sums are taken in columns of shared memory, one to a thread
-// (no atomics: equal addresses within a warp would queue), then over the
-// threads and the cluster.  A thread owns a run of consecutive entries, so its
-// columns above the end that is found add up to what its run contributes to
-// the draw, and only the thread in whose run the draw falls looks at single
-// entries again.
+// A thread owns a run of consecutive entries, so its columns above the end that
+// is found add up to what its run contributes to the draw, and only the thread
+// in whose run the draw falls looks at single entries again.
 #include <algorithm>
 
 #include "hq4_host.cuh"
@@ -33,14 +33,15 @@ namespace hq4 {
 int check_device_cap();
 int* status_word();
 
-constexpr int kSrDigit = 4;             // bits
-constexpr int kSrBins = 1 << kSrDigit;
-constexpr float kSrSteps = 4096.0f;    // of the search's keys
-constexpr double kSrOctaves = 44.0;    // that have mass
-constexpr int kSrList = 512;            // entries of one step that are compared directly
+constexpr int kSrBits = 12;              // of the search's keys
+constexpr float kSrSteps = 4096.0f;
+constexpr double kSrOctaves = 44.0;      // that have mass
+constexpr int kSrList = 128;             // entries of a CTA that are compared directly
+constexpr int kSrFew = 384;              // entries of a row that top-k may leave for that
 constexpr int kSrMaxCluster = 8;
-constexpr int kSrMaxSlice = 36864;     // entries of a CTA
-constexpr size_t kSrSmem = 212 * 1024;
+constexpr int kSrMaxSlice = 36864;       // entries of a CTA
+// Dynamic shared memory at most, by the bits of the first digit (the lists and sums take the rest).
+constexpr size_t sr_smem_max(int bits) { return (bits == 5 ? 204 : 196) * 1024; }
 
 struct SampleRowsParams {
     const void* x;
@@ -60,18 +61,8 @@ typedef unsigned long long u64;
 __device__ __forceinline__ void st_cluster_u64(uint32_t addr, u64 v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
-__device__ __forceinline__ u64 ld_cluster_u64(uint32_t addr) {
-    u64 v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
-    return v;
-}
 __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-__device__ __forceinline__ uint32_t atom_add_cluster(uint32_t addr, uint32_t v) {
-    uint32_t r;
-    asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(r) : "r"(addr), "r"(v) : "memory");
-    return r;
 }
 // Bits that order as the floats do, and back.
 __device__ __forceinline__ uint32_t order_bits(float x) {
@@ -82,33 +73,43 @@ __device__ __forceinline__ float order_value(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
-template <int T>
+// B1: bits of the first digit.
+template <int T, int B1>
 struct SampleRowsShared {
-    u64 all[2][kSrMaxCluster][kSrBins];  // the CTAs' sums of a digit, by turns
-    u64 sums[kSrBins];
+    static constexpr int kBins1 = 1 << B1, kBins2 = 1 << (kSrBits - B1);
+    uint32_t table[64];                  // 2^30 * 2^(1 - j / 64), and below 2^31
+    u64 all1[2][kSrMaxCluster][kBins1];  // the CTAs' sums of a digit; by turns for the two searches
+    u64 all2[kSrMaxCluster][kBins2];
+    uint32_t part[3][kBins2];            // this CTA's of the second digit: 15 bits of the masses each, or counts
     u64 warp[T / 32];
     u64 pair[2][kSrMaxCluster];          // a number of each CTA, by turns
-    uint32_t list[kSrList];              // rank 0's: keys of one step's entries, and their weights
-    u64 list_w[kSrList];
-    u64 target;
+    uint32_t key[kSrMaxCluster][kSrList], idx[kSrMaxCluster][kSrList];  // the CTAs' lists
+    uint32_t count[kSrMaxCluster];
     uint32_t n_list, best;
-    u64 best_above;
-    u64 bin_before;
+    u64 best_above, target, before, here;
     int bin;
 };
 
-template <class E, int T>
+template <class E, int T, int B1>
 struct SampleRow {
-    SampleRowsShared<T>& sh;
-    u64* hist;         // [kSrBins][T]
+    typedef SampleRowsShared<T, B1> Shared;
+    static constexpr int kBins1 = Shared::kBins1, kBins2 = Shared::kBins2, kB2 = kSrBits - B1;
+    Shared& sh;
+    u64* hist;         // [kBins1][T]; once a search is at its list, that list
     const E* xs;       // this CTA's slice
-    int a, b;          // the thread's run in it
+    int lo, a, b;      // its first entry in the row; the thread's run in it
     int rank, nr, turn, pturn;
     float top, steps;  // the maximum; steps of the search's keys for a unit of x
-    double oct;        // octaves for a unit of x
-    double top_wide;   // the maximum
+    float oct, oct_lo; // octaves for a unit of x, as a sum of two
+    float shift;       // 0, or the maximum where that is far from 0
+    int top_q;         // the maximum's 64ths of an octave, as mass() has them
 
+    __device__ __forceinline__ u64* list_mass() const { return hist; }
+    __device__ __forceinline__ u64* list_above() const { return hist + kSrMaxCluster * kSrList; }
+    // order bits, then the index inverted: of two entries the one that comes first is the larger
+    __device__ __forceinline__ u64* list_entry() const { return hist + 2 * kSrMaxCluster * kSrList; }
     __device__ __forceinline__ float at(int i) const { return Elem<E>::to(xs[i]) + 0.0f; }  // -0 counts as 0
+
     // Sum over the cluster; every thread gets it, and the sum of lower ranks.
     __device__ u64 cluster_sum(u64 v, u64* lower = nullptr) {
 #pragma unroll
@@ -122,13 +123,13 @@ struct SampleRow {
             st_cluster_u64(map_to_rank(smem_u32(&sh.pair[pturn][rank]), threadIdx.x), t);
         }
         cluster_sync();
-        u64 t = 0, lo = 0;
+        u64 t = 0, low = 0;
         for (int r = 0; r < nr; r++) {
-            if (r < rank) lo += sh.pair[pturn][r];
+            if (r < rank) low += sh.pair[pturn][r];
             t += sh.pair[pturn][r];
         }
         pturn ^= 1;
-        if (lower) *lower = lo;
+        if (lower) *lower = low;
         return t;
     }
     // Sum over the CTA's threads before this one.
@@ -145,6 +146,16 @@ struct SampleRow {
         u64 before = inc - v;
         for (int w = 0; w < (int)(threadIdx.x >> 5); w++) before += sh.warp[w];
         return before;
+    }
+    __device__ u64 cta_sum(u64 v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = v;
+        __syncthreads();
+        u64 t = 0;
+        for (int w = 0; w < T / 32; w++) t += sh.warp[w];
+        return t;
     }
     __device__ uint32_t cluster_max(uint32_t v) {  // of 32-bit numbers
         v = __reduce_max_sync(0xffffffffu, v);
@@ -165,37 +176,28 @@ struct SampleRow {
     // The search's key of x, at least kSrSteps for an entry without mass.
     __device__ __forceinline__ float key(float x) const { return (top - x) * steps; }
     __device__ __forceinline__ bool has_mass(float x) const { return key(x) < kSrSteps; }
-    static __device__ __forceinline__ double widen(float x) {
-        const uint32_t b = __float_as_uint(x);
-        return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
-    }
-    // The mass of an entry that has some: 2^-z = 2^-n 2^-f with n the nearest
-    // integer (left in the low bits by adding 1.5 * 2^52) and f in [-1/2, 1/2],
-    // whose power is its Taylor series (the term left out is below 2e-10); the
-    // last step scales it and rounds it to an integer in the low bits of 2^52.
-    // Conversions between types would be slower than all of this: the fp64
-    // value of x is put together from its bits (of a subnormal's or zero's,
-    // 2^-127 or less, something as small).
+    // The mass of an entry that has some, in fp32 and 32-bit integer
+    // arithmetic (fp64 is several times slower).  x * oct is Q / 64 + g: its
+    // product as a sum of two floats (a fused multiply-add gives the rounding
+    // error), Q the nearest integer (left in the low bits by adding 1.5 * 2^23),
+    // |g| <= 2^-7; 2^g - 1 is three terms of its series (the fourth is below
+    // 4e-11), at most 5.5e-3, as an integer of 2^-29 (9e-10); 2^(Q/64) comes
+    // from a table and a shift.  The maximum's own g is left in all masses
+    // alike, which changes no ratio: they are up to 2^(1/64) times 2^44.
     __device__ __forceinline__ u64 mass(float x) const {
-        const double z = (top_wide - widen(x)) * oct;
-        const double r = z + 6755399441055744.0;
-        const double f = z - (r - 6755399441055744.0);
-        const int n = __double2loint(r);
-        // (-ln 2)^k / k!
-        double s = 1.3215486790144307e-6;
-        s = fma(s, f, -1.5252733804059841e-5);
-        s = fma(s, f, 1.5403530393381609e-4);
-        s = fma(s, f, -1.3333558146428443e-3);
-        s = fma(s, f, 9.6181291076284772e-3);
-        s = fma(s, f, -5.5504108664821580e-2);
-        s = fma(s, f, 2.4022650695910071e-1);
-        s = fma(s, f, -6.9314718055994531e-1);
-        s = fma(s, f, 1.0);
-        const double m = fma(s, __hiloint2double((1023 + 44 - n) << 20, 0), 4503599627370496.0);
-        const u64 w = (u64)__double_as_longlong(m) & 0xfffffffffffffull;
-        return w ? w : 1;
+        x -= shift;
+        const float z = x * oct;
+        const float zl = fmaf(x, oct_lo, fmaf(x, oct, -z));
+        const float q = fmaf(z, 64.0f, 12582912.0f);
+        const float g = fmaf(q - 12582912.0f, -0.015625f, z) + zl;
+        const float m = g * fmaf(g, fmaf(g, 5.5504109e-2f, 2.4022651e-1f), 6.9314718e-1f);
+        const int mi = __float_as_int(fmaf(m, 536870912.0f, 12582912.0f)) - 0x4b400000;
+        const int Q = top_q - (int)__float_as_uint(q);  // 64ths of an octave below the maximum
+        const uint32_t w = sh.table[Q & 63];            // 2^30 to 2^31
+        const u64 y = ((u64)(w + __mulhi((int)w, mi << 3)) << 32) >> ((19 + (Q >> 6)) & 63);
+        return y ? y : 1;
     }
-    // f(x, i) of the run's entries four at a time, so that their arithmetic
+    // f(x, w, i) of the run's entries four at a time, so that their arithmetic
     // overlaps: first `pick` chooses, then the masses of the four are worked
     // out, then `use` gets those of the chosen ones in order.
     template <class Pick, class Use>
@@ -213,160 +215,241 @@ struct SampleRow {
             for (int j = 0; j < 4; j++) w[j] = counting ? 1 : mass(x[j]);
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                if (on[j]) use(x[j], w[j]);
+                if (on[j]) use(x[j], w[j], i + j);
         }
     }
-    __device__ __forceinline__ u64 weight(float x, bool counting) const { return counting ? 1 : mass(x); }
 
-    // The order bits of the smallest value v >= floor of an entry with mass such that the
-    // entries above it weigh less than the target (each its mass, or one), and
-    // what those weigh.  The target is `count`, or, of the masses, share times
-    // `whole` (of all masses where that is 0), at least 1, so that there is
-    // such a value.  `mine` gets the masses of the thread's run above v's step;
-    // `step` is that step.
-    __device__ uint32_t find_end(bool counting, u64 count, double share, u64 whole, float floor, u64& above,
-                                 u64& mine, int& step) {
-        u64 target = count;
-        u64 before = 0;  // weight of the entries above the searched range
-        int prefix = 0;  // the key's digits so far
-        mine = 0;
-        for (int shift = 2 * kSrDigit; shift >= 0; shift -= kSrDigit) {
-#pragma unroll
-            for (int i = 0; i < kSrBins; i++) hist[i * T + threadIdx.x] = 0;
-            masses(counting,
-                   [&](float x) {
-                       const float k = key(x);
-                       return k < kSrSteps && x >= floor && (int)k >> (shift + kSrDigit) == prefix;
-                   },
-                   [&](float x, u64 w) { hist[((int)key(x) >> shift & (kSrBins - 1)) * T + threadIdx.x] += w; });
-            __syncthreads();
-            const int lane = threadIdx.x & 31;
-            for (int i = threadIdx.x >> 5; i < kSrBins; i += T / 32) {
-                u64 v = 0;
-#pragma unroll
-                for (int j = 0; j < T / 32; j++) v += hist[i * T + j * 32 + lane];
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                if (lane < nr) st_cluster_u64(map_to_rank(smem_u32(&sh.all[turn][rank][i]), lane), v);
-            }
-            cluster_sync();
-            if (threadIdx.x < 32) {  // a bin to a lane
-                u64 v = 0;
-                if (lane < kSrBins)
-                    for (int r = 0; r < nr; r++) v += sh.all[turn][r][lane];
-                u64 upto = v;
-#pragma unroll
-                for (int o = 1; o < kSrBins; o <<= 1) {
-                    const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += y;
-                }
-                if (!counting && shift == 2 * kSrDigit) {
-                    const u64 all = whole ? whole : __shfl_sync(0xffffffffu, upto, kSrBins - 1);
-                    const double want = ceil(share * (double)all);
-                    target = want >= 1.0 ? (u64)want : 1;
-                    if (lane == 0) sh.target = target;
-                }
-                const u64 excl = before + upto - v;
-                const uint32_t ok = __ballot_sync(0xffffffffu, v != 0 && excl < target);
-                const int i = ok ? 31 - __clz(ok) : 0;  // the last step that begins below the target
-                if (lane == i) {
-                    sh.bin = i;
-                    sh.bin_before = excl;
-                }
-            }
-            __syncthreads();
-            turn ^= 1;
-            if (!counting) target = sh.target;
-            before = sh.bin_before;
-            const int bin = sh.bin;
-            if (!counting)
-                for (int i = 0; i < bin; i++) mine += hist[i * T + threadIdx.x];
-            prefix = prefix << kSrDigit | bin;
+    // The bin among n (the cluster's sums in all[r][.]) that is the last to
+    // begin below the target, with what lies before it and in it; `base` is
+    // what lies before the first.  Thread i < n looks after bin i.
+    template <int kBins>
+    __device__ int find_bin(const u64 (*all)[kBins], u64 base, u64 target, u64& before, u64& here) {
+        static_assert(kBins <= T, "a bin to a thread");
+        u64 v = 0;
+        if ((int)threadIdx.x < kBins)
+            for (int r = 0; r < nr; r++) v += all[r][threadIdx.x];
+        if (threadIdx.x == 0) sh.bin = 0;
+        const u64 excl = base + cta_before(v);  // (has barriers)
+        const bool ok = v != 0 && excl < target;
+        const uint32_t any = __ballot_sync(0xffffffffu, ok);
+        if (any && (threadIdx.x & 31) == 31 - __clz(any)) atomicMax(&sh.bin, (int)threadIdx.x);
+        __syncthreads();
+        const int bin = sh.bin;
+        if ((int)threadIdx.x == bin) {
+            sh.before = excl;
+            sh.here = v;
         }
-        step = prefix;
-        // the entries of the last step
+        __syncthreads();
+        before = sh.before;
+        here = sh.here;
+        return bin;
+    }
+
+    // Where a filter ends.
+    struct End {
+        float v;        // the value, once it is known
+        u64 above;      // what the entries above it weigh (each its mass, or one)
+        u64 mine;       // mass of the thread's run above the value's step
+        int step;       // that step
+        int i0, i1;     // the entries of the run in that step lie in [i0, i1)
+        bool listed;    // not resolved: the list holds all entries down to that step,
+        int n;          // so many
+    };
+    // The smallest value v >= floor of an entry with mass such that the entries
+    // above it weigh less than the target.  The target is `count`, or, of the
+    // masses, share times `whole` (of all masses where that is 0), at least 1,
+    // so that there is such a value.
+    __device__ End find_end(bool counting, u64 count, double share, u64 whole, float floor) {
+        End e = {};
+        // first digit
+#pragma unroll
+        for (int i = 0; i < kBins1; i++) hist[i * T + threadIdx.x] = 0;
+        masses(counting, [&](float x) { return has_mass(x) && x >= floor; },
+               [&](float x, u64 w, int) { hist[((int)key(x) >> kB2) * T + threadIdx.x] += w; });
+        for (int i = threadIdx.x; i < 3 * kBins2; i += T) sh.part[0][i] = 0;
+        __syncthreads();
+        const int lane = threadIdx.x & 31;
+        for (int i = threadIdx.x >> 5; i < kBins1; i += T / 32) {
+            u64 v = 0;
+#pragma unroll
+            for (int j = 0; j < T / 32; j++) v += hist[i * T + j * 32 + lane];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (lane < nr) st_cluster_u64(map_to_rank(smem_u32(&sh.all1[turn][rank][i]), lane), v);
+        }
+        cluster_sync();
+        u64 target = count, before, here;
+        if (!counting) {
+            u64 all = whole;
+            if (!all)
+                for (int i = lane; i < kBins1 * nr; i += 32) all += sh.all1[turn][i / kBins1][i % kBins1];
+            if (!whole)
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+            const double want = ceil(share * (double)all);
+            target = want >= 1.0 ? (u64)want : 1;
+        }
+        const int bin1 = find_bin<kBins1>(sh.all1[turn], 0, target, before, here);
+        turn ^= 1;
+        if (!counting)
+            for (int i = 0; i < bin1; i++) e.mine += hist[i * T + threadIdx.x];
+        // second digit, of the entries that have the first
+        masses(counting,
+               [&](float x) { return has_mass(x) && x >= floor && (int)key(x) >> kB2 == bin1; },
+               [&](float x, u64 w, int) {
+                   const int i = (int)key(x) & (kBins2 - 1);
+                   atomicAdd(&sh.part[0][i], (uint32_t)w & 0x7fffu);
+                   if (!counting) {
+                       atomicAdd(&sh.part[1][i], (uint32_t)(w >> 15) & 0x7fffu);
+                       atomicAdd(&sh.part[2][i], (uint32_t)(w >> 30));
+                   }
+               });
         if (threadIdx.x == 0) {
             sh.n_list = 0;
             sh.best = 0xffffffffu;
         }
-        cluster_sync();
-        const uint32_t head = map_to_rank(smem_u32(&sh.n_list), 0);
-        uint32_t low = 0xffffffffu, high = 0;
-        for (int i = a; i < b; i++) {
-            const float x = at(i), k = key(x);
-            if (!(k < kSrSteps) || (int)k != prefix || x < floor) continue;
-            const uint32_t ob = order_bits(x);
-            low = min(low, ob);
-            high = max(high, ob);
-            const uint32_t place = atom_add_cluster(head, 1);
-            if (place < kSrList) st_cluster_u32(map_to_rank(smem_u32(&sh.list[place]), 0), ob);
+        __syncthreads();
+        for (int i = threadIdx.x; i < kBins2 * nr; i += T) {
+            const int k = i & (kBins2 - 1);
+            st_cluster_u64(map_to_rank(smem_u32(&sh.all2[rank][k]), i >> kB2),
+                           (u64)sh.part[0][k] + ((u64)sh.part[1][k] << 15) + ((u64)sh.part[2][k] << 30));
         }
         cluster_sync();
-        const uint32_t n = (uint32_t)ld_cluster_u32(head);
-        if (n <= kSrList) {
-            if (rank == 0) {
-                for (uint32_t i = threadIdx.x; i < n; i += T) sh.list_w[i] = weight(order_value(sh.list[i]), counting);
-                __syncthreads();
-                for (uint32_t i = threadIdx.x; i < n; i += T) {
-                    const uint32_t key_i = sh.list[i];
-                    u64 w = before;
-                    for (uint32_t j = 0; j < n; j++)
-                        if (sh.list[j] > key_i) w += sh.list_w[j];
-                    if (w < target) atomicMin(&sh.best, key_i);
-                }
-                __syncthreads();
-                const uint32_t v = sh.best;
-                u64 w = 0;
-                for (uint32_t i = threadIdx.x; i < n; i += T)
-                    if (sh.list[i] > v) w += sh.list_w[i];
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-                if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = w;
-                __syncthreads();
-                if (threadIdx.x == 0) {
-                    w = before;
-                    for (int i = 0; i < T / 32; i++) w += sh.warp[i];
-                    sh.best_above = w;
-                }
+        const u64 base = before;
+        const int bin2 = find_bin<kBins2>(sh.all2, base, target, before, here);
+        e.step = bin1 << kB2 | bin2;
+        // the entries of the last step; or, where top-k ends early, all down to it
+        const bool few = counting && before + here <= kSrFew;
+        e.i0 = e.i1 = 0;
+        const int low_key = few ? 0 : counting ? e.step : bin1 << kB2;
+        masses(counting,
+               [&](float x) {
+                   const float k = key(x);
+                   return k < (float)(e.step + 1) && (int)k >= low_key && x >= floor;
+               },
+               [&](float x, u64 w, int i) {
+                   if (!few && (int)key(x) < e.step) {
+                       e.mine += w;
+                       return;
+                   }
+                   if (e.i1 == 0) e.i0 = i;
+                   e.i1 = i + 1;
+                   const uint32_t place = atomicAdd(&sh.n_list, 1);
+                   if (place < kSrList) {
+                       sh.key[rank][place] = order_bits(x);
+                       sh.idx[rank][place] = lo + i;
+                   }
+               });
+        if (counting) e.mine = 0;
+        __syncthreads();
+        const uint32_t n_mine = sh.n_list;
+        for (int i = threadIdx.x; i < (int)min(n_mine, (uint32_t)kSrList) * nr; i += T) {
+            const int k = i / nr, r = i - k * nr;
+            if (r == rank) continue;
+            st_cluster_u32(map_to_rank(smem_u32(&sh.key[rank][k]), r), sh.key[rank][k]);
+            st_cluster_u32(map_to_rank(smem_u32(&sh.idx[rank][k]), r), sh.idx[rank][k]);
+        }
+        if ((int)threadIdx.x < nr) st_cluster_u32(map_to_rank(smem_u32(&sh.count[rank]), threadIdx.x), n_mine);
+        cluster_sync();
+        bool fits = true;
+        int n_all = 0;
+        for (int r = 0; r < nr; r++) {
+            fits = fits && sh.count[r] <= kSrList;
+            n_all += (int)sh.count[r];
+        }
+        if (fits) {
+            // one list of all CTAs', in every CTA alike
+            for (int i = threadIdx.x; i < n_all; i += T) {
+                int r = 0, j = i;
+                while (j >= (int)sh.count[r]) j -= (int)sh.count[r++];
+                const uint32_t k = sh.key[r][j];
+                list_entry()[i] = (u64)k << 32 | ~sh.idx[r][j];
+                list_mass()[i] = counting && !few ? 1 : mass(order_value(k));
             }
-            cluster_sync();
-            const uint32_t v = ld_cluster_u32(map_to_rank(smem_u32(&sh.best), 0));
-            above = ld_cluster_u64(map_to_rank(smem_u32(&sh.best_above), 0));
-            cluster_sync();  // rank 0 may begin another search
-            return v;
+            __syncthreads();
+            e.n = n_all;
+            if (few) {
+                e.listed = true;
+                return e;
+            }
+            for (int i = threadIdx.x; i < n_all; i += T) {
+                const uint32_t k = (uint32_t)(list_entry()[i] >> 32);
+                u64 w = before;
+#pragma unroll 8
+                for (int j = 0; j < n_all; j++)
+                    if ((uint32_t)(list_entry()[j] >> 32) > k) w += list_mass()[j];
+                list_above()[i] = w;
+                if (w < target) atomicMin(&sh.best, k);
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < n_all; i += T)
+                if ((uint32_t)(list_entry()[i] >> 32) == sh.best) sh.best_above = list_above()[i];
+            __syncthreads();
+            e.v = order_value(sh.best);
+            e.above = sh.best_above;
+            __syncthreads();
+            return e;
         }
         // many entries within one step (equal ones, or a high temperature): bisection over their order
-        uint32_t lo = ~cluster_max(~low), hi = cluster_max(high);  // lo <= the end <= hi
-        above = before;
-        while (lo < hi) {
-            const uint32_t mid = lo + ((hi - lo) >> 1);
+        e.i0 = a;
+        e.i1 = b;
+        uint32_t low = 0xffffffffu, high = 0;
+        auto in_step = [&](float x) { return has_mass(x) && x >= floor && (int)key(x) == e.step; };
+        for (int i = a; i < b; i++) {
+            const float x = at(i);
+            if (!in_step(x)) continue;
+            low = min(low, order_bits(x));
+            high = max(high, order_bits(x));
+        }
+        low = ~cluster_max(~low);
+        high = cluster_max(high);  // low <= the end <= high
+        e.above = before;
+        while (low < high) {
+            const uint32_t mid = low + ((high - low) >> 1);
+            const float v = order_value(mid);
             u64 w = 0;
-            for (int i = a; i < b; i++) {
-                const float x = at(i), k = key(x);
-                if (k < kSrSteps && (int)k == prefix && order_bits(x) > mid) w += weight(x, counting);
-            }
+            masses(counting, [&](float x) { return in_step(x) && x > v; }, [&](float, u64 m, int) { w += m; });
             w = before + cluster_sum(w);
             if (w < target) {
-                hi = mid;
-                above = w;
+                high = mid;
+                e.above = w;
             } else {
-                lo = mid + 1;
+                low = mid + 1;
             }
         }
-        return lo;
-    }
-    static __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
-        uint32_t v;
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-        return v;
+        e.v = order_value(low);
+        return e;
     }
 };
 
-template <class E, int T>
+// The smallest value that min_p keeps (above -inf; at most the maximum).
+__device__ __forceinline__ float min_p_end(float min_p, float top, double oct) {
+    const double most = -log2((double)fminf(min_p, 1.0f));
+    auto stays = [&](float x) { return ((double)top - (double)x) * oct <= most; };
+    const float guess = (float)((double)top - most / oct);
+    uint32_t k = order_bits(fminf(guess == guess ? guess : top, top) + 0.0f);
+    const uint32_t last = order_bits(top);
+    while (k < last && !stays(order_value(k))) k++;  // a rounding or two
+    while (k > 0x00800000u && stays(order_value(k - 1))) k--;
+    return order_value(k) + 0.0f;
+}
+// The place in [0, total) that u falls on.
+__device__ __forceinline__ u64 draw_place(double u, u64 total) {
+    const double want = (u > 0.0 ? u : 0.0) * (double)total;
+    return want >= (double)total ? total - 1 : (u64)want;
+}
+// The log of 2^((x - max) oct) over the total; the maximum's mass says what the total is counted in.
+template <class Row>
+__device__ __forceinline__ float log_prob(float x, const Row& s, double oct, u64 total) {
+    return (float)(-((double)s.top - (double)x) * oct * 0.6931471805599453094 - log((double)total / (double)s.mass(s.top)));
+}
+
+template <class E, int T, int B1>
 __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p) {
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ SampleRowsShared<T> sh;
+    __shared__ SampleRowsShared<T, B1> sh;
     pdl_launch_dependents();
+    if (threadIdx.x < 64) sh.table[threadIdx.x] = (uint32_t)fmin(exp2(31.0 - threadIdx.x / 64.0) + 0.5, 2147483647.0);
     pdl_wait();
     const int rank = (int)cluster_ctarank(), nr = (int)cluster_nctarank();
     const int row = blockIdx.x / nr;
@@ -374,7 +457,7 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
     const E* src = static_cast<const E*>(p.x) + (long long)row * p.stride + lo;
     constexpr int kV = 16 / sizeof(E);
     const int off = (int)((uintptr_t)src & 15) / (int)sizeof(E);  // the slice keeps the row's alignment
-    E* xs = reinterpret_cast<E*>(smem + sizeof(u64) * kSrBins * T) + off;
+    E* xs = reinterpret_cast<E*>(smem + sizeof(u64) * (1 << B1) * T) + off;
 
     // ---- the slice, all copies in flight at once ---------------------------------
     const int head = min(cnt, (kV - off) % kV), vecs = (cnt - head) / kV;
@@ -392,7 +475,8 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
 
     // ---- its largest entry, the first of its equals; NaN ---------------------------
     const int run = ((cnt + T - 1) / T) | 1;  // entries of a thread: odd, which spreads a warp over the banks
-    SampleRow<E, T> s{sh, reinterpret_cast<u64*>(smem), xs, min(cnt, (int)threadIdx.x * run), 0, rank, nr, 0, 0, 0.0f, 0.0f, 0.0, 0.0};
+    SampleRow<E, T, B1> s{sh, reinterpret_cast<u64*>(smem), xs, lo, min(cnt, (int)threadIdx.x * run), 0, rank, nr,
+                          0, 0, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0};
     s.b = min(cnt, s.a + run);
     uint32_t best = 0, first = 0x7fffffffu;  // order bits (of a NaN: all ones), index in the row
     for (int i = s.a; i < s.b; i++) {
@@ -421,29 +505,79 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
         }
         return;
     }
+    const double oct = 1.4426950408889634074 / (double)temp;
     s.top = top;
-    s.oct = 1.4426950408889634074 / (double)temp;
-    s.top_wide = s.widen(top);
-    s.steps = fminf((float)(s.oct * (kSrSteps / kSrOctaves)), 1e30f);
+    s.oct = (float)fmin(oct, 1e30);
+    s.oct_lo = (float)(fmin(oct, 1e30) - (double)s.oct);
+    // a maximum of so many octaves: the entries within 44 of it are so near that their distance to it is exact
+    s.shift = fabs((double)top * oct) < 60000.0 ? 0.0f : top;
+    s.top_q = (int)__float_as_uint(fmaf((top - s.shift) * s.oct, 64.0f, 12582912.0f));
+    s.steps = fminf((float)(oct * (kSrSteps / kSrOctaves)), 1e30f);
 
     // ---- where the filters end ---------------------------------------------------
     float floor = -INFINITY;  // entries below are out
     int ties = 0x7fffffff;    // of the entries equal to tie, how many stay
     float tie = 0.0f;
-    u64 mine = 0;             // mass that stays of the thread's run, as far as it is known:
-    int step = -1;            // that above this step
+    typename SampleRow<E, T, B1>::End e = {};
+    bool summed = false;      // e.mine holds the thread's mass above e.step
+    const float p_end = min_p > 0.0f ? min_p_end(min_p, top, oct) : -INFINITY;
     if (top_k > 0 && top_k < p.n) {
-        u64 above;
-        floor = tie = order_value(s.find_end(true, (u64)top_k, 0.0, 0, floor, above, mine, step));
-        ties = top_k - (int)above;
-        step = -1;
+        e = s.find_end(true, (u64)top_k, 0.0, 0, floor);
+        if (e.listed) {
+            // ---- few entries: all of them against one another, in every CTA alike ------
+            // ranks, and what lies above each; then the draw among those that stay
+            u64 *above = s.list_above(), *mass = s.list_mass(), *entry = s.list_entry();
+            u64 kept = 0;
+            for (int i = threadIdx.x; i < e.n; i += T) {
+                const u64 me = entry[i];
+                u64 w = 0;
+                int before = 0;
+#pragma unroll 8
+                for (int j = 0; j < e.n; j++) {
+                    const u64 other = entry[j];
+                    if ((uint32_t)(other >> 32) > (uint32_t)(me >> 32)) w += mass[j];
+                    before += other > me ? 1 : 0;
+                }
+                above[i] = before >= top_k ? ~0ull : w;  // (never below a target)
+                if (before < top_k) kept += mass[i];
+            }
+            u64 target = ~0ull;
+            if (top_p < 1.0f) {
+                const double want = ceil((double)top_p * (double)s.cta_sum(kept));
+                target = want >= 1.0 ? (u64)want : 1;
+            }
+            __syncthreads();
+            kept = 0;
+            for (int i = threadIdx.x; i < e.n; i += T) {
+                const float x = order_value((uint32_t)(entry[i] >> 32));
+                if (!(above[i] < target) || x < p_end) mass[i] = 0;
+                kept += mass[i];
+            }
+            const u64 total = s.cta_sum(kept);  // (its barriers: the masses are written)
+            const u64 goal = draw_place(u, total);
+            if (rank == 0)
+                for (int i = threadIdx.x; i < e.n; i += T) {
+                    const uint32_t me = (uint32_t)entry[i];
+                    u64 c = 0;
+#pragma unroll 8
+                    for (int j = 0; j < e.n; j++)
+                        if ((uint32_t)entry[j] > me) c += mass[j];  // a lower index
+                    if (mass[i] && goal >= c && goal < c + mass[i]) {
+                        p.tok[row] = (int)~me;
+                        if (p.logp) p.logp[row] = log_prob(order_value((uint32_t)(entry[i] >> 32)), s, oct, total);
+                    }
+                }
+            return;
+        }
+        floor = tie = e.v;
+        ties = top_k - (int)e.above;
     }
     if (top_p < 1.0f) {
         u64 whole = 0;
-        if (ties != 0x7fffffff) {  // the mass of those top_k: few, with of the equal last ones those that stay
+        if (ties != 0x7fffffff) {  // the mass of those top_k, with of the equal last ones those that stay
             u64 m = 0, equal = 0;
             s.masses(false, [&](float x) { return x >= tie; },
-                     [&](float x, u64 w) {
+                     [&](float x, u64 w, int) {
                          if (x == tie) equal++;
                          else m += w;
                      });
@@ -451,28 +585,19 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
             if ((u64)ties > equal) ties = (int)equal;  // all entries with mass stay
             whole = s.cluster_sum(m) + (u64)ties * s.mass(tie);
         }
-        u64 above;
-        floor = order_value(s.find_end(false, 0, (double)top_p, whole, floor, above, mine, step));
+        e = s.find_end(false, 0, (double)top_p, whole, floor);
+        floor = e.v;
+        summed = true;
     }
-    if (min_p > 0.0f) {  // the smallest value that it keeps
-        const double most = -log2((double)fminf(min_p, 1.0f));
-        auto stays = [&](float x) { return ((double)top - (double)x) * s.oct <= most; };
-        const float guess = (float)((double)top - most / s.oct);
-        uint32_t k = order_bits(fminf(guess == guess ? guess : top, top) + 0.0f);
-        const uint32_t last = order_bits(top);
-        while (k < last && !stays(order_value(k))) k++;  // a rounding or two
-        while (k > 0x00800000u && stays(order_value(k - 1))) k--;
-        const float end = order_value(k) + 0.0f;
-        if (end > floor) {
-            floor = end;
-            step = -1;
-        }
+    if (p_end > floor) {
+        floor = p_end;
+        summed = false;
     }
 
     // ---- the draw, in index order --------------------------------------------------
-    const bool few = ties != 0x7fffffff && floor == tie;
+    const bool tied = ties != 0x7fffffff && floor == tie;
     int tie_before = 0;  // entries equal to the tie before this run
-    if (few) {
+    if (tied) {
         u64 eq = 0, lower;
         for (int i = s.a; i < s.b; i++) eq += s.at(i) == tie ? 1 : 0;
         s.cluster_sum(eq, &lower);
@@ -482,20 +607,22 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
     // whether the next entry of the run stays (it is asked once for each, in order)
     auto stays = [&](float x) {
         if (x < floor || !s.has_mass(x)) return false;
-        return !(few && x == tie && seen++ >= ties);
+        return !(tied && x == tie && seen++ >= ties);
     };
-    if (step < 0) {
-        mine = 0;
-        s.masses(false, stays, [&](float, u64 w) { mine += w; });
-    } else {  // what lies above the last search's step has been added up
-        s.masses(false, [&](float x) { return s.has_mass(x) && (int)s.key(x) == step && stays(x); },
-                 [&](float, u64 w) { mine += w; });
+    u64 mine = 0;
+    if (!summed) {
+        s.masses(false, stays, [&](float, u64 w, int) { mine += w; });
+    } else {  // what lies above the search's last step has been added up
+        mine = e.mine;
+        for (int i = e.i0; i < e.i1; i++) {
+            const float x = s.at(i);
+            if (s.has_mass(x) && (int)s.key(x) == e.step && stays(x)) mine += s.mass(x);
+        }
     }
     u64 lower;
     const u64 total = s.cluster_sum(mine, &lower);
     u64 c = lower + s.cta_before(mine);
-    const double want = (u > 0.0 ? u : 0.0) * (double)total;
-    const u64 goal = want >= (double)total ? total - 1 : (u64)want;
+    const u64 goal = draw_place(u, total);
     if (goal >= c && goal < c + mine) {  // one thread of the cluster
         seen = tie_before;
         for (int i = s.a; i < s.b; i++) {
@@ -503,20 +630,18 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
             if (stays(x)) c += s.mass(x);
             if (c > goal) {
                 p.tok[row] = lo + i;
-                if (p.logp)
-                    p.logp[row] = (float)(-((double)top - (double)x) * s.oct * 0.6931471805599453094 -
-                                          log((double)total / 17592186044416.0));
+                if (p.logp) p.logp[row] = log_prob(x, s, oct, total);
                 break;
             }
         }
     }
 }
 
-template <class E, int T>
+template <class E, int T, int B1>
 static int launch_sample_rows(const SampleRowsParams& p, int rows, int cluster, size_t smem, cudaStream_t st) {
-    auto kern = sample_rows_kernel<E, T>;
+    auto kern = sample_rows_kernel<E, T, B1>;
     static PerDeviceOnce once;
-    if (smem_opt_in(once, kern, (int)kSrSmem) != cudaSuccess) return HQ4_ERR_LAUNCH;
+    if (smem_opt_in(once, kern, (int)sr_smem_max(B1)) != cudaSuccess) return HQ4_ERR_LAUNCH;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -534,41 +659,37 @@ static int launch_sample_rows(const SampleRowsParams& p, int rows, int cluster, 
     return cudaLaunchKernelEx(&lc, kern, p) == cudaSuccess ? HQ4_OK : HQ4_ERR_LAUNCH;
 }
 
-// Shared memory of a CTA (without its static part).
-static size_t sr_smem(int n, int cluster, int threads, size_t elem) {
-    return (size_t)((n + cluster - 1) / cluster + 16) * elem + sizeof(u64) * kSrBins * threads;
-}
+// How a row is divided: CTAs, their threads, bits of the first digit.
+struct SrShape {
+    int cluster, threads, bits;
+    size_t smem;
+};
 
-// The largest cluster whose CTAs all fit the device at once (a row then takes
-// the least time), else the one with the fewest CTAs that holds a row; 512
-// threads, or 256 where that lets more CTAs share an SM or a slice fit.
 template <class E>
 static int sample_rows(SampleRowsParams p, int rows, int sms, cudaStream_t st) {
-    int best_cluster = 0, best_threads = 0;
-    double best = 0.0;
+    SrShape best = {0, 0, 0, 0};
+    double best_cost = 0.0;
     for (int cluster = kSrMaxCluster; cluster >= 1; cluster >>= 1) {
         if (cluster > 1 && p.n / cluster < 2048) continue;
-        for (int threads = 512; threads >= 256; threads >>= 1) {
-            const size_t smem = sr_smem(p.n, cluster, threads, sizeof(E));
-            if (smem > kSrSmem) continue;
-            const int per_sm = std::min<int>(2048 / threads, (int)(kSrSmem / (smem + 8 * 1024)) < 1 ? 1 : (int)(kSrSmem / (smem + 8 * 1024)));
-            const int at_once = std::max(1, sms * per_sm / cluster);  // rows
-            const double waves = (rows + at_once - 1) / at_once;
-            // a row's time: passes over its entries (shared by the CTAs of an SM), and the cluster's barriers
-            const double each = (double)p.n / cluster / threads * std::max(1.0, (double)std::min(per_sm, (rows * cluster + sms - 1) / sms) * threads / 512.0);
-            const double cost = waves * (each + 40.0 + 4.0 * cluster);
-            if (!best_cluster || cost < best) {
-                best = cost;
-                best_cluster = cluster;
-                best_threads = threads;
+        for (int small = 0; small < 2; small++) {
+            SrShape s = {cluster, small ? 256 : 512, small ? 4 : 5, 0};
+            s.smem = (size_t)((p.n + cluster - 1) / cluster + 16) * sizeof(E) + (sizeof(u64) << s.bits) * s.threads;
+            if (s.smem > sr_smem_max(s.bits)) continue;
+            const int per_sm = std::min<int>(small ? 4 : 2, (int)((size_t)227 * 1024 / (s.smem + 24 * 1024)));
+            const int at_once = std::max(1, sms * std::max(1, per_sm) / cluster);
+            const int waves = (rows + at_once - 1) / at_once;
+            const int sharing = std::min(std::max(1, per_sm), (rows * cluster + sms - 1) / sms);  // CTAs of an SM
+            const double cost = waves * ((double)p.n / cluster / 512.0 * std::max(1.0, sharing * s.threads / 512.0) + 40.0 + 4.0 * cluster);
+            if (!best.cluster || cost < best_cost) {
+                best_cost = cost;
+                best = s;
             }
         }
     }
-    if (!best_cluster) return HQ4_ERR_SHAPE;
-    p.chunk = (p.n + best_cluster - 1) / best_cluster;
-    const size_t smem = sr_smem(p.n, best_cluster, best_threads, sizeof(E));
-    return best_threads == 512 ? launch_sample_rows<E, 512>(p, rows, best_cluster, smem, st)
-                               : launch_sample_rows<E, 256>(p, rows, best_cluster, smem, st);
+    if (!best.cluster) return HQ4_ERR_SHAPE;
+    p.chunk = (p.n + best.cluster - 1) / best.cluster;
+    return best.threads == 512 ? launch_sample_rows<E, 512, 5>(p, rows, best.cluster, best.smem, st)
+                               : launch_sample_rows<E, 256, 4>(p, rows, best.cluster, best.smem, st);
 }
 
 }  // namespace hq4

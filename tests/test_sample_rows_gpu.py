@@ -1,11 +1,11 @@
 """Batch sampling (hq4_sample_rows) against oracle/paged.py's row sampler.
 
-Tokens are equal wherever the draw is further than 2^-38 from the ends of the
-oracle's interval (the kernel's masses are 44-bit fixed point of arithmetic
-good to 2e-10 of each mass, cumulated over at most 2^18 entries, and the
-oracle's sums are fp64); inputs are seeded, so that this is so is a property of
-the inputs, which the tests assert.  Log probabilities are good to 2^-23 of
-their size plus the masses' 2^-31.
+Tokens are equal wherever the draw is further than 2^-28 from the ends of the
+oracle's interval (the kernel's masses are integers of 2^-44, each good to 2e-9
+of itself by its fp32 series: 9e-10 of rounding to an integer, 7e-10 of the
+series' own, and their sums are exact; the oracle's are fp64); inputs are
+seeded, so that this is so is a property of the inputs, which the tests assert.
+Log probabilities are good to 2^-23 of their size plus the masses' 2^-28.
 """
 import numpy as np
 import pytest
@@ -31,9 +31,9 @@ def check(x, u, dtype=None, **kw):
     for i in range(len(u)):
         par = {k: (int(v[i]) if k == "top_k" else float(np.float32(v[i]))) for k, v in kw.items()}
         want, wlp, gap = op.sample(seen[i], min(max(u[i], 0.0), 1.0 - 2.0 ** -53), **par)
-        assert gap > 2.0 ** -38 or gap == 0.0, f"row {i}: the draw lies on a border, take another seed"
+        assert gap > 2.0 ** -28 or gap == 0.0, f"row {i}: the draw lies on a border, take another seed"
         assert tok[i] == want, (i, tok[i], want, par)
-        assert (np.isnan(wlp) and np.isnan(lp[i])) or abs(lp[i] - wlp) <= 2.0 ** -23 * abs(wlp) + 2.0 ** -31, (lp[i], wlp)
+        assert (np.isnan(wlp) and np.isnan(lp[i])) or abs(lp[i] - wlp) <= 2.0 ** -23 * abs(wlp) + 2.0 ** -28, (lp[i], wlp)
     return tok
 
 
@@ -60,7 +60,7 @@ def test_mixed_parameters(cuda, n, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("name,values", [("temperature", [0.01, 0.2, 1.0, 3.0, 50.0, 1e9]), ("top_k", [1, 2, 3, 50, 900, 5000]),
+@pytest.mark.parametrize("name,values", [("temperature", [1e-7, 1e-4, 0.01, 0.2, 1.0, 3.0, 50.0, 1e9]), ("top_k", [1, 2, 3, 50, 900, 5000]),
                                          ("top_p", [0.01, 0.3, 0.8, 0.9, 0.99, 0.99999]),
                                          ("min_p", [1e-6, 0.01, 0.1, 0.5, 0.99, 1.0])])
 def test_one_filter(cuda, name, values):
@@ -150,7 +150,7 @@ def test_small_filters_keep_the_largest(cuda):
     rng = np.random.default_rng(4)
     x = logits(rng, 5, 3000)
     _, tok, lp = run(x, rng.random(5), top_p=[0.0, -1.0, 1e-30, 1.0, 1.0], min_p=[0.0, 0.0, 0.0, 1.0, 7.0])
-    assert (tok == x.argmax(1)).all() and (abs(lp) < 2.0 ** -30).all()
+    assert (tok == x.argmax(1)).all() and (abs(lp) < 2.0 ** -28).all()
 
 
 @pytest.mark.gpu
