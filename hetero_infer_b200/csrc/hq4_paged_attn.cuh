@@ -9,8 +9,9 @@
 // which CTA c takes the c-th equal part.  A part may begin or end inside an
 // item: then the CTA leaves the item's running maximum, sum and unnormalised
 // output of its keys in the workspace, and the combine kernel joins them in
-// key order.  A CTA has at most two such pieces (its first and its last), and
-// every CTA works the same number of key tiles whatever the lengths are.
+// key order.  A CTA has at most two such pieces (its first and its last).  An
+// item counts `extra` units before its tiles, for what beginning and ending one
+// costs, so that CTAs with many short items finish with the others.
 #pragma once
 #include "hq4_paged.cuh"
 
@@ -28,6 +29,7 @@ struct PagedAttnParams {
     const uint32_t* tree_mask;     // [n_rows][mask_words], or null: causal
     int mask_words;
     int split;                     // units are key tiles; else whole items
+    int extra;                     // units of an item before its tiles
     void* ws;
     PagedBatch b;
 };
@@ -68,8 +70,10 @@ __device__ __forceinline__ void paged_row_tile(const PagedAttnParams& p, int rt,
     it.rt = rt;
     it.keys = (int)min(max((long long)it.len + n, 0ll), (long long)cap);
     it.tiles = max((it.keys + kKeys - 1) / kKeys, 1);  // an item without keys still writes its zeros
-    it.weight = p.split ? it.tiles : 1;
+    it.weight = p.split ? p.extra + it.tiles : 1;
 }
+// The tiles of an item before its unit u.
+__device__ __forceinline__ int paged_tiles_before(const PagedAttnParams& p, int u) { return max(u - p.extra, 0); }
 template <int kRows, int kKeys>
 __device__ __forceinline__ long long paged_seq_units(const PagedAttnParams& p, int s) {
     PagedItem it;
@@ -79,7 +83,7 @@ __device__ __forceinline__ long long paged_seq_units(const PagedAttnParams& p, i
     long long w = 0;
     for (int rt = 0; rt < n; rt++) {
         paged_row_tile<kRows, kKeys>(p, rt, it);
-        w += it.tiles;
+        w += it.weight;
     }
     return w * p.n_kv;
 }
@@ -250,34 +254,43 @@ struct PagedWs {
 static_assert(sizeof(PagedStart) % 16 == 0, "the pieces behind the items keep their alignment");
 
 // CTA (c, y): if part c begins inside an item, and c is the first part that
-// does in that item, joins kCombineRows rows of the item's pieces in key order;
-// a warp takes a row, a lane 4 consecutive values of each 128.
+// does in that item, joins rows of the item's pieces.  With few rows to an item
+// (decode, where a long sequence has many pieces) a CTA takes one, its warps a
+// part of the pieces each; else a warp takes a row.  A lane has 4 consecutive
+// values of each 128.  The order of the sums does not depend on timing.
 constexpr int kCombineWarps = 4;
-constexpr int kCombineRows = 8;  // of a CTA
+template <int kRows>
+constexpr int combine_rows() { return kRows <= 32 ? 1 : 8; }  // of a CTA
 template <class A, class C, int kRows, int kDim>
 __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const __grid_constant__ PagedAttnParams p,
                                                                            int ctas) {
+    constexpr int kTake = combine_rows<kRows>();
+    constexpr int kShare = kTake == 1 ? kCombineWarps : 1;  // warps of a row
+    constexpr int kPer = (kDim + 127) / 128;
+    __shared__ float4 s_acc[kShare][kPer][32];
+    __shared__ float s_l[kShare];
     pdl_launch_dependents();
     pdl_wait();
     const PagedWs<kRows, kDim> ws(p.ws, ctas);
     const int c = blockIdx.x + 1;
+    const PagedStart st = ws.info[c];
     const long long total = ws.info[0].total;
     const long long parts = min((long long)ctas, total);
     if (c >= parts) return;
-    const PagedStart st = ws.info[c];
     const PagedItem& it = st.it;
     const long long start = c * total / parts, before = (c - 1) * total / parts;
-    if (st.first == start || st.first < before) return;
+    // nothing to join where no tile lies before this cut, or one lies before the last cut
+    if (start - st.first <= p.extra || before - st.first > p.extra) return;
     const int rows = min(kRows, it.n_tok * p.group - it.rt * kRows);
-    const int first_piece = 2 * (c - 1) + (st.first == before ? 0 : 1);
+    const int first_piece = 2 * (c - 1) + (st.first <= before ? 0 : 1);
     // pieces: that one, then the first ones of parts c, c + 1, ... up to the one with the item's last unit
     const long long last = st.first + it.weight - 1;
     long long owner = last * parts / total;  // or the one after it, by rounding
     while ((owner + 1) * total / parts <= last) owner++;
     const int n = (int)(owner - (c - 1)) + 1;
-    const int lane = threadIdx.x & 31, D = p.head_dim;
-    constexpr int kPer = (kDim + 127) / 128;
-    for (int r = blockIdx.y * kCombineRows + (threadIdx.x >> 5); r < min(rows, (int)(blockIdx.y + 1) * kCombineRows);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = p.head_dim;
+    const int mine = kTake == 1 ? warp : 0;  // the warp's share of the pieces: each kShare-th
+    for (int r = blockIdx.y * kTake + (kTake == 1 ? 0 : warp); r < min(rows, (int)(blockIdx.y + 1) * kTake);
          r += kCombineWarps) {
         auto at = [&](int i) { return (size_t)(i == 0 ? first_piece : 2 * (c - 1 + i)) * kRows + r; };
         float m = -INFINITY;
@@ -289,21 +302,48 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
         float l = 0.0f;
 #pragma unroll
         for (int j = 0; j < kPer; j++) acc[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int i = 0; i < n; i++) {
-            const float2 ml = ws.ml[at(i)];
-            const float w = exp2f(ml.x - mu);
-            l = fmaf(ml.y, w, l);
-            const float* o = ws.o + at(i) * kDim;
+        for (int i0 = mine; i0 < n; i0 += 32 * kShare) {  // 32 pieces' weights, a lane each, then their values
+            float w = 0.0f;
+            if (i0 + lane * kShare < n) {
+                const float2 ml = ws.ml[at(i0 + lane * kShare)];
+                w = exp2f(ml.x - mu);
+                l = fmaf(ml.y, w, l);
+            }
+            const int k = min(32, (n - i0 + kShare - 1) / kShare);
+#pragma unroll 8
+            for (int i = 0; i < k; i++) {
+                const float wi = __shfl_sync(0xffffffffu, w, i);
+                const float* o = ws.o + at(i0 + i * kShare) * kDim;
 #pragma unroll
-            for (int j = 0; j < kPer; j++)
-                if (lane * 4 + 128 * j < D) {
-                    const float4 v = *reinterpret_cast<const float4*>(o + lane * 4 + 128 * j);
-                    acc[j].x = fmaf(v.x, w, acc[j].x);
-                    acc[j].y = fmaf(v.y, w, acc[j].y);
-                    acc[j].z = fmaf(v.z, w, acc[j].z);
-                    acc[j].w = fmaf(v.w, w, acc[j].w);
+                for (int j = 0; j < kPer; j++)
+                    if (lane * 4 + 128 * j < D) {
+                        const float4 v = *reinterpret_cast<const float4*>(o + lane * 4 + 128 * j);
+                        acc[j].x = fmaf(v.x, wi, acc[j].x);
+                        acc[j].y = fmaf(v.y, wi, acc[j].y);
+                        acc[j].z = fmaf(v.z, wi, acc[j].z);
+                        acc[j].w = fmaf(v.w, wi, acc[j].w);
+                    }
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if constexpr (kShare > 1) {
+#pragma unroll
+            for (int j = 0; j < kPer; j++) s_acc[warp][j][lane] = acc[j];
+            if (lane == 0) s_l[warp] = l;
+            __syncthreads();
+            if (warp != 0) return;
+            for (int w = 1; w < kShare; w++) {
+                l += s_l[w];
+#pragma unroll
+                for (int j = 0; j < kPer; j++) {
+                    const float4 v = s_acc[w][j][lane];
+                    acc[j].x += v.x;
+                    acc[j].y += v.y;
+                    acc[j].z += v.z;
+                    acc[j].w += v.w;
                 }
+            }
         }
         const int row = it.rt * kRows + r, tok = row / p.group, head = it.h * p.group + row % p.group;
         A* out = static_cast<A*>(p.out) + ((long long)(it.row0 + tok) * p.n_heads + head) * D;
@@ -326,7 +366,7 @@ struct PaPlan {
     int tc;     // tensor-memory kernel (hq4_paged_tc.cuh), else the warp-level one (hq4_paged_rows.cuh)
     int nt;     // 8-row tiles of the latter
     int dim;    // head_dim rounded up to what the kernels are built for
-    int ctas, split;
+    int ctas, split, extra;
     long long ws;
 };
 

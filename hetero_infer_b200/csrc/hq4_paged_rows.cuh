@@ -75,10 +75,12 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     constexpr int kTile = PaShape<kDim>::kTile, kRing = PaShape<kDim>::kRing;
     constexpr int kChunks = kDim / 8, kOs = kDim + 4;
     static_assert(kRows * kOs * 4 <= kRing, "a warp's outputs fit its ring");
+    // where a warp's outputs fit one stage, the next item's first tiles are under way while this one's are joined
+    constexpr bool kAhead = kRows * kOs * 4 <= 2 * kTile;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ PagedScan scan;
     __shared__ float s_m[kPaWarps][kRows], s_l[kPaWarps][kRows], s_qs[kRows];
-    __shared__ int s_bad[kRows];
+    __shared__ int s_os[kPaWarps];  // where in shared memory each warp has left its outputs
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int D = p.head_dim, ksteps = D >> 4;
@@ -93,57 +95,73 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     PagedItem it = begin.it;
     int left = (int)(end - pos), from = (int)(pos - begin.first);  // units still to do; the first of them in the item
     int pieces = 0;
-    unsigned char* ring = smem + warp * kRing;
-    const uint32_t ring_u = smem_u32(ring);
+    const uint32_t ring_u = smem_u32(smem + warp * kRing);
     unsigned char* qs = smem + kPaWarps * kRing;
     const uint32_t qs_u = smem_u32(qs);
     const C* kc = static_cast<const C*>(p.k);
     const C* vc = static_cast<const C*>(p.v);
     const int in_page = (1 << p.b.page_shift) - 1;
-    float* os = reinterpret_cast<float*>(ring);
+    int stage = 0;                // of the ring: the next tile's
+    unsigned long long oks = 0;   // 16 bits of a tile on its way, the next one lowest: which of its keys have a page
 
-    while (left > 0) {
-        const int units = min(left, it.weight - from);
-        const int t0 = p.split ? from : 0, t1 = p.split ? from + units : it.tiles;
-        const bool whole = t0 == 0 && t1 == it.tiles;
-        const int rows = min(kRows, it.n_tok * p.group - it.rt * kRows);
-        if (units == left) pdl_launch_dependents();
-        if (threadIdx.x == 0 && (it.len < 0 || (long long)it.len + it.n_tok > (long long)p.b.pages_per_seq << p.b.page_shift))
-            atomicOr(p.b.status, kStatusPaged);  // rows whose entries have no place
-
-        // ---- this part's keys start to arrive ------------------------------
-        auto load_tile = [&](int t, int stage) -> uint32_t {
-            const int e = t * kPaKeys + (lane & 15);
-            int page = -1;
-            if (t < t1 && e < it.keys) {
-                page = find_page(p.b, it.s, e);
-                if (page < 0 && lane < 16) atomicOr(p.b.status, kStatusPaged);
-            }
-            const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
-            const long long at = page < 0 ? 0
-                                          : (long long)page * p.b.page_stride +
-                                                (((long long)it.h << p.b.page_shift) + (e & in_page)) * D;
-            if (t < t1) {
-                const uint32_t kd = ring_u + stage * 2 * kTile, vd = kd + kTile;
+    // Starts tile t of an item's piece that ends before t1 (nothing, beyond that).
+    auto load_tile = [&](const PagedItem& it, int t, int t1, int stage) -> uint32_t {
+        const int e = t * kPaKeys + (lane & 15);
+        int page = -1;
+        if (t < t1 && e < it.keys) {
+            page = find_page(p.b, it.s, e);
+            if (page < 0 && lane < 16) atomicOr(p.b.status, kStatusPaged);
+        }
+        const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
+        const long long at = page < 0 ? 0
+                                      : (long long)page * p.b.page_stride +
+                                            (((long long)it.h << p.b.page_shift) + (e & in_page)) * D;
+        if (t < t1) {
+            const uint32_t kd = ring_u + stage * 2 * kTile, vd = kd + kTile;
 #pragma unroll
-                for (int i = 0; i < kPaKeys * kChunks / 32; i++) {
-                    const int idx = lane + 32 * i, r = idx / kChunks, c = idx % kChunks;
-                    const long long src = __shfl_sync(0xffffffffu, at, r) + c * 8;
-                    const bool on = ok >> r & 1;
-                    if (c * 8 < D) {  // without a page: zeros, so that what lies there does not reach the products
-                        const int d = tile_at<kDim>(r, c);
-                        cp_async16(kd + d, kc + (on ? src : 0), on);
-                        cp_async16(vd + d, vc + (on ? src : 0), on);
-                    }
+            for (int i = 0; i < kPaKeys * kChunks / 32; i++) {
+                const int idx = lane + 32 * i, r = idx / kChunks, c = idx % kChunks;
+                const long long src = __shfl_sync(0xffffffffu, at, r) + c * 8;
+                const bool on = ok >> r & 1;
+                if (c * 8 < D) {  // without a page: zeros, so that what lies there does not reach the products
+                    const int d = tile_at<kDim>(r, c);
+                    cp_async16(kd + d, kc + (on ? src : 0), on);
+                    cp_async16(vd + d, vc + (on ? src : 0), on);
                 }
             }
-            cp_async_commit();
-            return ok;
-        };
-        unsigned long long oks = 0;  // 16 bits of a stage: which of its keys have a page
+        }
+        cp_async_commit();
+        return ok;
+    };
+    auto begin_item = [&](const PagedItem& it, int t0, int t1) {  // its first tiles
+        oks = 0;
 #pragma unroll
-        for (int s = 0; s < kStages - 1; s++)
-            oks |= (unsigned long long)load_tile(t0 + warp + s * kPaWarps, s) << (16 * s);
+        for (int s = 0; s < kStages - 1; s++) {
+            const int at = stage + s < kStages ? stage + s : stage + s - kStages;
+            oks |= (unsigned long long)load_tile(it, t0 + warp + s * kPaWarps, t1, at) << (16 * s);
+        }
+    };
+    auto units_of = [&](const PagedItem& it, int from, int left) { return min(left, it.weight - from); };
+    auto t_begin = [&](int from) { return p.split ? paged_tiles_before(p, from) : 0; };
+    auto t_end = [&](const PagedItem& it, int from, int units) {
+        return p.split ? paged_tiles_before(p, from + units) : it.tiles;
+    };
+    {
+        const int units = units_of(it, from, left);
+        begin_item(it, t_begin(from), t_end(it, from, units));
+    }
+
+    while (left > 0) {
+        const int units = units_of(it, from, left);
+        const int t0 = t_begin(from), t1 = t_end(it, from, units);
+        if (t1 == 0) break;  // the part ends before the item's first tile
+        const bool whole = t0 == 0 && t1 == it.tiles;
+        const int rows = min(kRows, it.n_tok * p.group - it.rt * kRows);
+        PagedItem nx = it;
+        if (units < left) paged_next<kRows, kPaKeys>(p, nx);
+        else pdl_launch_dependents();
+        if (threadIdx.x == 0 && (it.len < 0 || (long long)it.len + it.n_tok > (long long)p.b.pages_per_seq << p.b.page_shift))
+            atomicOr(p.b.status, kStatusPaged);  // rows whose entries have no place
 
         // ---- the queries, as 16-bit terms ----------------------------------
         for (int r = warp; r < kRows; r += kPaWarps) {
@@ -204,7 +222,6 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
                 }
             }
         }
-        if (threadIdx.x < kRows) s_bad[threadIdx.x] = 0;
         __syncthreads();
 
         // ---- the keys --------------------------------------------------------
@@ -224,22 +241,23 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
             }
         }
         const int first_tok = it.rt * kRows / p.group;
-        int stage = 0;
         for (int t = t0 + warp; t < t1; t += kPaWarps) {
             int ahead = stage + kStages - 1;
             if (ahead >= kStages) ahead -= kStages;
             __syncwarp();  // the tile that is overwritten was read by all lanes
-            const uint32_t more = load_tile(t + (kStages - 1) * kPaWarps, ahead);
+            const uint32_t more = load_tile(it, t + (kStages - 1) * kPaWarps, t1, ahead);
             const uint32_t ok = (uint32_t)oks & 0xffffu;
             oks = (oks >> 16) | (unsigned long long)more << (16 * (kStages - 2));
             cp_async_wait<kStages - 1>();
             __syncwarp();
             const uint32_t kd = ring_u + stage * 2 * kTile, vd = kd + kTile;
-            float sc[NT][4];
+            // fp32's precision: several short sums, since the matrix unit cuts off what a sum does not hold
+            constexpr int kSums = kTerms == 1 ? 1 : 4;
+            float sc[NT][4], part[NT][kSums][4];
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) sc[n][i] = 0.0f;
+                for (int i = 0; i < 4 * kSums; i++) part[n][i >> 2][i & 3] = 0.0f;
 #pragma unroll
             for (int k2 = 0; k2 < kDim / 32; k2++) {
                 if (k2 * 2 >= ksteps) break;
@@ -253,11 +271,19 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
                     for (int term = kTerms - 1; term >= 0; term--) {
                         uint32_t b[4];
                         ldsm4(qs_u + term * (kRows * kDim * 2) + tile_at<kDim>(n * 8 + (lane & 7), k2 * 4 + (lane >> 3)), b);
-                        mma16<C>(sc[n], a0, b[0], b[1]);
-                        mma16<C>(sc[n], a1, b[2], b[3]);
+                        const int s0 = kSums == 1 ? 0 : term ? 2 : k2 & 1, s1 = kSums == 1 ? 0 : term ? 3 : k2 & 1;
+                        mma16<C>(part[n][s0], a0, b[0], b[1]);
+                        mma16<C>(part[n][s1], a1, b[2], b[3]);
                     }
             }
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    sc[n][i] = kSums == 1 ? part[n][0][i]
+                                          : (part[n][0][i] + part[n][1 % kSums][i]) + (part[n][2 % kSums][i] + part[n][3 % kSums][i]);
             const bool plain = ok == 0xffffu && (t + 1) * kPaKeys <= it.len + (p.tree_mask ? 0 : first_tok + 1);
+            float keep[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -271,7 +297,6 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
                     }
                     sc[n][i] = z;
                 }
-                float keep[2];
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     float x = fmaxf(sc[n][i], sc[n][i + 2]);
@@ -279,20 +304,17 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                     const float m1 = fmaxf(m[n][i], x), mu = m1 == -INFINITY ? 0.0f : m1;
-                    keep[i] = ex2(m[n][i] - mu);
+                    keep[n][i] = ex2(m[n][i] - mu);
                     m[n][i] = m1;
                     sc[n][i] = ex2(sc[n][i] - mu);
                     sc[n][i + 2] = ex2(sc[n][i + 2] - mu);
-                    l[n][i] = fmaf(l[n][i], keep[i], sc[n][i] + sc[n][i + 2]);
+                    l[n][i] = fmaf(l[n][i], keep[n][i], sc[n][i] + sc[n][i + 2]);
                 }
-                if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f)) {
+                if (kTerms == 1 && __any_sync(0xffffffffu, keep[n][0] != 1.0f || keep[n][1] != 1.0f)) {
 #pragma unroll
-                    for (int d = 0; d < kDim / 16; d++) {
-                        acc[d][n][0] *= keep[0];
-                        acc[d][n][1] *= keep[1];
-                        acc[d][n][2] *= keep[0];
-                        acc[d][n][3] *= keep[1];
-                    }
+                    for (int d = 0; d < kDim / 16; d++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[d][n][i] *= keep[n][i & 1];
                 }
             }
             // the probabilities as 16-bit terms (of fp16: scaled by 2^14, which the epilogue takes back, so that
@@ -322,17 +344,33 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
                 uint32_t a[4];
                 ldsm4_t(vd + tile_at<kDim>((lane & 7) + (lane >> 4) * 8, d * 2 + (lane >> 3 & 1)), a);
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+                for (int n = 0; n < NT; n++) {
+                    if constexpr (kTerms == 1) {
+                        mma16<C>(acc[d][n], a, pb[n][0][0], pb[n][0][1]);
+                    } else {  // fp32's precision: a tile's sum by itself, then rounded to nearest into the whole
+                        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int term = kTerms - 1; term >= 0; term--) mma16<C>(acc[d][n], a, pb[n][term][0], pb[n][term][1]);
+                        for (int term = kTerms - 1; term >= 0; term--) mma16<C>(sum, a, pb[n][term][0], pb[n][term][1]);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[d][n][i] = fmaf(acc[d][n][i], keep[n][i & 1], sum[i]);
+                    }
+                }
             }
             if (++stage == kStages) stage = 0;
         }
-        cp_async_wait<0>();
-
-        // ---- the warps' results, joined --------------------------------------
+        // ---- the next item's first tiles; the warps' results, joined ----------
         const float back = kTerms == 2 ? 1.0f / 16384.0f : 1.0f;
         __syncwarp();  // the ring is the warp's own: its lanes have read their last tile
+        int os_at = warp * kRing;
+        if constexpr (kAhead) {
+            if (units < left) begin_item(nx, t_begin(0), t_end(nx, 0, units_of(nx, 0, left - units)));
+            os_at += (stage + kStages - 1) % kStages * 2 * kTile;  // the stage that those leave free
+        } else {
+            cp_async_wait<0>();
+            __syncwarp();
+        }
+        float* os = reinterpret_cast<float*>(smem + os_at);
+        if (lane == 0) s_os[warp] = os_at;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -377,7 +415,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
                 float y = 0.0f;
 #pragma unroll
                 for (int i = 0; i < kPaWarps; i++)
-                    y = fmaf(reinterpret_cast<const float*>(smem + i * kRing)[r * kOs + d], w[i], y);
+                    y = fmaf(reinterpret_cast<const float*>(smem + s_os[i])[r * kOs + d], w[i], y);
                 if (whole) {
                     if (ll == 0.0f) y = 0.0f;
                     bad |= y != y;
@@ -392,7 +430,8 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
         __syncthreads();  // the rings and the queries are free again
         left -= units;
         from = 0;
-        if (left > 0) paged_next<kRows, kPaKeys>(p, it);
+        it = nx;
+        if (!kAhead && left > 0) begin_item(it, t_begin(0), t_end(it, 0, units_of(it, 0, left)));
     }
 }
 
@@ -425,7 +464,7 @@ static int launch_pa(PagedAttnParams p, const PaPlan& pl, cudaStream_t st) {
     int ctas = pl.ctas;
     void* cargs[] = {&p, &ctas};
     return launch_pdl_kernel((const void*)paged_combine_kernel<A, C, 8 * NT, kDim>,
-                             dim3(pl.ctas - 1, (8 * NT + kCombineRows - 1) / kCombineRows), dim3(kCombineWarps * 32),
+                             dim3(pl.ctas - 1, (8 * NT) / combine_rows<8 * NT>()), dim3(kCombineWarps * 32),
                              0, st, cargs) == cudaSuccess
                ? HQ4_OK
                : HQ4_ERR_LAUNCH;

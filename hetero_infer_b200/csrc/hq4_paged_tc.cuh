@@ -281,8 +281,8 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
     // The key tiles of the part's piece of the item, and the units that it takes; then the next item.
     auto piece = [&](int& t0, int& t1) -> int {
         const int units = min(left, it->weight - from);
-        t0 = p.split ? from : 0;
-        t1 = p.split ? from + units : it->tiles;
+        t0 = p.split ? paged_tiles_before(p, from) : 0;
+        t1 = p.split ? paged_tiles_before(p, from + units) : it->tiles;
         return units;
     };
     auto next = [&](int units) {
@@ -344,6 +344,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
         while (left > 0 && !fail) {
             int t0, t1;
             const int units = piece(t0, t1);
+            if (t1 == 0) break;  // the part ends before the item's first tile
             const bool whole = t0 == 0 && t1 == it->tiles;
             const bool in = g < groups_of();
             const int row = it->rt * kRows + g * 128 + in_group, rows = it->n_tok * p.group;
@@ -509,6 +510,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
         while (left > 0 && !fail) {
             int t0, t1;
             const int units = piece(t0, t1);
+            if (t1 == 0) break;  // the part ends before the item's first tile
             const int ng = groups_of();
             if (!full(n_slot)) break;
             for (int g = 0; g < ng && !fail; g++) {
@@ -574,6 +576,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
         while (left > 0 && !fail) {
             int t0, t1;
             const int units = piece(t0, t1);
+            if (t1 == 0) break;  // the part ends before the item's first tile
             if (lane == 0 && (it->len < 0 || (long long)it->len + it->n_tok > (long long)p.b.pages_per_seq << p.b.page_shift))
                 atomicOr(p.b.status, kStatusPaged);  // rows whose entries have no place
             for (int t = t0; t < t1 && !fail; t++, tile_no++) {
@@ -661,7 +664,7 @@ static int launch_pt(const PagedAttnParams& p, const PaPlan& pl, cudaStream_t st
     lc.numAttrs = 1;
     if (cudaLaunchKernelEx(&lc, kern, tk, tv, p) != cudaSuccess) return HQ4_ERR_LAUNCH;
     if (!p.split || pl.ctas < 2) return HQ4_OK;
-    lc.gridDim = dim3(pl.ctas - 1, (S::kRows + kCombineRows - 1) / kCombineRows);
+    lc.gridDim = dim3(pl.ctas - 1, S::kRows / combine_rows<S::kRows>());
     lc.blockDim = dim3(kCombineWarps * 32);
     lc.dynamicSmemBytes = 0;
     return cudaLaunchKernelEx(&lc, paged_combine_kernel<C, C, S::kRows, kDim>, p, pl.ctas) == cudaSuccess
