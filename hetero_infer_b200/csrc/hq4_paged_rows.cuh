@@ -104,18 +104,21 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     int stage = 0;                // of the ring: the next tile's
     unsigned long long oks = 0;   // 16 bits of a tile on its way, the next one lowest: which of its keys have a page
 
-    // Starts tile t of an item's piece that ends before t1 (nothing, beyond that).
-    auto load_tile = [&](const PagedItem& it, int t, int t1, int stage) -> uint32_t {
+    // Lanes 0-15 (and 16-31 alike) look up where a tile's keys lie: the page, -1 for none.  A step
+    // ahead of the copies, so that those do not wait for it.
+    auto look_up = [&](const PagedItem& it, int t, int t1) -> int {
         const int e = t * kPaKeys + (lane & 15);
-        int page = -1;
-        if (t < t1 && e < it.keys) {
-            page = find_page(p.b, it.s, e);
-            if (page < 0 && lane < 16) atomicOr(p.b.status, kStatusPaged);
-        }
+        if (t >= t1 || e >= it.keys) return -1;
+        const int page = find_page(p.b, it.s, e);
+        if (page < 0 && lane < 16) atomicOr(p.b.status, kStatusPaged);
+        return page;
+    };
+    // Starts tile t of an item's piece that ends before t1 (nothing, beyond that).
+    auto load_tile = [&](const PagedItem& it, int t, int t1, int page, int stage) -> uint32_t {
         const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0) & 0xffffu;
         const long long at = page < 0 ? 0
                                       : (long long)page * p.b.page_stride +
-                                            (((long long)it.h << p.b.page_shift) + (e & in_page)) * D;
+                                            (((long long)it.h << p.b.page_shift) + ((t * kPaKeys + (lane & 15)) & in_page)) * D;
         if (t < t1) {
             const uint32_t kd = ring_u + stage * 2 * kTile, vd = kd + kTile;
 #pragma unroll
@@ -133,13 +136,18 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
         cp_async_commit();
         return ok;
     };
+    int page_next = -1;  // of the first tile that has not been started
     auto begin_item = [&](const PagedItem& it, int t0, int t1) {  // its first tiles
         oks = 0;
+        int page[kStages];
+#pragma unroll
+        for (int s = 0; s < kStages; s++) page[s] = look_up(it, t0 + warp + s * kPaWarps, t1);
 #pragma unroll
         for (int s = 0; s < kStages - 1; s++) {
             const int at = stage + s < kStages ? stage + s : stage + s - kStages;
-            oks |= (unsigned long long)load_tile(it, t0 + warp + s * kPaWarps, t1, at) << (16 * s);
+            oks |= (unsigned long long)load_tile(it, t0 + warp + s * kPaWarps, t1, page[s], at) << (16 * s);
         }
+        page_next = page[kStages - 1];
     };
     auto units_of = [&](const PagedItem& it, int from, int left) { return min(left, it.weight - from); };
     auto t_begin = [&](int from) { return p.split ? paged_tiles_before(p, from) : 0; };
@@ -245,7 +253,8 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
             int ahead = stage + kStages - 1;
             if (ahead >= kStages) ahead -= kStages;
             __syncwarp();  // the tile that is overwritten was read by all lanes
-            const uint32_t more = load_tile(it, t + (kStages - 1) * kPaWarps, t1, ahead);
+            const uint32_t more = load_tile(it, t + (kStages - 1) * kPaWarps, t1, page_next, ahead);
+            page_next = look_up(it, t + kStages * kPaWarps, t1);
             const uint32_t ok = (uint32_t)oks & 0xffffu;
             oks = (oks >> 16) | (unsigned long long)more << (16 * (kStages - 2));
             cp_async_wait<kStages - 1>();
