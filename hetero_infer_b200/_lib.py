@@ -116,6 +116,32 @@ def load(path: str = None) -> ctypes.CDLL:
     return lib
 
 
+_torch_calls = None
+
+
+def torch_calls():
+    """The module that makes the paged operators' calls from tensors
+    (csrc/hq4_torch.cpp), bound to the loaded library."""
+    global _torch_calls
+    if _torch_calls is not None:
+        return _torch_calls
+    path = _build.TORCH_LIB
+    if not os.path.exists(path):
+        raise RuntimeError(f"{path} is missing: build it with `python -m hetero_infer_b200.build`")
+    import importlib.util
+
+    import torch  # noqa: F401  (its libraries)
+    lib = load()
+    spec = importlib.util.spec_from_file_location("hetero_infer_b200._hq4_torch", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    names = ("hq4_paged_append", "hq4_paged_attention", "hq4_tree_attention", "hq4_paged_attention_workspace_bytes",
+             "hq4_sample_rows")
+    mod.bind(check, {n: ctypes.cast(getattr(lib, n), _P).value for n in names})
+    _torch_calls = mod
+    return mod
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         raise RuntimeError(f"{what} failed with {rc}: {ERRORS.get(rc, 'unknown error')}")

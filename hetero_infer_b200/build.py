@@ -1,7 +1,8 @@
 """Build the sm_100a shared library ``libhq4.so`` in-tree with nvcc.
 
-The library is plain C ABI (``include/hq4.h``) over hand-written CUDA; no torch
-headers are involved, so it builds in seconds and without a GPU.
+The library is plain C ABI (``include/hq4.h``) over hand-written CUDA, without
+torch headers.  Beside it, ``_hq4_torch`` (host code only, one file over torch's
+headers) makes the paged operators' calls from tensors.  Both build without a GPU.
 """
 from __future__ import annotations
 
@@ -15,6 +16,8 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libhq4.so")
+TORCH_SRC = os.path.join(CSRC, "hq4_torch.cpp")
+TORCH_LIB = os.path.join(PKG, "_hq4_torch.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
@@ -36,16 +39,33 @@ def headers():
     return sorted(glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h")))
 
 
-def up_to_date() -> bool:
-    if not os.path.exists(LIB):
+def up_to_date(lib: str = LIB) -> bool:
+    if not os.path.exists(lib):
         return False
-    t = os.path.getmtime(LIB)
-    return all(os.path.getmtime(f) <= t for f in sources() + headers() + [__file__])
+    t = os.path.getmtime(lib)
+    deps = [TORCH_SRC] if lib == TORCH_LIB else sources()
+    return all(os.path.getmtime(f) <= t for f in deps + headers() + [__file__])
+
+
+def torch_command():
+    """The compile command of _hq4_torch."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    libdir = os.path.join(os.path.dirname(torch.__file__), "lib")
+    inc = [f"-I{d}" for d in cpp_extension.include_paths() + [os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include"),
+                                                             sysconfig.get_paths()["include"], INCLUDE]]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *inc, TORCH_SRC, "-o", TORCH_LIB + ".tmp",
+            f"-L{libdir}", f"-Wl,-rpath,{libdir}", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
+            "-ltorch_python"]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile every csrc/*.cu into libhq4.so (skipped when up to date)."""
-    if not force and up_to_date():
+    """Compile every csrc/*.cu into libhq4.so, and _hq4_torch.so (each skipped when up to date)."""
+    todo = [lib for lib in (LIB, TORCH_LIB) if force or not up_to_date(lib)]
+    if not todo:
         return LIB
     import concurrent.futures
     import tempfile
@@ -53,17 +73,22 @@ def build(force: bool = False, verbose: bool = False) -> str:
     def run(cmd):
         out = subprocess.run(cmd, capture_output=True, text=True)
         if out.returncode != 0:
-            raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + out.stdout + out.stderr)
+            raise RuntimeError("the build failed:\n" + " ".join(cmd) + "\n" + out.stdout + out.stderr)
         return out.stderr
 
     with tempfile.TemporaryDirectory() as tmp:  # the files side by side, then one link
-        objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in sources()]
+        files = sources() if LIB in todo else []
+        objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in files]
         cmds = [[nvcc(), *ARCH_FLAGS, *NVCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", s, "-o", o]
-                for s, o in zip(sources(), objs)]
+                for s, o in zip(files, objs)]
+        if TORCH_LIB in todo:
+            cmds.append(torch_command())
         with concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
             logs = list(pool.map(run, cmds))
-        run([nvcc(), *ARCH_FLAGS, "-shared", "-o", LIB + ".tmp", *objs])
-    os.replace(LIB + ".tmp", LIB)
+        if files:
+            run([nvcc(), *ARCH_FLAGS, "-shared", "-o", LIB + ".tmp", *objs])
+    for lib in todo:
+        os.replace(lib + ".tmp", lib)
     if verbose:
         sys.stdout.write("".join(logs))
     return LIB

@@ -219,67 +219,8 @@ def act_decode_i8(payload: torch.Tensor, rows: int, cols: int, dtype=torch.float
 # int32 CUDA tensors that the kernels read when they run, so a captured step can
 # be replayed while the sequences grow.  A step appends first, then attends.
 
-_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
-def _stream_of(t: torch.Tensor) -> int:
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
-
-
-def _need_rows(t: torch.Tensor, name: str, heads, head_dim, like: Optional[torch.Tensor] = None) -> None:
-    """[rows, heads, head_dim] whose rows may be apart (a view of a fused projection)."""
-    if t.dim() != 3 or (heads is not None and t.shape[1] != heads) or (head_dim is not None and t.shape[2] != head_dim):
-        raise RuntimeError(f"{name} must be [rows, heads, head_dim], got {tuple(t.shape)}")
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must be a CUDA tensor (no CPU fallback)")
-    if t.dtype not in _TYPES:
-        raise RuntimeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
-        raise RuntimeError(f"{name}'s heads must lie one after another within a row")
-    if like is not None and (t.dtype != like.dtype or t.shape[0] != like.shape[0] or t.device != like.device):
-        raise RuntimeError(f"{name} must have q's rows, type and device")
-
-
-def _need_ints(t: torch.Tensor, name: str, device, shape) -> None:
-    if not t.is_cuda or t.device != device or t.dtype != torch.int32 or not t.is_contiguous() or t.shape != shape:
-        raise RuntimeError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on {device}, "
-                           f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    """Elements from a row to the next (a lone row has none of its own)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
-
-
-def _need_caches(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor):
-    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if t.dim() != 4 or not t.is_cuda or t.device != q.device:
-            raise RuntimeError(f"{name} must be [n_pages, n_kv, page_size, head_dim] on {q.device}")
-        if t.dtype not in (torch.bfloat16, torch.float16) or t.dtype != k_cache.dtype:
-            raise RuntimeError("the caches must be both bfloat16 or both float16")
-        _, _, ps, hd = t.shape
-        if t.stride()[1:] != (ps * hd, hd, 1):
-            raise RuntimeError(f"{name}'s pages must each be contiguous")
-    if v_cache.shape != k_cache.shape or v_cache.stride(0) != k_cache.stride(0):
-        raise RuntimeError("k_cache and v_cache must have the same shape and strides")
-    if q.dtype != torch.float32 and q.dtype != k_cache.dtype:
-        raise RuntimeError(f"activations must be float32 or the caches' {k_cache.dtype}, got {q.dtype}")
-    if q.device.index != torch.cuda.current_device():
-        raise RuntimeError(f"tensors on {q.device}, current device {torch.cuda.current_device()}")
-
-
-def _need_batch(q, pages, cu_rows, lens):
-    n_seqs = lens.numel()
-    _need_ints(lens, "lens", q.device, (n_seqs,))
-    _need_ints(cu_rows, "cu_rows", q.device, (n_seqs + 1,))
-    if pages.dim() != 2:
-        raise RuntimeError("pages must be [n_seqs, pages_per_seq]")
-    _need_ints(pages, "pages", q.device, (n_seqs, pages.shape[1]))
-    return n_seqs
-
-
-def _page_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2] * t.shape[3]
+# The calls are checked and made in native code (csrc/hq4_torch.cpp): in Python
+# that takes longer than the kernels of a small step.
 
 
 def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -295,92 +236,14 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: tor
     float32 [max_pos, head_dim / 2].  A row's position is its entry's number or
     positions[row] (int32); q_norm, k_norm: float32 [head_dim], an RMS norm of
     each head before the rotation."""
-    hd = k_cache.shape[-1] if k_cache.dim() == 4 else None
-    _need_rows(q, "q", None, hd)
-    _need_caches(q, k_cache, v_cache)
-    n_pages, n_kv, ps, hd = k_cache.shape
-    _need_rows(k, "k", n_kv, hd, q)
-    _need_rows(v, "v", n_kv, hd, q)
-    n_seqs = _need_batch(q, pages, cu_rows, lens)
-    rows, nh = q.shape[0], q.shape[1]
-    for t, name in ((rope_cos, "rope_cos"), (rope_sin, "rope_sin")):
-        _need_cuda(t, name, torch.float32)
-        if t.dim() != 2 or t.shape[1] * 2 != hd or t.shape != rope_cos.shape or t.device != q.device:
-            raise RuntimeError(f"{name} must be [max_pos, head_dim / 2] on {q.device}")
-    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if t is not None:
-            _need_cuda(t, name, torch.float32)
-            if t.shape != (hd,) or t.device != q.device:
-                raise RuntimeError(f"{name} must be [head_dim] on {q.device}")
-    if positions is not None:
-        _need_ints(positions, "positions", q.device, (rows,))
-    if out is None:
-        out = torch.empty((rows, nh, hd), dtype=q.dtype, device=q.device)
-    else:
-        _need_cuda(out, "out", q.dtype)
-        if out.shape != q.shape or out.device != q.device:
-            raise RuntimeError("out must have q's shape and device")
-    if rows == 0:
-        return out
-    rc = _lib.load().hq4_paged_append(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), _TYPES[q.dtype], rows, nh, n_kv, hd, _row_stride(q), _row_stride(k),
-        _row_stride(v), None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(),
-        eps, cu_rows.data_ptr(), lens.data_ptr(), n_seqs, None if positions is None else positions.data_ptr(),
-        rope_cos.data_ptr(), rope_sin.data_ptr(), rope_cos.shape[0], pages.data_ptr(), pages.shape[1],
-        k_cache.data_ptr(), v_cache.data_ptr(), _TYPES[k_cache.dtype], n_pages, ps, _page_stride(k_cache),
-        out.data_ptr(), _stream_of(q))
-    if rc:
-        _lib.check(rc, "hq4_paged_append")
-    return out
+    return _lib.torch_calls().paged_append(q, k, v, k_cache, v_cache, pages, cu_rows, lens, rope_cos, rope_sin,
+                                           positions, q_norm, k_norm, eps, out)
 
 
 def paged_attention_workspace(q: torch.Tensor, k_cache: torch.Tensor, pages: torch.Tensor) -> torch.Tensor:
     """A workspace for paged_attention / tree_attention calls of these shapes
     (one to a stream; the calls take a fresh one where none is given)."""
-    n = int(_lib.load().hq4_paged_attention_workspace_bytes(
-        _TYPES[q.dtype], q.shape[0], q.shape[1], k_cache.shape[1], q.shape[2], pages.shape[0], pages.shape[1],
-        k_cache.shape[2]))
-    if n < 0:
-        raise RuntimeError(f"hq4_paged_attention_workspace_bytes = {n} for q {tuple(q.shape)}, "
-                           f"cache {tuple(k_cache.shape)}")
-    return torch.empty(n, dtype=torch.uint8, device=q.device)
-
-
-def _attend(q, k_cache, v_cache, pages, cu_rows, lens, tree_mask, scale, out, workspace):
-    hd = k_cache.shape[-1] if k_cache.dim() == 4 else None
-    _need_rows(q, "q", None, hd)
-    _need_caches(q, k_cache, v_cache)
-    n_seqs = _need_batch(q, pages, cu_rows, lens)
-    n_pages, n_kv, ps, hd = k_cache.shape
-    rows, nh = q.shape[0], q.shape[1]
-    if scale is None:
-        scale = hd ** -0.5
-    if out is None:
-        out = torch.empty((rows, nh, hd), dtype=q.dtype, device=q.device)
-    else:
-        _need_cuda(out, "out", q.dtype)
-        if out.shape != q.shape or out.device != q.device:
-            raise RuntimeError("out must have q's shape and device")
-    if rows == 0:
-        return out
-    if workspace is None:
-        workspace = paged_attention_workspace(q, k_cache, pages)
-    else:
-        _need_cuda(workspace, "workspace", torch.uint8)
-        if workspace.device != q.device:
-            raise RuntimeError(f"workspace must be on {q.device}")
-    lib = _lib.load()
-    head = (q.data_ptr(), _TYPES[q.dtype], rows, nh, n_kv, hd, _row_stride(q), cu_rows.data_ptr(), lens.data_ptr(),
-            n_seqs, pages.data_ptr(), pages.shape[1], k_cache.data_ptr(), v_cache.data_ptr(), _TYPES[k_cache.dtype],
-            n_pages, ps, _page_stride(k_cache))
-    tail = (scale, out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream_of(q))
-    if tree_mask is None:
-        rc = lib.hq4_paged_attention(*head, *tail)
-    else:
-        rc = lib.hq4_tree_attention(*head, tree_mask.data_ptr(), tree_mask.shape[1], *tail)
-    if rc:
-        _lib.check(rc, "hq4_paged_attention" if tree_mask is None else "hq4_tree_attention")
-    return out
+    return _lib.torch_calls().workspace(q, k_cache, pages)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pages: torch.Tensor,
@@ -390,7 +253,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (hq4_paged_attention): row i of sequence s sees entries 0 .. lens[s] + i.
     q: [rows, n_heads, head_dim] as paged_append returns it; scale defaults to
     head_dim ** -0.5.  Decode, prompt chunks and mixtures of them alike."""
-    return _attend(q, k_cache, v_cache, pages, cu_rows, lens, None, scale, out, workspace)
+    return _lib.torch_calls().attend(q, k_cache, v_cache, pages, cu_rows, lens, None, scale, out, workspace)
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pages: torch.Tensor,
@@ -399,11 +262,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     """paged_attention for trees of drafted tokens (hq4_tree_attention): row i
     of sequence s sees the entries before lens[s], and entry lens[s] + j where
     bit j % 32 of tree_mask[row, j // 32] is set (int32 words)."""
-    _need_cuda(tree_mask, "tree_mask", torch.int32)
-    if tree_mask.dim() != 2 or tree_mask.shape[0] != q.shape[0] or tree_mask.shape[1] < 1 \
-            or tree_mask.device != q.device:
-        raise RuntimeError(f"tree_mask must be int32 [rows, words] on {q.device}")
-    return _attend(q, k_cache, v_cache, pages, cu_rows, lens, tree_mask, scale, out, workspace)
+    if tree_mask is None:
+        raise RuntimeError("tree_mask must be int32 [rows, words]")
+    return _lib.torch_calls().attend(q, k_cache, v_cache, pages, cu_rows, lens, tree_mask, scale, out, workspace)
 
 
 def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,
@@ -414,31 +275,4 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[tor
 
     u: float64 [rows], uniform in [0, 1); temperature, top_p, min_p: float32
     [rows], top_k: int32 [rows], None for off.  temperature <= 0 is greedy."""
-    if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in _TYPES:
-        raise RuntimeError("logits must be a CUDA float32, bfloat16 or float16 tensor [rows, vocab]")
-    rows, n = logits.shape
-    if n > 1 and logits.stride(1) != 1:
-        raise RuntimeError("logits' rows must each be contiguous")
-    if logits.device.index != torch.cuda.current_device():
-        raise RuntimeError(f"tensors on {logits.device}, current device {torch.cuda.current_device()}")
-    ptrs = []
-    for t, name, dt in ((u, "u", torch.float64), (temperature, "temperature", torch.float32),
-                        (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
-                        (min_p, "min_p", torch.float32), (out, "out", torch.int32)):
-        if t is None:
-            ptrs.append(None)
-            continue
-        if not t.is_cuda or t.dtype != dt or t.shape != (rows,) or not t.is_contiguous() or t.device != logits.device:
-            raise RuntimeError(f"{name} must be a contiguous {dt} tensor of {rows} values on {logits.device}")
-        ptrs.append(t.data_ptr())
-    if out is None:
-        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
-        ptrs[5] = out.data_ptr()
-    lp = torch.empty(rows, dtype=torch.float32, device=logits.device) if logprob else None
-    if rows:
-        rc = _lib.load().hq4_sample_rows(
-            logits.data_ptr(), _TYPES[logits.dtype], rows, n, logits.stride(0) if rows > 1 else n, ptrs[1], ptrs[2],
-            ptrs[3], ptrs[4], ptrs[0], ptrs[5], None if lp is None else lp.data_ptr(), _stream_of(logits))
-        if rc:
-            _lib.check(rc, "hq4_sample_rows")
-    return (out, lp) if logprob else out
+    return _lib.torch_calls().sample_rows(logits, u, temperature, top_k, top_p, min_p, out, logprob)

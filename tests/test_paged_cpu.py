@@ -89,6 +89,23 @@ def test_wrappers_want_cuda():
         ops.sample_rows(torch.zeros(2, 4), torch.zeros(2, dtype=torch.float64))
 
 
+def test_wrappers_say_what_they_got():
+    import torch
+    from hetero_infer_b200 import ops
+    c = torch.zeros(3, 2, 16, 64, dtype=torch.bfloat16)
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match=r"q must be \[rows, heads, head_dim\], got \[2, 4\]"):
+        ops.paged_attention(torch.zeros(2, 4), c, c, i[None], i, i[:1])
+    with pytest.raises(RuntimeError, match="must be a torch.Tensor"):
+        ops.paged_attention([1.0], c, c, i[None], i, i[:1])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.paged_attention_workspace(torch.zeros(2, 4, 64), c, i[None])
+    with pytest.raises(RuntimeError):
+        ops.tree_attention(torch.zeros(2, 4, 64), c, c, i[None], i, i[:1], None)
+    with pytest.raises(TypeError):
+        ops.paged_append(torch.zeros(2, 4, 64), *[torch.zeros(2, 2, 64)] * 2, c, c, i[None], i, i[:1], c, c, eps="x")
+
+
 def test_oracle_attention_is_a_mean_without_scores():
     rng = np.random.default_rng(0)
     kc, vc = rng.standard_normal((2, 5, 1, 8, 32))
