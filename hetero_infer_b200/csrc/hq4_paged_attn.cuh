@@ -61,24 +61,22 @@ template <int kRows>
 __device__ __forceinline__ int paged_row_tiles(const PagedAttnParams& p, const PagedItem& it) {
     return (it.n_tok * p.group + kRows - 1) / kRows;
 }
-// Keys and weight of row tile rt.  kHalves: a tile of at most kRows / 2 rows has
-// units of two key tiles, one for each half of the CTA.
-template <int kRows, int kKeys, bool kHalves>
+// Keys and weight of row tile rt.
+template <int kRows, int kKeys>
 __device__ __forceinline__ void paged_row_tile(const PagedAttnParams& p, int rt, PagedItem& it) {
     const int cap = p.b.pages_per_seq << p.b.page_shift;
     const int last = min((rt + 1) * kRows, it.n_tok * p.group) - 1;
     const int n = p.tree_mask ? it.n_tok : last / p.group + 1;
     it.rt = rt;
     it.keys = (int)min(max((long long)it.len + n, 0ll), (long long)cap);
-    const int unit = kHalves && it.n_tok * p.group - rt * kRows <= kRows / 2 ? 2 * kKeys : kKeys;
-    it.tiles = max((it.keys + unit - 1) / unit, 1);  // an item without keys still writes its zeros
+    it.tiles = max((it.keys + kKeys - 1) / kKeys, 1);  // an item without keys still writes its zeros
     it.weight = p.split ? p.extra + it.tiles : 1;
 }
 // The tiles of an item before its unit u.
 __device__ __forceinline__ int paged_tiles_before(const PagedAttnParams& p, int u) { return max(u - p.extra, 0); }
 // Units of sequence s, whose lane asks for it (s < 0: none).  A sequence of
 // many row tiles is added up by its whole warp.
-template <int kRows, int kKeys, bool kHalves>
+template <int kRows, int kKeys>
 __device__ __forceinline__ long long paged_seq_units(const PagedAttnParams& p, int s) {
     PagedItem it = {};
     int n = 0;
@@ -90,7 +88,7 @@ __device__ __forceinline__ long long paged_seq_units(const PagedAttnParams& p, i
     long long w = 0;
     if (n <= 4)
         for (int rt = 0; rt < n; rt++) {
-            paged_row_tile<kRows, kKeys, kHalves>(p, rt, it);
+            paged_row_tile<kRows, kKeys>(p, rt, it);
             w += it.weight;
         }
     for (uint32_t many = __ballot_sync(0xffffffffu, n > 4); many; many &= many - 1) {
@@ -100,7 +98,7 @@ __device__ __forceinline__ long long paged_seq_units(const PagedAttnParams& p, i
         o.len = __shfl_sync(0xffffffffu, it.len, from);
         long long sum = 0;
         for (int rt = threadIdx.x & 31; rt < tiles; rt += 32) {
-            paged_row_tile<kRows, kKeys, kHalves>(p, rt, o);
+            paged_row_tile<kRows, kKeys>(p, rt, o);
             sum += o.weight;
         }
 #pragma unroll
@@ -139,19 +137,19 @@ __device__ __forceinline__ long long cta_scan(PagedScan& sh, long long v, long l
 // The CTA's part [pos, end) and the item that holds its first unit; pos == end
 // for a CTA without work.  Parts are cut for min(gridDim.x, total) CTAs, so that
 // every one of those has some.  All threads take part and get the same.
-template <int kRows, int kKeys, bool kHalves, int kThreads>
+template <int kRows, int kKeys, int kThreads>
 __device__ __forceinline__ PagedStart paged_part(const PagedAttnParams& p, PagedScan& sh, long long& pos,
                                                  long long& end) {
     PagedStart st = {};
     PagedItem& it = st.it;
     const int n = p.b.n_seqs;
     long long total = 0, all;
-    long long mine = paged_seq_units<kRows, kKeys, kHalves>(p, (int)threadIdx.x < n ? (int)threadIdx.x : -1);
+    long long mine = paged_seq_units<kRows, kKeys>(p, (int)threadIdx.x < n ? (int)threadIdx.x : -1);
     long long upto = cta_scan<kThreads>(sh, mine, &total);
     const long long total0 = total;
     for (int base = kThreads; base < n; base += kThreads) {
         const int s = base + threadIdx.x;
-        cta_scan<kThreads>(sh, paged_seq_units<kRows, kKeys, kHalves>(p, s < n ? s : -1), &all);
+        cta_scan<kThreads>(sh, paged_seq_units<kRows, kKeys>(p, s < n ? s : -1), &all);
         total += all;
     }
     const long long parts = min((long long)gridDim.x, total);
@@ -173,7 +171,7 @@ __device__ __forceinline__ PagedStart paged_part(const PagedAttnParams& p, Paged
         }
         run += sum;
         const int s = base + kThreads + threadIdx.x;
-        mine = paged_seq_units<kRows, kKeys, kHalves>(p, s < n ? s : -1);
+        mine = paged_seq_units<kRows, kKeys>(p, s < n ? s : -1);
         upto = cta_scan<kThreads>(sh, mine, &sum);
     }
     paged_seq(p, sh.seq, it);
@@ -183,7 +181,7 @@ __device__ __forceinline__ PagedStart paged_part(const PagedAttnParams& p, Paged
         PagedItem o = it;
         long long w = 0;
         if (rt0 + lane < n_rt) {
-            paged_row_tile<kRows, kKeys, kHalves>(p, rt0 + lane, o);
+            paged_row_tile<kRows, kKeys>(p, rt0 + lane, o);
             w = (long long)o.weight * p.n_kv;
         }
         long long upto = w;
@@ -196,7 +194,7 @@ __device__ __forceinline__ PagedStart paged_part(const PagedAttnParams& p, Paged
         if (here || rt0 + 32 >= n_rt) {  // (pos lies in this sequence: one of its row tiles holds it)
             const int at = here ? __ffs(here) - 1 : 0;
             first += __shfl_sync(0xffffffffu, upto - w, at);
-            paged_row_tile<kRows, kKeys, kHalves>(p, rt0 + at, it);
+            paged_row_tile<kRows, kKeys>(p, rt0 + at, it);
             it.h = (int)((pos - first) / it.weight);
             st.first = first + (long long)it.h * it.weight;
             break;
@@ -206,7 +204,7 @@ __device__ __forceinline__ PagedStart paged_part(const PagedAttnParams& p, Paged
     return st;
 }
 // The item after `it`, if there is one.
-template <int kRows, int kKeys, bool kHalves>
+template <int kRows, int kKeys>
 __device__ __forceinline__ void paged_next(const PagedAttnParams& p, PagedItem& it) {
     if (++it.h < p.n_kv) return;
     it.h = 0;
@@ -215,7 +213,7 @@ __device__ __forceinline__ void paged_next(const PagedAttnParams& p, PagedItem& 
         rt = 0;
         paged_seq(p, it.s + 1, it);
     }
-    paged_row_tile<kRows, kKeys, kHalves>(p, rt, it);
+    paged_row_tile<kRows, kKeys>(p, rt, it);
 }
 
 // Whether token tok of the item's sequence sees entry e (0 <= e < keys).

@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int D = p.head_dim, ksteps = D >> 4;
     long long pos, end;
-    const PagedStart begin = paged_part<kRows, kPaKeys, false, kPaThreads>(p, scan, pos, end);
+    const PagedStart begin = paged_part<kRows, kPaKeys, kPaThreads>(p, scan, pos, end);
     const PagedWs<kRows, kDim> ws(p.ws, gridDim.x);
     if (p.ws && threadIdx.x == 0 && (pos < end || blockIdx.x == 0)) ws.info[blockIdx.x] = begin;
     if (pos >= end) {
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
         const bool whole = t0 == 0 && t1 == it.tiles;
         const int rows = min(kRows, it.n_tok * p.group - it.rt * kRows);
         PagedItem nx = it;
-        if (units < left) paged_next<kRows, kPaKeys, false>(p, nx);
+        if (units < left) paged_next<kRows, kPaKeys>(p, nx);
         else pdl_launch_dependents();
         if (threadIdx.x == 0 && (it.len < 0 || (long long)it.len + it.n_tok > (long long)p.b.pages_per_seq << p.b.page_shift))
             atomicOr(p.b.status, kStatusPaged);  // rows whose entries have no place

@@ -13,9 +13,6 @@
 //  the one after    looks the pages up and copies tiles of keys and values
 //                   (TMA, one box to a page) into a ring of slots
 //
-// An item of at most 128 rows gives both groups the same rows and a key tile
-// each of every two; the first group joins their outputs.
-//
 // The running maximum m only follows a row's true maximum when that passes it
 // by 2^8, so O is rarely rescaled; P stays below 2^8 and the sums are fp32.
 // P V is complete when S of the next tile is (matrix instructions complete in
@@ -51,7 +48,7 @@ struct PtShape {
     // Two groups: whole warpgroups, which share out the registers: at launch 168 a thread, of which
     // the third keeps 88 and the two of the rows take 208 (168 x 3 = 88 + 208 x 2).
     static constexpr int kThreads = kGroups == 2 ? 384 : 192;
-    static constexpr int kSmem = kGroups * kQBytes + kSlots * kSlot;  // (from a 1024-byte boundary on)
+    static constexpr int kSmem = kGroups * kQBytes + kSlots * kSlot + 1024;
     static constexpr int kOCol = kGroups * kKeys;         // TMEM column of the first group's O
 };
 
@@ -204,14 +201,13 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
     constexpr int kKeys = S::kKeys, kGroups = S::kGroups, kRows = S::kRows;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     __shared__ PagedScan scan;
-    __shared__ __align__(8) uint64_t bars[2 * S::kSlots + 4 * kGroups + 1 + 8];
-    __shared__ float2 s_ml[kGroups == 2 ? 128 : 1];  // the second group's maxima and sums of shared rows
+    __shared__ __align__(8) uint64_t bars[2 * S::kSlots + 4 * kGroups + 1];
     __shared__ uint32_t s_valid[8][kKeys / 32];
     __shared__ uint32_t s_tmem;
     __shared__ volatile int s_dead;
     __shared__ PagedItem s_items[4 * kGroups + 2][2];
-    unsigned char* sm = smem_raw;
-    const uint32_t base = smem_u32(sm);
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    unsigned char* sm = smem_raw + (base - smem_u32(smem_raw));
     const uint32_t ring = base + kGroups * S::kQBytes;
     const uint32_t bar0 = smem_u32(bars);
     auto full_bar = [&](int s) { return bar0 + 8u * s; };
@@ -221,9 +217,6 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
     auto p_bar = [&](int g) { return bar0 + 8u * (2 * S::kSlots + 2 * kGroups + g); };
     auto o_bar = [&](int g) { return bar0 + 8u * (2 * S::kSlots + 3 * kGroups + g); };
     const uint32_t end_bar = bar0 + 8u * (2 * S::kSlots + 4 * kGroups);
-    // shared rows, a quarter of them each: the second group is done; the first has taken its outputs
-    auto done_bar = [&](int q) { return end_bar + 8u * (1 + q); };
-    auto taken_bar = [&](int q) { return end_bar + 8u * (5 + q); };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -238,10 +231,6 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
             mbar_init_nofence(o_bar(g), 1);
         }
         mbar_init_nofence(end_bar, 1);
-        for (int q = 0; q < 4; q++) {
-            mbar_init_nofence(done_bar(q), 1);
-            mbar_init_nofence(taken_bar(q), 1);
-        }
         mbar_init_fence();
         s_dead = 0;
     }
@@ -263,7 +252,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
     const PagedWs<kRows, kDim> ws(p.ws, gridDim.x);
     {
         long long pos, end;
-        const PagedStart begin = paged_part<kRows, kKeys, kGroups == 2, S::kThreads>(p, scan, pos, end);
+        const PagedStart begin = paged_part<kRows, kKeys, S::kThreads>(p, scan, pos, end);
         busy = pos < end;
         if (p.ws && threadIdx.x == 0 && (busy || blockIdx.x == 0)) ws.info[blockIdx.x] = begin;
         left = (int)(end - pos);
@@ -304,15 +293,14 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
             __syncwarp();
             if (lane == 0) {
                 PagedItem i = *it;
-                paged_next<kRows, kKeys, kGroups == 2>(p, i);
+                paged_next<kRows, kKeys>(p, i);
                 *n = i;
             }
             __syncwarp();
             it = n;
         }
     };
-    // Whether the groups share the item's rows and take its key tiles by turns.
-    auto shared_rows = [&]() { return kGroups == 2 && it->n_tok * p.group - it->rt * kRows <= 128; };
+    auto groups_of = [&]() { return it->n_tok * p.group - it->rt * kRows > 128 ? kGroups : 1; };
 
     if (busy && warp < 4 * kGroups) {
         // ---- rows ------------------------------------------------------------------
@@ -350,27 +338,24 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(q_bar(g));
         };
-        uint32_t n_s = 0, n_o = 0, tile_no = 0;  // tiles of this group, pieces, tiles of the CTA so far
-        uint32_t n_shared = 0;                   // pieces of shared rows so far
-        auto loads_q = [&]() { return g == 0 || !shared_rows(); };
-        if (loads_q()) load_q();
+        uint32_t n_s = 0, n_o = 0, tile_no = 0;  // tiles of this group, pieces of it, tiles of the CTA so far
+        if (g < groups_of()) load_q();
         int pieces = 0;
         while (left > 0 && !fail) {
             int t0, t1;
             const int units = piece(t0, t1);
             if (t1 == 0) break;  // the part ends before the item's first tile
             const bool whole = t0 == 0 && t1 == it->tiles;
-            const bool shared = shared_rows();
-            const int row0 = it->rt * kRows + (shared ? 0 : g * 128), rows = it->n_tok * p.group;  // the group's first
-            const int row = row0 + in_group;
-            const bool on = row < rows, warp_on = row0 + (warp & 3) * 32 < rows;
+            const bool in = g < groups_of();
+            const int row = it->rt * kRows + g * 128 + in_group, rows = it->n_tok * p.group;
+            const bool on = in && row < rows;
+            const bool warp_on = in && it->rt * kRows + g * 128 + (warp & 3) * 32 < rows;
             const int tok = on ? row / p.group : 0;
             float m = -INFINITY, l = 0.0f;  // of scaled scores (log2), and the row's sum
             const int t_plain = (it->len + (p.tree_mask ? 0 : it->rt * kRows / p.group + 1)) / kKeys;  // before: all seen
             const float c2 = fmaxf(fabsf(p.scale_log2), 1e-30f);  // not 0: masked scores stay -inf
-            {
-                for (int u = t0; u < t1; u++, n_s++) {
-                    const int t = shared ? 2 * u + g : u, nth = shared ? 2 * (u - t0) + g : u - t0;
+            if (in) {
+                for (int t = t0; t < t1; t++, n_s++) {
                     if (!wait(s_bar(g), n_s)) break;
                     __syncwarp();
                     tc_fence_after();
@@ -380,7 +365,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
 #pragma unroll
                         for (int i = 0; i < kParts; i++) tmem_ld32(s_col + i * 32, s[i]);
                         tmem_wait_ld();
-                        const uint32_t* valid = s_valid[(tile_no + nth) & 7];
+                        const uint32_t* valid = s_valid[(tile_no + (t - t0)) & 7];
                         bool plain = t < t_plain;
 #pragma unroll
                         for (int i = 0; i < kParts; i++) plain = plain && valid[i] == 0xffffffffu;
@@ -411,7 +396,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                             const float keep = move ? pt_ex2(m - m1) : 1.0f;  // 0 from -inf
                             l *= keep;
                             m = m1;
-                            if (u > t0) {
+                            if (t > t0) {
 #pragma unroll 1
                                 for (int c = 0; c < D; c += 8) {
                                     uint32_t o[8];
@@ -448,40 +433,21 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                     if (lane == 0) mbar_arrive(p_bar(g));
                 }
             }
-            tile_no += (t1 - t0) * (shared ? 2 : 1);
+            tile_no += t1 - t0;
             // ---- the next item's rows (S of the last tile is done: Q is free), then this one's output ----
             if (fail) break;
             const PagedItem* const mine = it;
             const int piece_no = 2 * blockIdx.x + (pieces++ ? 1 : 0);
-            const int quad = warp & 3;
             next(units);
-            if (shared && g == 1) {  // to the first group, and on when it has taken them
-                if (!wait(o_bar(1), n_o++)) break;
-                s_ml[in_group] = make_float2(m, l);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(done_bar(quad));
-                if (!wait(taken_bar(quad), n_shared++)) break;
-                if (left > 0 && loads_q()) load_q();
-                continue;
-            }
-            if (!shared && left > 0 && loads_q()) load_q();
+            if (left > 0 && g < groups_of()) load_q();
+            if (!in) continue;
             if (!wait(o_bar(g), n_o)) break;
             n_o++;
-            float w0 = 1.0f, w1 = 0.0f;  // of shared rows: the groups' shares
-            if (shared) {
-                if (!wait(done_bar(quad), n_shared++)) break;
-                const float2 other = s_ml[in_group];
-                const float both = fmaxf(m, other.x), mu = both == -INFINITY ? 0.0f : both;
-                w0 = pt_ex2(m - mu);
-                w1 = pt_ex2(other.x - mu);
-                m = both;
-                l = l * w0 + other.y * w1;
-            }
             __syncwarp();
             tc_fence_after();
             if (warp_on) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                const int r = (shared ? 0 : g * 128) + in_group;
+                const int r = g * 128 + in_group;
                 C* out = static_cast<C*>(p.out) +
                          ((long long)(mine->row0 + tok) * p.n_heads + mine->h * p.group + row % p.group) * D;
                 const size_t at = (size_t)piece_no * kRows + r;
@@ -490,14 +456,6 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                     uint32_t o[32];
                     tmem_ld32(o_col + c, o);
                     tmem_wait_ld();
-                    if (kGroups == 2 && shared) {
-                        uint32_t o1[32];
-                        tmem_ld32(o_col + kDim + c, o1);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            o[j] = __float_as_uint(__uint_as_float(o[j]) * w0 + __uint_as_float(o1[j]) * w1);
-                    }
                     if (on && whole) {
                         float y[32];
 #pragma unroll
@@ -523,11 +481,6 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                 }
             }
             tc_fence_before();
-            if (shared) {  // the second group may go on; all of the first group's Q is free, by both groups' last S
-                __syncwarp();
-                if (lane == 0) mbar_arrive(taken_bar(quad));
-                if (left > 0) load_q();
-            }
         }
     } else if (busy && warp == 4 * kGroups) {
         // ---- matrix instructions -------------------------------------------------------
@@ -539,86 +492,76 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
         for (int g = 0; g < kGroups; g++) n_q[g] = n_p[g] = 0;
         auto slot_at = [&](uint32_t n) { return ring + (n % S::kSlots) * S::kSlot; };
         auto full = [&](uint32_t n) { return wait(full_bar(n % S::kSlots), n / S::kSlots); };
-        // (one elected lane) S of group g, of the rows of group q
-        auto scores = [&](int g, int q, uint32_t slot) {
-            const uint64_t a = sw128_desc(base + q * S::kQBytes), b = sw128_desc(slot);
+        auto scores = [&](int g, uint32_t slot) {
+            const uint64_t a = sw128_desc(base + g * S::kQBytes), b = sw128_desc(slot);
             const uint32_t d = tmem + g * kKeys;
+            if (pt_elect()) {
 #pragma unroll
-            for (int k = 0; k < kDim / 16; k++) {
-                if (k >= ksteps) break;
-                // 16 dims: 32 bytes on within a 128-byte row, then the next block of 64 dims
-                pt_mma_ss(d, a + ((k >> 2) * (128 * 128 / 16) + 2 * (k & 3)),
-                          b + ((k >> 2) * (kKeys * 128 / 16) + 2 * (k & 3)), id_s, k ? 1u : 0u);
+                for (int k = 0; k < kDim / 16; k++) {
+                    if (k >= ksteps) break;
+                    // 16 dims: 32 bytes on within a 128-byte row, then the next block of 64 dims
+                    pt_mma_ss(d, a + ((k >> 2) * (128 * 128 / 16) + 2 * (k & 3)),
+                              b + ((k >> 2) * (kKeys * 128 / 16) + 2 * (k & 3)), id_s, k ? 1u : 0u);
+                }
+                umma_commit(s_bar(g));
             }
-            umma_commit(s_bar(g));
-        };
-        auto outputs = [&](int g, uint32_t slot, bool add) {
-            const uint64_t b = sw128_mn_desc(slot, kKeys * 128);
-            const uint32_t d = tmem + S::kOCol + g * kDim, a = tmem + g * kKeys;
-#pragma unroll
-            for (int k = 0; k < kKeys / 16; k++)  // 16 keys: 2048 bytes on
-                pt_mma_ts(d, a + 8 * k, b + k * (2048 / 16), id_o, k || add ? 1u : 0u);
-        };
-        // Values of key tile t that no row sees may be anything: zeros instead.
-        auto clear_past = [&](int t, uint32_t slot) {
-            const int past = max(it->keys - t * kKeys, 0);
-            if (past >= kKeys) return;
-            for (int i = lane; i < (kKeys - past) * (kDim / 8); i += 32) {
-                const int r = past + i / (kDim / 8), c = i % (kDim / 8);
-                *reinterpret_cast<uint4*>(sm + (slot - base) + (c >> 3) * (kKeys * 128) + sw128_off(r, c & 7)) =
-                    make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
             __syncwarp();
         };
         while (left > 0 && !fail) {
             int t0, t1;
             const int units = piece(t0, t1);
             if (t1 == 0) break;  // the part ends before the item's first tile
-            const bool shared = shared_rows();
-            // the groups' tiles: one pair of slots for both, or one each
-            const int per = shared ? 4 : 2, off = shared ? 2 : 0;
-            for (int g = 0; g < kGroups && !fail; g++) {
-                if (g == 0 || shared) {
-                    if (!full(n_slot + g * off)) break;
-                }
-                if (g == 0 || !shared) {
-                    if (!wait(q_bar(g), n_q[g])) break;
-                    n_q[g]++;
-                }
+            const int ng = groups_of();
+            if (!full(n_slot)) break;
+            for (int g = 0; g < ng && !fail; g++) {
+                if (!wait(q_bar(g), n_q[g])) break;
+                n_q[g]++;
                 tc_fence_after();
-                if (pt_elect()) {
-                    scores(g, shared ? 0 : g, slot_at(n_slot + g * off));
-                    if (shared || g == kGroups - 1) umma_commit(empty_bar((n_slot + g * off) % S::kSlots));
-                }
-                __syncwarp();
+                scores(g, slot_at(n_slot));
             }
-            for (int u = t0; u < t1 && !fail; u++) {
-                const bool more = u + 1 < t1;
-#pragma unroll
-                for (int g = 0; g < kGroups; g++) {
-                    const uint32_t nv = n_slot + g * off + 1, nk = n_slot + g * off + per;  // this values', the next keys'
-                    if (fail) break;
-                    if (g == 0 || shared) {
-                        if (!full(nv)) break;
-                        clear_past(shared ? 2 * u + g : u, slot_at(nv));
-                        if (more && !full(nk)) break;
+            if (fail) break;
+            if (pt_elect()) umma_commit(empty_bar(n_slot % S::kSlots));
+            __syncwarp();
+            for (int t = t0; t < t1 && !fail; t++) {
+                const uint32_t nv = n_slot + 1, nk = n_slot + 2;  // this tile's values, the next one's keys
+                const bool more = t + 1 < t1;
+                if (!full(nv)) break;
+                const int past = it->keys - t * kKeys;  // values that no row sees may be anything: zeros instead
+                if (past < kKeys) {
+                    for (int i = lane; i < (kKeys - max(past, 0)) * (kDim / 8); i += 32) {
+                        const int r = max(past, 0) + i / (kDim / 8), c = i % (kDim / 8);
+                        *reinterpret_cast<uint4*>(sm + (slot_at(nv) - base) + (c >> 3) * (kKeys * 128) +
+                                                  sw128_off(r, c & 7)) = make_uint4(0, 0, 0, 0);
                     }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                for (int g = 0; g < ng && !fail; g++) {
                     if (!wait(p_bar(g), n_p[g])) break;
                     n_p[g]++;
                     tc_fence_after();
+                    const uint64_t b = sw128_mn_desc(slot_at(nv), kKeys * 128);
+                    const uint32_t d = tmem + S::kOCol + g * kDim, a = tmem + g * kKeys;
                     if (pt_elect()) {
-                        outputs(g, slot_at(nv), u > t0);
-                        if (more) scores(g, shared ? 0 : g, slot_at(nk));
-                        else umma_commit(o_bar(g));
-                        if (shared || g == kGroups - 1) {
-                            umma_commit(empty_bar(nv % S::kSlots));
-                            if (more) umma_commit(empty_bar(nk % S::kSlots));
-                        }
+#pragma unroll
+                        for (int k = 0; k < kKeys / 16; k++)  // 16 keys: 2048 bytes on
+                            pt_mma_ts(d, a + 8 * k, b + k * (2048 / 16), id_o, k || t > t0 ? 1u : 0u);
+                        if (!more) umma_commit(o_bar(g));
                     }
                     __syncwarp();
+                    if (more) {
+                        if (g == 0 && !full(nk)) break;
+                        tc_fence_after();
+                        scores(g, slot_at(nk));
+                    }
                 }
-                n_slot += per;
+                if (fail) break;
+                if (pt_elect()) {
+                    umma_commit(empty_bar(nv % S::kSlots));
+                    if (more) umma_commit(empty_bar(nk % S::kSlots));
+                }
+                __syncwarp();
+                n_slot += 2;
             }
             next(units);
         }
@@ -638,8 +581,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
             if (t1 == 0) break;  // the part ends before the item's first tile
             if (lane == 0 && (it->len < 0 || (long long)it->len + it->n_tok > (long long)p.b.pages_per_seq << p.b.page_shift))
                 atomicOr(p.b.status, kStatusPaged);  // rows whose entries have no place
-            const int per = shared_rows() ? 2 : 1;  // key tiles of a unit
-            for (int t = t0 * per; t < t1 * per && !fail; t++, tile_no++) {
+            for (int t = t0; t < t1 && !fail; t++, tile_no++) {
                 const int e = t * kKeys + lane * box;
                 int page = -1;
                 if (lane < boxes && e < it->keys) {
