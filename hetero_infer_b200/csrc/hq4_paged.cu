@@ -10,9 +10,12 @@
 // queries' type.
 //
 // The work is bytes: every value is read once and written once.  One thread
-// takes 8 consecutive values of a head's first half and the 8 they rotate
-// with (16-byte loads and stores of 16-bit types), so a head is a group of
-// D/16 threads, whose sum of squares is a shuffle tree.
+// takes 8 consecutive values of a head's first half and the 8 they rotate with
+// (16-byte loads and stores of 16-bit types), so a head is a group of D/16
+// lanes, whose sum of squares is a shuffle tree, and a warp has the heads that
+// fit its lanes, kAppendAhead times.  Its values are asked for first: where
+// they go (sequence, length, page, cosines: four loads that wait for one
+// another) is looked up meanwhile.
 #include <algorithm>
 
 #include "hq4_host.cuh"
@@ -23,8 +26,8 @@ namespace hq4 {
 int check_device_cap();
 int* status_word();
 
-constexpr int kAppendThreads = 256;
-constexpr int kAppendRows = 8;  // rows of a CTA at most
+constexpr int kAppendWarps = 8;
+constexpr int kAppendAhead = 2;  // times the heads of a warp (8191 rows: 1: 36.5 us, 2: 35.6, 3: 34.6; 8 rows: 2.9, 3.2, 4.5)
 
 struct AppendParams {
     const void *q, *k, *v;
@@ -33,92 +36,86 @@ struct AppendParams {
     float eps;
     const int* positions;
     const float *cos, *sin;
-    int max_pos, n_heads, n_kv, head_dim, rows_per_cta;
+    int max_pos, n_heads, n_kv, head_dim, warps_per_row;
     void *k_cache, *v_cache, *q_out;
     PagedBatch b;
 };
 
 template <class A, class C>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendParams p) {
-    __shared__ int s_pos[kAppendRows];
-    __shared__ long long s_at[kAppendRows];  // element of the entry in its page's first head; -1: not written
+__global__ void __launch_bounds__(kAppendWarps * 32, 4) paged_append_kernel(const __grid_constant__ AppendParams p) {
     pdl_launch_dependents();
     pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const long long w = (long long)blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
+    const int t = (int)(w / p.warps_per_row), part = (int)(w - (long long)t * p.warps_per_row);
+    if (t >= p.b.n_rows) return;
     const int D = p.head_dim, half = D >> 1;
-    const int row0 = blockIdx.x * p.rows_per_cta;
-    const int rows = min(p.rows_per_cta, p.b.n_rows - row0);
-    if (threadIdx.x < rows) {
-        const int t = row0 + threadIdx.x;
-        const int s = find_seq(p.b.cu_rows, p.b.n_seqs, t);
-        long long at = -1;
-        int pos = 0;
-        if (s >= 0) {
-            const int e = __ldg(p.b.lens + s) + (t - __ldg(p.b.cu_rows + s));
-            const int page = find_page(p.b, s, e);
-            pos = p.positions ? __ldg(p.positions + t) : e;
-            if (page >= 0 && pos >= 0 && pos < p.max_pos)
-                at = (long long)page * p.b.page_stride + (long long)(e & ((1 << p.b.page_shift) - 1)) * D;
-            else
-                atomicOr(p.b.status, kStatusPaged);
-        }
-        s_pos[threadIdx.x] = pos;
-        s_at[threadIdx.x] = at;
-    }
-    __syncthreads();
-    const int tph = D >> 4;                            // threads of a head
-    const int gw = tph <= 2 ? 2 : tph <= 4 ? 4 : tph <= 8 ? 8 : 16;  // lanes of a head: a power of two
-    const int lane = threadIdx.x & (gw - 1);
-    const int heads = p.n_heads + 2 * p.n_kv;
-    const int items = rows * heads;
-    const int step = kAppendThreads / gw;
-    const int rounds = (items + step - 1) / step;  // the same for all lanes: shuffles below are warp-wide
-    for (int r = 0; r < rounds; r++) {
-        const int it = r * step + threadIdx.x / gw;
-        const int row = it / heads, h = it - row * heads;
-        const bool on = it < items && lane < tph && s_at[min(row, kAppendRows - 1)] >= 0;
-        const int t = row0 + row;
-        const int j = lane * 8;
-        float a[8], b[8];
-        const bool is_q = h < p.n_heads, is_k = !is_q && h < p.n_heads + p.n_kv;
-        const int kh = h - p.n_heads - (is_k ? 0 : p.n_kv);
-        if (on) {
-            const A* src = is_q ? static_cast<const A*>(p.q) + t * p.q_stride + (long long)h * D
-                         : is_k ? static_cast<const A*>(p.k) + t * p.k_stride + (long long)kh * D
-                                : static_cast<const A*>(p.v) + t * p.v_stride + (long long)kh * D;
-            load8(src + j, a);
-            load8(src + half + j, b);
-        } else {
+    const int tph = D >> 4;                                          // lanes of a head
+    const int gw = tph <= 2 ? 2 : tph <= 4 ? 4 : tph <= 8 ? 8 : 16;  // those and idle ones: a power of two
+    const int sub = lane & (gw - 1), per = 32 / gw;
+    const int j = sub * 8, heads = p.n_heads + 2 * p.n_kv;
+    const int h0 = part * kAppendAhead * per + lane / gw;  // the thread's first head; the next ones `per` on
+    const bool on = sub < tph;
+    Raw8<A> ra[kAppendAhead], rb[kAppendAhead];
 #pragma unroll
-            for (int i = 0; i < 8; i++) a[i] = b[i] = 0.0f;
-        }
-        const float* nw = is_q ? p.q_norm : is_k ? p.k_norm : nullptr;
+    for (int i = 0; i < kAppendAhead; i++) {
+        const int h = h0 + i * per;
+        if (!on || h >= heads) continue;
+        const A* src = h < p.n_heads ? static_cast<const A*>(p.q) + t * p.q_stride + (long long)h * D
+                     : h < p.n_heads + p.n_kv
+                         ? static_cast<const A*>(p.k) + t * p.k_stride + (long long)(h - p.n_heads) * D
+                         : static_cast<const A*>(p.v) + t * p.v_stride + (long long)(h - p.n_heads - p.n_kv) * D;
+        ra[i].load(src + j);
+        rb[i].load(src + half + j);
+    }
+    const int s = find_seq(p.b.cu_rows, p.b.n_seqs, t);
+    if (s < 0) return;
+    const int e = __ldg(p.b.lens + s) + (t - __ldg(p.b.cu_rows + s));
+    const int page = find_page(p.b, s, e), pos = p.positions ? __ldg(p.positions + t) : e;
+    if (page < 0 || pos < 0 || pos >= p.max_pos) {
+        if (part == 0 && lane == 0) atomicOr(p.b.status, kStatusPaged);
+        return;
+    }
+    // the entry's place in its page's first head
+    const long long at = (long long)page * p.b.page_stride + (long long)(e & ((1 << p.b.page_shift) - 1)) * D;
+    float c[8], sn[8];
+    if (on) {
+        load8(p.cos + (size_t)pos * half + j, c);
+        load8(p.sin + (size_t)pos * half + j, sn);
+    }
+#pragma unroll
+    for (int i = 0; i < kAppendAhead; i++) {
+        const int h = h0 + i * per;
+        const bool is_q = h < p.n_heads, is_k = !is_q && h < p.n_heads + p.n_kv;
+        float a[8], b[8];
+        ra[i].get(a);
+        rb[i].get(b);
         if (p.q_norm || p.k_norm) {
             float ss = 0.0f;
+            if (on && h < heads)
 #pragma unroll
-            for (int i = 0; i < 8; i++) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+                for (int x = 0; x < 8; x++) ss = fmaf(a[x], a[x], fmaf(b[x], b[x], ss));
             for (int o = gw >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (nw && on) {
+            const float* nw = is_q ? p.q_norm : is_k ? p.k_norm : nullptr;
+            if (on && nw) {
                 const float inv = 1.0f / sqrtf(ss / (float)D + p.eps);
                 float wa[8], wb[8];
                 load8(nw + j, wa);
                 load8(nw + half + j, wb);
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    a[i] = a[i] * inv * wa[i];
-                    b[i] = b[i] * inv * wb[i];
+                for (int x = 0; x < 8; x++) {
+                    a[x] = a[x] * inv * wa[x];
+                    b[x] = b[x] * inv * wb[x];
                 }
             }
         }
-        if (!on) continue;
+        if (!on || h >= heads) continue;
         if (is_q || is_k) {
-            float c[8], s[8];
-            load8(p.cos + (size_t)s_pos[row] * half + j, c);
-            load8(p.sin + (size_t)s_pos[row] * half + j, s);
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float x = a[i], y = b[i];
-                a[i] = x * c[i] - y * s[i];
-                b[i] = y * c[i] + x * s[i];
+            for (int x = 0; x < 8; x++) {
+                const float y = a[x], z = b[x];
+                a[x] = y * c[x] - z * sn[x];
+                b[x] = z * c[x] + y * sn[x];
             }
         }
         if (is_q) {
@@ -126,8 +123,8 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
             store8(dst + j, a);
             store8(dst + half + j, b);
         } else {
-            C* dst = static_cast<C*>(is_k ? p.k_cache : p.v_cache) + s_at[row] +
-                     ((long long)kh << p.b.page_shift) * D;
+            const int kh = h - p.n_heads - (is_k ? 0 : p.n_kv);
+            C* dst = static_cast<C*>(is_k ? p.k_cache : p.v_cache) + at + ((long long)kh << p.b.page_shift) * D;
             store8(dst + j, a);
             store8(dst + half + j, b);
         }
@@ -140,8 +137,8 @@ static int launch_append(const AppendParams& p, cudaStream_t st) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((p.b.n_rows + p.rows_per_cta - 1) / p.rows_per_cta);
-    lc.blockDim = dim3(kAppendThreads);
+    lc.gridDim = dim3((unsigned)(((long long)p.b.n_rows * p.warps_per_row + kAppendWarps - 1) / kAppendWarps));
+    lc.blockDim = dim3(kAppendWarps * 32);
     lc.stream = st;
     lc.attrs = attr;
     lc.numAttrs = 1;
@@ -225,8 +222,8 @@ extern "C" int hq4_paged_append(const void* q, const void* k, const void* v, int
     p.k_cache = k_cache;
     p.v_cache = v_cache;
     p.q_out = q_out;
-    // rows of a CTA: enough that its threads have work, few while there are few rows
-    p.rows_per_cta = n_rows < 4 * 148 ? 1 : std::min(kAppendRows, std::max(1, n_rows / (4 * 148)));
+    const int tph = head_dim >> 4, per = 32 / (tph <= 2 ? 2 : tph <= 4 ? 4 : tph <= 8 ? 8 : 16);
+    p.warps_per_row = (n_heads + 2 * n_kv + per * kAppendAhead - 1) / (per * kAppendAhead);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (cache_type == HQ4_BF16)
         return act_type == HQ4_F32 ? launch_append<float, __nv_bfloat16>(p, st)

@@ -107,6 +107,34 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 
+// Eight consecutive elements (16-byte aligned) as they lie in memory.
+template <class T>
+struct Raw8 {
+    uint4 v[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    }
+    __device__ __forceinline__ void get(float (&f)[8]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                f[4 * i] = __uint_as_float(v[i].x);
+                f[4 * i + 1] = __uint_as_float(v[i].y);
+                f[4 * i + 2] = __uint_as_float(v[i].z);
+                f[4 * i + 3] = __uint_as_float(v[i].w);
+            }
+        } else {
+            const uint32_t w[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 x = unpack2<T>(w[i]);
+                f[2 * i] = x.x;
+                f[2 * i + 1] = x.y;
+            }
+        }
+    }
+};
 // Eight consecutive elements (16-byte aligned) as fp32, and back.
 __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
     const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
