@@ -30,6 +30,7 @@ struct PagedAttnParams {
     int mask_words;
     int split;                     // units are key tiles; else whole items
     int extra;                     // units of an item before its tiles
+    int take;                      // rows of a joining CTA
     void* ws;
     PagedBatch b;
 };
@@ -134,6 +135,20 @@ __device__ __forceinline__ long long cta_scan(PagedScan& sh, long long v, long l
     return v;
 }
 
+// Where the parts are cut: part c of min(ctas, total) begins at unit
+// floor(c total / parts), by 32-bit divisions unless the units are very many.
+struct PagedCuts {
+    long long q;
+    unsigned r, parts;
+    __device__ __forceinline__ PagedCuts(long long total, int ctas) {
+        parts = (unsigned)min((long long)ctas, total);
+        const unsigned by = max(parts, 1u);
+        q = total >> 32 ? total / by : (long long)((unsigned)total / by);
+        r = (unsigned)(total - q * by);
+    }
+    __device__ __forceinline__ long long at(unsigned c) const { return c * q + c * r / parts; }  // c, r < 2^16
+};
+
 // The CTA's part [pos, end) and the item that holds its first unit; pos == end
 // for a CTA without work.  Parts are cut for min(gridDim.x, total) CTAs, so that
 // every one of those has some.  All threads take part and get the same.
@@ -152,12 +167,12 @@ __device__ __forceinline__ PagedStart paged_part(const PagedAttnParams& p, Paged
         cta_scan<kThreads>(sh, paged_seq_units<kRows, kKeys>(p, s < n ? s : -1), &all);
         total += all;
     }
-    const long long parts = min((long long)gridDim.x, total);
+    const PagedCuts cuts(total, gridDim.x);
     pos = end = 0;
     st.total = total;
-    if ((long long)blockIdx.x >= parts) return st;
-    pos = blockIdx.x * total / parts;
-    end = (blockIdx.x + 1) * total / parts;
+    if (blockIdx.x >= cuts.parts) return st;
+    pos = cuts.at(blockIdx.x);
+    end = cuts.at(blockIdx.x + 1);
     long long run = 0, sum = total0;
     for (int base = 0;; base += kThreads) {  // ends at the chunk that holds pos: pos < total
         if (pos < run + sum) {
@@ -291,43 +306,53 @@ static_assert(sizeof(PagedStart) % 16 == 0, "the pieces behind the items keep th
 // CTA (c, y): if part c begins inside an item, and c is the first part that
 // does in that item, joins rows of the item's pieces.  With few rows to an item
 // (decode, where a long sequence has many pieces) a CTA takes one, its warps a
-// part of the pieces each; else a warp takes a row.  A lane has 4 consecutive
+// part of the pieces each; else `take`, a warp a row.  A lane has 4 consecutive
 // values of each 128.  The order of the sums does not depend on timing.
 constexpr int kCombineWarps = 4;
-template <int kRows>
-constexpr int combine_rows() { return kRows <= 32 ? 1 : 8; }  // of a CTA
 template <class A, class C, int kRows, int kDim>
 __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const __grid_constant__ PagedAttnParams p,
                                                                            int ctas) {
-    constexpr int kTake = combine_rows<kRows>();
-    constexpr int kShare = kTake == 1 ? kCombineWarps : 1;  // warps of a row
-    constexpr int kPer = (kDim + 127) / 128;
+    constexpr int kShare = kRows <= 32 ? kCombineWarps : 1;  // warps of a row
+    constexpr int kPer = (kDim + 127) / 128, kDeep = 8 / kPer;  // pieces whose values are asked for at once
     __shared__ float4 s_acc[kShare][kPer][32];
     __shared__ float s_l[kShare];
     pdl_launch_dependents();
     pdl_wait();
     const PagedWs<kRows, kDim> ws(p.ws, ctas);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = p.head_dim;
     const int c = blockIdx.x + 1;
     const PagedStart st = ws.info[c];
-    const long long total = ws.info[0].total;
-    const long long parts = min((long long)ctas, total);
-    if (c >= parts) return;
     const PagedItem& it = st.it;
-    const long long start = c * total / parts, before = (c - 1) * total / parts;
+    const PagedCuts cuts(ws.info[0].total, ctas);
+    if (c >= (int)cuts.parts) return;
     // nothing to join where no tile lies before this cut, or one lies before the last cut
-    if (start - st.first <= p.extra || before - st.first > p.extra) return;
+    const long long before = cuts.at(c - 1);
+    if (cuts.at(c) - st.first <= p.extra || before - st.first > p.extra) return;
     const int rows = min(kRows, it.n_tok * p.group - it.rt * kRows);
     const int first_piece = 2 * (c - 1) + (st.first <= before ? 0 : 1);
     // pieces: that one, then the first ones of parts c, c + 1, ... up to the one with the item's last unit
     const long long last = st.first + it.weight - 1;
-    long long owner = last * parts / total;  // or the one after it, by rounding
-    while ((owner + 1) * total / parts <= last) owner++;
-    const int n = (int)(owner - (c - 1)) + 1;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = p.head_dim;
-    const int mine = kTake == 1 ? warp : 0;  // the warp's share of the pieces: each kShare-th
-    for (int r = blockIdx.y * kTake + (kTake == 1 ? 0 : warp); r < min(rows, (int)(blockIdx.y + 1) * kTake);
-         r += kCombineWarps) {
+    int owner = min((int)__fdividef((float)last, (float)cuts.q + __fdividef((float)cuts.r, (float)cuts.parts)),
+                    (int)cuts.parts - 1);
+    while (cuts.at(owner) > last) owner--;
+    while (cuts.at(owner + 1) <= last) owner++;
+    const int n = owner - (c - 1) + 1;
+    const int mine = kShare > 1 ? warp : 0;  // the warp's share of the pieces: each kShare-th
+    const int end = kShare > 1 ? min(rows, (int)blockIdx.y + 1) : min(rows, (int)(blockIdx.y + 1) * p.take);
+    for (int r = kShare > 1 ? blockIdx.y : blockIdx.y * p.take + warp; r < end; r += kCombineWarps) {
         auto at = [&](int i) { return (size_t)(i == 0 ? first_piece : 2 * (c - 1 + i)) * kRows + r; };
+        float4 v[kDeep][kPer];
+        auto ask = [&](int i0) {  // values of the share's next pieces, zeros behind the last
+#pragma unroll
+            for (int i = 0; i < kDeep; i++) {
+                const float* o = ws.o + at(min(i0 + i * kShare, n - 1)) * kDim;
+#pragma unroll
+                for (int j = 0; j < kPer; j++)
+                    v[i][j] = i0 + i * kShare < n && lane * 4 + 128 * j < D
+                                  ? *reinterpret_cast<const float4*>(o + lane * 4 + 128 * j) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+        };
+        ask(mine);  // (before the weights are known)
         float m = -INFINITY;
         for (int i = lane; i < n; i += 32) m = fmaxf(m, ws.ml[at(i)].x);
 #pragma unroll
@@ -344,20 +369,19 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
                 w = exp2f(ml.x - mu);
                 l = fmaf(ml.y, w, l);
             }
-            const int k = min(32, (n - i0 + kShare - 1) / kShare);
-#pragma unroll 8
-            for (int i = 0; i < k; i++) {
-                const float wi = __shfl_sync(0xffffffffu, w, i);
-                const float* o = ws.o + at(i0 + i * kShare) * kDim;
+            for (int i1 = 0; i1 < 32 && i0 + i1 * kShare < n; i1 += kDeep) {
 #pragma unroll
-                for (int j = 0; j < kPer; j++)
-                    if (lane * 4 + 128 * j < D) {
-                        const float4 v = *reinterpret_cast<const float4*>(o + lane * 4 + 128 * j);
-                        acc[j].x = fmaf(v.x, wi, acc[j].x);
-                        acc[j].y = fmaf(v.y, wi, acc[j].y);
-                        acc[j].z = fmaf(v.z, wi, acc[j].z);
-                        acc[j].w = fmaf(v.w, wi, acc[j].w);
+                for (int i = 0; i < kDeep; i++) {
+                    const float wi = __shfl_sync(0xffffffffu, w, i1 + i);  // 0 behind the last
+#pragma unroll
+                    for (int j = 0; j < kPer; j++) {
+                        acc[j].x = fmaf(v[i][j].x, wi, acc[j].x);
+                        acc[j].y = fmaf(v[i][j].y, wi, acc[j].y);
+                        acc[j].z = fmaf(v[i][j].z, wi, acc[j].z);
+                        acc[j].w = fmaf(v[i][j].w, wi, acc[j].w);
                     }
+                }
+                if (i0 + (i1 + kDeep) * kShare < n) ask(i0 + (i1 + kDeep) * kShare);
             }
         }
 #pragma unroll
@@ -399,9 +423,11 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
 // How a call is run (host).
 struct PaPlan {
     int tc;     // tensor-memory kernel (hq4_paged_tc.cuh), else the warp-level one (hq4_paged_rows.cuh)
-    int nt;     // 8-row tiles of the latter
+    int nt;     // 8-row tiles of the latter, and its warps
+    int warps;
     int dim;    // head_dim rounded up to what the kernels are built for
     int ctas, split, extra;
+    int join, take;  // rows of an item at most, and those of a CTA that joins pieces
     long long ws;
 };
 

@@ -20,8 +20,6 @@
 
 namespace hq4 {
 
-constexpr int kPaWarps = 4;
-constexpr int kPaThreads = kPaWarps * 32;
 constexpr int kPaKeys = 16;  // keys of a tile
 
 template <int kDim>
@@ -32,8 +30,8 @@ struct PaShape {
 };
 template <class A, class C>
 constexpr int pa_terms() { return sizeof(A) == 2 ? 1 : Elem<C>::code == HQ4_BF16 ? 3 : 2; }
-template <int kDim, int kRows, int kTerms>
-constexpr int pa_smem() { return kPaWarps * PaShape<kDim>::kRing + kTerms * kRows * kDim * 2; }
+template <int kDim, int kRows, int kTerms, int W>
+constexpr int pa_smem() { return W * PaShape<kDim>::kRing + kTerms * kRows * kDim * 2; }
 
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -69,8 +67,9 @@ __device__ __forceinline__ float ex2(float x) {
 template <int kDim>
 __device__ __forceinline__ int tile_at(int r, int c) { return r * (kDim * 2) + ((c ^ (r & 7)) << 4); }
 
-template <class A, class C, int kDim, int NT>
-__global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
+// NT: 8-row tiles; W: warps.
+template <class A, class C, int kDim, int NT, int W>
+__global__ void __launch_bounds__(W * 32) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
     constexpr int kRows = 8 * NT, kTerms = pa_terms<A, C>(), kStages = PaShape<kDim>::kStages;
     constexpr int kTile = PaShape<kDim>::kTile, kRing = PaShape<kDim>::kRing;
     constexpr int kChunks = kDim / 8, kOs = kDim + 4;
@@ -79,13 +78,13 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     constexpr bool kAhead = kRows * kOs * 4 <= 2 * kTile;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ PagedScan scan;
-    __shared__ float s_m[kPaWarps][kRows], s_l[kPaWarps][kRows], s_qs[kRows];
-    __shared__ int s_os[kPaWarps];  // where in shared memory each warp has left its outputs
+    __shared__ float s_m[W][kRows], s_l[W][kRows], s_qs[kRows];
+    __shared__ int s_os[W];  // where in shared memory each warp has left its outputs
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int D = p.head_dim, ksteps = D >> 4;
     long long pos, end;
-    const PagedStart begin = paged_part<kRows, kPaKeys, kPaThreads>(p, scan, pos, end);
+    const PagedStart begin = paged_part<kRows, kPaKeys, W * 32>(p, scan, pos, end);
     const PagedWs<kRows, kDim> ws(p.ws, gridDim.x);
     if (p.ws && threadIdx.x == 0 && (pos < end || blockIdx.x == 0)) ws.info[blockIdx.x] = begin;
     if (pos >= end) {
@@ -96,7 +95,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
     int left = (int)(end - pos), from = (int)(pos - begin.first);  // units still to do; the first of them in the item
     int pieces = 0;
     const uint32_t ring_u = smem_u32(smem + warp * kRing);
-    unsigned char* qs = smem + kPaWarps * kRing;
+    unsigned char* qs = smem + W * kRing;
     const uint32_t qs_u = smem_u32(qs);
     const C* kc = static_cast<const C*>(p.k);
     const C* vc = static_cast<const C*>(p.v);
@@ -141,11 +140,11 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
         oks = 0;
         int page[kStages];
 #pragma unroll
-        for (int s = 0; s < kStages; s++) page[s] = look_up(it, t0 + warp + s * kPaWarps, t1);
+        for (int s = 0; s < kStages; s++) page[s] = look_up(it, t0 + warp + s * W, t1);
 #pragma unroll
         for (int s = 0; s < kStages - 1; s++) {
             const int at = stage + s < kStages ? stage + s : stage + s - kStages;
-            oks |= (unsigned long long)load_tile(it, t0 + warp + s * kPaWarps, t1, page[s], at) << (16 * s);
+            oks |= (unsigned long long)load_tile(it, t0 + warp + s * W, t1, page[s], at) << (16 * s);
         }
         page_next = page[kStages - 1];
     };
@@ -172,7 +171,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
             atomicOr(p.b.status, kStatusPaged);  // rows whose entries have no place
 
         // ---- the queries, as 16-bit terms ----------------------------------
-        for (int r = warp; r < kRows; r += kPaWarps) {
+        for (int r = warp; r < kRows; r += W) {
             const int row = it.rt * kRows + r;
             const bool on = r < rows;
             const A* src = static_cast<const A*>(p.q) + (long long)(it.row0 + (on ? row / p.group : 0)) * p.q_stride +
@@ -249,12 +248,12 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
             }
         }
         const int first_tok = it.rt * kRows / p.group;
-        for (int t = t0 + warp; t < t1; t += kPaWarps) {
+        for (int t = t0 + warp; t < t1; t += W) {
             int ahead = stage + kStages - 1;
             if (ahead >= kStages) ahead -= kStages;
             __syncwarp();  // the tile that is overwritten was read by all lanes
-            const uint32_t more = load_tile(it, t + (kStages - 1) * kPaWarps, t1, page_next, ahead);
-            page_next = look_up(it, t + kStages * kPaWarps, t1);
+            const uint32_t more = load_tile(it, t + (kStages - 1) * W, t1, page_next, ahead);
+            page_next = look_up(it, t + kStages * W, t1);
             const uint32_t ok = (uint32_t)oks & 0xffffu;
             oks = (oks >> 16) | (unsigned long long)more << (16 * (kStages - 2));
             cp_async_wait<kStages - 1>();
@@ -403,27 +402,27 @@ __global__ void __launch_bounds__(kPaThreads) paged_attn_kernel(const __grid_con
         }
         __syncthreads();
         const int piece = 2 * blockIdx.x + (pieces++ ? 1 : 0);
-        for (int r = warp; r < rows; r += kPaWarps) {
-            float mm = -INFINITY, ll = 0.0f, w[kPaWarps];
+        for (int r = warp; r < rows; r += W) {
+            float mm = -INFINITY, ll = 0.0f, w[W];
 #pragma unroll
-            for (int i = 0; i < kPaWarps; i++) mm = fmaxf(mm, s_m[i][r]);
+            for (int i = 0; i < W; i++) mm = fmaxf(mm, s_m[i][r]);
             const float mu = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
-            for (int i = 0; i < kPaWarps; i++) {
+            for (int i = 0; i < W; i++) {
                 w[i] = exp2f(s_m[i][r] - mu);
                 ll = fmaf(s_l[i][r], w[i], ll);
             }
             const int row = it.rt * kRows + r;
             if (whole)
 #pragma unroll
-                for (int i = 0; i < kPaWarps; i++) w[i] = ll == 0.0f ? 0.0f : w[i] / ll;
+                for (int i = 0; i < W; i++) w[i] = ll == 0.0f ? 0.0f : w[i] / ll;
             A* out = static_cast<A*>(p.out) + ((long long)(it.row0 + row / p.group) * p.n_heads + it.h * p.group + row % p.group) * D;
             float* part = ws.o + ((size_t)piece * kRows + r) * kDim;
             bool bad = false;
             for (int d = lane; d < D; d += 32) {
                 float y = 0.0f;
 #pragma unroll
-                for (int i = 0; i < kPaWarps; i++)
+                for (int i = 0; i < W; i++)
                     y = fmaf(reinterpret_cast<const float*>(smem + s_os[i])[r * kOs + d], w[i], y);
                 if (whole) {
                     if (ll == 0.0f) y = 0.0f;
@@ -460,30 +459,34 @@ static inline cudaError_t launch_pdl_kernel(const void* fn, dim3 grid, dim3 bloc
     return cudaLaunchKernelExC(&lc, fn, args);
 }
 
-template <class A, class C, int kDim, int NT>
+template <class A, class C, int kDim, int NT, int W>
 static int launch_pa(PagedAttnParams p, const PaPlan& pl, cudaStream_t st) {
-    constexpr int smem = pa_smem<kDim, 8 * NT, pa_terms<A, C>()>();
-    auto kern = paged_attn_kernel<A, C, kDim, NT>;
+    constexpr int smem = pa_smem<kDim, 8 * NT, pa_terms<A, C>(), W>();
+    auto kern = paged_attn_kernel<A, C, kDim, NT, W>;
     static PerDeviceOnce once;
     if (smem_opt_in(once, kern, smem) != cudaSuccess) return HQ4_ERR_LAUNCH;
     void* args[] = {&p};
-    if (launch_pdl_kernel((const void*)kern, dim3(pl.ctas), dim3(kPaThreads), smem, st, args) != cudaSuccess)
+    if (launch_pdl_kernel((const void*)kern, dim3(pl.ctas), dim3(W * 32), smem, st, args) != cudaSuccess)
         return HQ4_ERR_LAUNCH;
     if (!pl.split || pl.ctas < 2) return HQ4_OK;
     int ctas = pl.ctas;
     void* cargs[] = {&p, &ctas};
     return launch_pdl_kernel((const void*)paged_combine_kernel<A, C, 8 * NT, kDim>,
-                             dim3(pl.ctas - 1, (8 * NT) / combine_rows<8 * NT>()), dim3(kCombineWarps * 32),
-                             0, st, cargs) == cudaSuccess
+                             dim3(pl.ctas - 1, pl.join), dim3(kCombineWarps * 32), 0, st, cargs) == cudaSuccess
                ? HQ4_OK
                : HQ4_ERR_LAUNCH;
 }
 template <class A, class C, int kDim>
 static int launch_pa_nt(const PagedAttnParams& p, const PaPlan& pl, cudaStream_t st) {
-    if constexpr (kDim <= 128) {
-        if (pl.nt == 4) return launch_pa<A, C, kDim, 4>(p, pl, st);
+    if (pl.warps == 2) return launch_pa<A, C, kDim, 1, 2>(p, pl, st);
+    // 16-bit activations of more rows have the tensor-memory kernel
+    if constexpr (sizeof(A) == 4 && kDim <= 128) {
+        if (pl.nt == 4) return launch_pa<A, C, kDim, 4, 4>(p, pl, st);
     }
-    return pl.nt == 1 ? launch_pa<A, C, kDim, 1>(p, pl, st) : launch_pa<A, C, kDim, 2>(p, pl, st);
+    if constexpr (sizeof(A) == 4 || kDim == 64) {
+        if (pl.nt == 2) return launch_pa<A, C, kDim, 2, 4>(p, pl, st);
+    }
+    return launch_pa<A, C, kDim, 1, 4>(p, pl, st);
 }
 template <class A, class C>
 static int launch_pa_dim(const PagedAttnParams& p, const PaPlan& pl, cudaStream_t st) {
