@@ -200,6 +200,12 @@ extern "C" int hq4_paged_append(const void* q, const void* k, const void* v, int
          (uintptr_t)q_norm | (uintptr_t)k_norm) & 15 ||
         ((uintptr_t)positions & 3) || ((q_stride | k_stride | v_stride) & per16))
         return HQ4_ERR_ALIGN;
+    const int elem = act_type == HQ4_F32 ? 4 : 2;
+    const long long q_row = (long long)n_heads * head_dim, k_row = (long long)n_kv * head_dim, out_bytes = n_rows * q_row * elem;
+    if (rows_overlap(q, n_rows, q_stride, q_row, elem, q_out, out_bytes) ||
+        rows_overlap(k, n_rows, k_stride, k_row, elem, q_out, out_bytes) ||
+        rows_overlap(v, n_rows, v_stride, k_row, elem, q_out, out_bytes))
+        return HQ4_ERR_SHAPE;
     if (int rc = check_device_cap()) return rc;
     p.b.status = status_word();
     if (!p.b.status) return HQ4_ERR_LAUNCH;

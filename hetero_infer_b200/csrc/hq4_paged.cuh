@@ -52,6 +52,13 @@ __device__ __forceinline__ int find_page(const PagedBatch& b, int s, int e) {
     return (unsigned)p < (unsigned)b.n_pages ? p : -1;
 }
 
+// Whether `rows` rows of `row` elements, `stride` apart, reach into the n_bytes at b (host).
+static inline bool rows_overlap(const void* a, long long rows, long long stride, long long row, int elem_bytes,
+                                const void* b, long long n_bytes) {
+    const __int128 from = (intptr_t)a, to = from + ((__int128)(rows - 1) * stride + row) * elem_bytes;
+    return from < (__int128)(intptr_t)b + n_bytes && (intptr_t)b < to;
+}
+
 template <class T>
 struct Elem;
 template <>

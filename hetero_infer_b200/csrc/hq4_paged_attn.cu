@@ -79,6 +79,9 @@ static int paged_attention(const void* q, int act_type, int n_rows, int n_heads,
     if ((((uintptr_t)q | (uintptr_t)out) & 15) || (q_stride & (act_type == HQ4_F32 ? 3 : 7)) ||
         ((uintptr_t)tree_mask & 3))
         return HQ4_ERR_ALIGN;
+    const long long q_row = (long long)n_heads * head_dim;
+    const int elem = act_type == HQ4_F32 ? 4 : 2;
+    if (rows_overlap(q, n_rows, q_stride, q_row, elem, out, n_rows * q_row * elem)) return HQ4_ERR_SHAPE;
     if (int rc = check_device_cap()) return rc;
     p.b.status = status_word();
     const int sms = device_sms();

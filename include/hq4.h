@@ -309,9 +309,9 @@ int hq4_advance_position(int* pos, int delta, void* stream);
 #define HQ4_F16 2
 
 /* Appends the rows of k (rotated) and v to their pages and writes the rotated
- * queries to q_out [n_rows][n_heads][head_dim] (which must not overlap q).
- * Rotation as hq4_qkv_rope: half-split, cos/sin tables [max_pos][head_dim/2];
- * a row's position is its entry's number, or positions[row] where positions
+ * queries to q_out [n_rows][n_heads][head_dim] (which must not overlap q, k or
+ * v).  Rotation as hq4_qkv_rope: half-split, cos/sin tables
+ * [max_pos][head_dim/2]; a row's position is its entry's number, or positions[row] where positions
  * is not NULL (the nodes of a drafted tree: entries one after another,
  * positions by depth).  q_norm / k_norm ([head_dim], each may be NULL): an RMS
  * norm of each query / key head before the rotation, x / sqrt(mean(x^2) + eps)
@@ -326,9 +326,9 @@ int hq4_paged_append(const void* q, const void* k, const void* v, int act_type, 
 
 /* Grouped-query attention of the batch's rows over the cache: row i of
  * sequence s attends to entries [0, lens[s] + i], its own among them
- * (hq4_paged_append first).  out [n_rows][n_heads][head_dim]; a row that sees
- * nothing is zeros.  What lies in entries that a row does not see (stale
- * pages, NaN, infinities) does not reach it.  The workspace
+ * (hq4_paged_append first).  out [n_rows][n_heads][head_dim] must not overlap
+ * q; a row that sees nothing is zeros.  What lies in entries that a row does
+ * not see (stale pages, NaN, infinities) does not reach it.  The workspace
  * (hq4_paged_attention_workspace_bytes, 128-byte aligned; may be NULL where
  * that is 0) is written and read by one call: calls that can run at the same
  * time must not share it.  Deterministic; allocates nothing. */

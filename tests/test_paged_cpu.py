@@ -132,3 +132,16 @@ def test_oracle_sample_is_the_one_row_oracle():
         got, _, gap = op.sample(x, u, t, 0, p)
         if gap > 1e-4:
             assert got == one.sample_with_u(x, t, p, u)
+
+
+@pytest.mark.parametrize("at,rc", [(0, -1), (3 * 512 * 2 + 512 * 2 - 16, -1), (-(4 * 512 * 2 - 16), -1)])
+def test_outputs_over_inputs_refused(at, rc):
+    """4 rows of 512 values: an output that begins or ends inside them."""
+    far = 1 << 30
+    assert attention(q=P * 8, out=P * 8 + at) == rc
+    assert attention(tree=True, q=P * 8, out=P * 8 + at) == rc
+    assert append(q=P * 8, k=far, v=far, out=P * 8 + at) == rc
+    assert append(q=far, k=P * 8, v=far, ks=512, out=P * 8 + min(at, 3 * 512 * 2 + 128 * 2 - 16)) == rc
+    assert append(q=far, k=far, v=P * 8, vs=512, out=P * 8 + min(at, 3 * 512 * 2 + 128 * 2 - 16)) == rc
+    # side by side: nothing to refuse before the device is looked at
+    assert attention(q=P * 8, out=P * 8 + 4 * 512 * 2) not in (-1, -2)

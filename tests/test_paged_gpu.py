@@ -623,3 +623,80 @@ def test_a_served_run(cuda):
     tok = ops.sample_rows(logits, torch.tensor([0.3, 0.9], dtype=torch.float64).cuda(),
                           temperature=torch.tensor([0.0, 0.8]).cuda())
     assert int(tok[0]) == int(logits[0].argmax()) and int(tok[1]) == op.sample(f64(logits[1]), 0.9, float(np.float32(0.8)))[0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,H,KV,D,act,cache,long", [(400, 4, 2, 64, "f16", "f16", 0), (300, 5, 1, 128, "f32", "bf16", 0),
+                                                     (120, 4, 2, 192, "bf16", "bf16", 600), (90, 2, 2, 256, "f32", "f16", 530)])
+def test_many_short_sequences(cuda, n, H, KV, D, act, cache, long):
+    """More items than CTAs of four warps; one sequence that is split among them."""
+    ctx = [(i * 29) % 70 for i in range(n)]
+    ctx[n // 2] = max(long, 1)
+    check_attention(Batch([1] * n, ctx, H, KV, D, 8, act, cache, seed=n))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,act,cache", [(64, "bf16", "bf16"), (32, "f16", "f16"), (64, "f32", "f16"), (128, "f16", "f16")])
+@pytest.mark.parametrize("ctx", [30, 700])
+def test_a_few_rows_to_a_head(cuda, D, act, cache, ctx):
+    """9 to 16 rows to a sequence and key/value head; masks as well."""
+    b = Batch([6, 5, 2], [ctx, 9, ctx // 2], 6, 2, D, 16, act, cache, seed=D + ctx)
+    check_attention(b)
+    check_attention(b, tree_mask=tree(b.rows, ctx))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,act", [([1, 1, 1], "bf16"), ([40, 70, 1], "bf16"), ([3, 1, 9], "f32")])
+def test_shared_and_repeated_pages(cuda, rows, act):
+    """Sequences that share the pages before their own, and a page that comes twice in one table."""
+    b = Batch(rows, [640, 640, 640], 4, 2, 64, 16, act, "bf16", seed=31)
+    b.pages[1, :40] = b.pages[0, :40]
+    b.pages[2, 3] = b.pages[2, 7]
+    check_attention(b)
+    check_append(b)
+    check_attention(b, tree_mask=tree(b.rows, 5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ci", [2, 3, 10, 13])
+def test_graphs_that_share_a_workspace(cuda, ci):
+    """Two captured graphs (causal and tree) over one workspace, replayed by turns with new queries."""
+    import torch
+    from hetero_infer_b200 import ops
+    b = Batch(*SHAPES[ci], seed=60 + ci)
+    m = tree(b.rows, ci)
+    ws = ops.paged_attention_workspace(b.q, b.kc, b.pages)
+    q = b.q.clone()
+    calls = [lambda **kw: ops.paged_attention(q, b.kc, b.vc, *b.batch(), **kw),
+             lambda **kw: ops.tree_attention(q, b.kc, b.vc, *b.batch(), m, **kw)]
+    graphs = []
+    for call in calls:
+        call(workspace=ws)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = call(workspace=ws)
+        graphs.append((gr, out))
+    for step in range(3):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(step)))
+        for _ in range(2):
+            for gr, _ in graphs:
+                gr.replay()
+        for (gr, out), call in zip(graphs, calls):
+            assert torch.equal(out, call())
+
+
+@pytest.mark.gpu
+def test_outputs_over_inputs_refused(cuda):
+    import torch
+    from hetero_infer_b200 import ops
+    b = Batch([2, 1], [5, 30], 4, 2, 64, 16, "bf16", "bf16")
+    cos, sin = tables(64, 64)
+    q = b.q.contiguous()
+    for call in (lambda out: ops.paged_attention(q, b.kc, b.vc, *b.batch(), out=out),
+                 lambda out: ops.paged_append(q, b.k, b.v, b.kc, b.vc, *b.batch(), cos, sin, out=out)):
+        with pytest.raises(RuntimeError):
+            call(q)
+    both = torch.zeros(5, 4, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError):
+        ops.paged_attention(both[:3], b.kc, b.vc, *b.batch(), out=both[2:])
