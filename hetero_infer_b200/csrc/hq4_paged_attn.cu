@@ -58,7 +58,7 @@ static PaPlan pa_plan(int act_type, int n_rows, int n_heads, int n_kv, int head_
     r.extra = units < 8ll * r.ctas ? 0 : r.tc ? 4 : 18;
     r.join = (int)std::min<long long>(rows, n_rows * group);
     // joining an item of many pieces is a long walk for a warp, and there are few such items; else fewer and larger
-    // CTAs do (a tree of 26 with 2000 entries, 8 items: 18.6 us with 4 rows to a CTA, 24.5 with 16; 16 trees of 64:
+    // CTAs do (a tree of 26 after 1001 entries, 4 heads: 18.6 us with 4 rows to a CTA, 24.5 with 16; 16 trees of 64:
     // 86 and 77)
     r.take = !r.tc ? 1 : items * 4 <= r.ctas ? 4 : 16;
     r.ws = r.split ? (long long)r.ctas * (sizeof(PagedStart) + 2ll * rows * (sizeof(float2) + r.dim * sizeof(float))) : 0;

@@ -19,6 +19,14 @@
 // order), so whoever sees S may touch O.  P is rounded to the cache's type,
 // at most half a step of each probability: the same size as the rounding of
 // the 16-bit output.
+//
+// 4 chunks of 1025 to 2048 tokens after up to 4096, 28 heads of 128: 317 us,
+// 1.04 PFLOP/s.  What bounds it is each group's own chain: a tile's softmax
+// takes its threads about 2000 cycles and the tensor cores 1024 for its two
+// products, and the two groups of an SM cover for one another only in part;
+// then the join of split items, 8 to 20 us.  (Half a tile at a time, with the
+// other half's products under way: 521 us; two threads to a row: slower; the
+// groups sharing the rows and splitting the keys: 391.)
 #pragma once
 #include <algorithm>
 
@@ -29,8 +37,8 @@
 
 namespace hq4 {
 
-// Of 8 pairs of exponentials, those by polynomial (4 prompt chunks of 600 to
-// 7700 tokens: none 328 us, one 322, two 328).
+// Of 8 pairs of exponentials, those by polynomial (4 prompt chunks of 1025
+// to 2048 tokens after up to 4096: none 328 us, one 322, two 328).
 constexpr int kPtSeries = 1;
 constexpr uint64_t kPtWaitNs = 1000000000ull;  // 1 s: a correct kernel never waits this long
 

@@ -9,19 +9,26 @@
 // below the maximum in 2^12 equal steps over the 43.9 octaves that have mass -- a
 // monotone function of the value whose digits, unlike the float's own, split a
 // row evenly.  A first digit's sums are taken in columns of shared memory, one
-// to a thread; the second's, of the few entries that the first leaves, by
+// to a thread or two; the second's, of the entries that the first leaves, by
 // shared-memory atomics; the entries of the last step are compared with one
 // another.  Where top-k keeps few entries, those alone are compared, and all
 // the rest of the work is theirs.
 //
-// Masses are integers of 2^-44 of the maximum's or so, and 0 below that, each good to 2e-9 of itself (see mass()).  Their
-// sums are exact, so the token does not depend on how the work is divided, and
+// What bounds it is neither memory (64 rows of 152064 fp32 are 6 us of it) nor
+// the issue rate, but how few warps an SM has beside the slices: each issues
+// about every fourth cycle (46% of the slots with 8 warps), with a cluster
+// barrier of about 0.8 us between the steps.  64 such rows take 13 us greedy,
+// 42 with top-k 50, 45 without filters and 119 with top-p 0.9; one row 5, 16,
+// 11 and 21.
+//
+// Masses are integers of 2^-44 of the maximum's or so, and 0 below that, each
+// good to 2e-9 of itself (see mass()).  Their sums are exact, so the token does not depend on how the work is divided, and
 // rounding errors of fp32 sums over 1.5e5 entries, 1e-6 of the whole, which
 // would move tokens, do not arise.
 //
 // A thread owns a run of consecutive entries, so its columns above the end that
-// is found add up to what its run contributes to the draw, and only the thread
-// in whose run the draw falls looks at single entries again.
+// is found add up to what its run (or its pair's) contributes to the draw, and
+// only the thread in whose run the draw falls looks at single entries again.
 #include <algorithm>
 
 #include "hq4_host.cuh"
@@ -39,6 +46,12 @@ constexpr int kSrList = 128;             // entries of a CTA that are compared d
 constexpr int kSrFew = 384;              // entries of a row that top-k may leave for that
 constexpr int kSrMaxCluster = 8;
 constexpr int kSrMaxSlice = 36864;       // entries of a CTA
+// Bytes of the first digit's sums, and of the lists that take their place.
+constexpr size_t sr_hist_bytes(int cols, int bits) {
+    const size_t sums = (sizeof(unsigned long long) << bits) * cols;
+    const size_t lists = 3 * sizeof(unsigned long long) * kSrMaxCluster * kSrList;
+    return sums > lists ? sums : lists;
+}
 // Dynamic shared memory at most, by the bits of the first digit (the lists and sums take the rest).
 constexpr size_t sr_smem_max(int bits) { return (bits == 5 ? 204 : 196) * 1024; }
 
@@ -89,14 +102,18 @@ struct SampleRowsShared {
     int bin;
 };
 
-template <class E, int T, int B1>
+// kCols: columns of mass sums, T or T / 2 (two threads to one then, by turns: less shared memory, so that a long
+// row's slice leaves room for 512 threads).
+template <class E, int T, int B1, int kCols>
 struct SampleRow {
     typedef SampleRowsShared<T, B1> Shared;
     static constexpr int kBins1 = Shared::kBins1, kBins2 = Shared::kBins2, kB2 = kSrBits - B1;
+    static constexpr bool kPairs = kCols < T;
+    static_assert(kCols == T || kCols == T / 2, "a thread or two to a column");
     Shared& sh;
-    u64* hist;         // [kBins1][T]; once a search is at its list, that list
+    u64* hist;         // [kBins1][kCols]; once a search is at its list, that list
     const E* xs;       // this CTA's slice
-    int lo, a, b;      // its first entry in the row; the thread's run in it
+    int lo, a, b, run; // its first entry in the row; the thread's run in it, and a run's entries
     int rank, nr, turn, pturn;
     float top, steps;  // the maximum; steps of the search's keys for a unit of x
     float oct, oct_lo; // octaves for a unit of x, as a sum of two
@@ -218,6 +235,53 @@ struct SampleRow {
         }
     }
 
+    // Which entries of the run `pick` chooses, a bit each; and use(x, w, i) of
+    // those, four at a time.  A warp's lanes then spend their masses on chosen
+    // entries alone, where masses() works them out for all six whenever any
+    // lane has chosen one.
+    struct Chosen {
+        u64 bits[3];
+    };
+    static_assert((kSrMaxSlice + 255) / 256 + 1 <= 192, "the bits hold a run");
+    template <class Pick>
+    __device__ __forceinline__ Chosen choose(Pick pick) const {
+        Chosen c;
+#pragma unroll
+        for (int w = 0; w < 6; w++) {
+            uint32_t m = 0;
+            const int i0 = a + 32 * w, n = min(32, b - i0);
+            for (int t = 0; t < n; t += 4)
+#pragma unroll
+                for (int j = 0; j < 4; j++) m |= (uint32_t)pick(t + j < n ? at(i0 + t + j) : -INFINITY) << (t + j);
+            if (w & 1) c.bits[w / 2] |= (u64)m << 32;
+            else c.bits[w / 2] = m;
+        }
+        return c;
+    }
+    template <class Use>
+    __device__ __forceinline__ void masses_of(const Chosen& c, bool counting, Use use) const {
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+            for (u64 m = c.bits[k]; m;) {
+                int i[4];
+                float x[4];
+                bool on[4];
+                u64 w[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    on[j] = m != 0;
+                    i[j] = a + 64 * k + (on[j] ? __ffsll(m) - 1 : 0);
+                    m &= m - 1;  // (0 stays 0)
+                    x[j] = at(i[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[j] = counting ? 1 : mass(x[j]);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (on[j]) use(x[j], w[j], i[j]);
+            }
+    }
+
     // The bin among n (the cluster's sums in all[r][.]) that is the last to
     // begin below the target, with what lies before it and in it; `base` is
     // what lies before the first.  Thread i < n looks after bin i.
@@ -248,7 +312,7 @@ struct SampleRow {
     struct End {
         float v;        // the value, once it is known
         u64 above;      // what the entries above it weigh (each its mass, or one)
-        u64 mine;       // mass of the thread's run above the value's step
+        u64 mine;       // mass above the value's step: (a pair's: of both runs)
         int step;       // that step
         int i0, i1;     // the entries of the run in that step lie in [i0, i1)
         bool listed;    // not resolved: the list holds all entries down to that step,
@@ -261,17 +325,52 @@ struct SampleRow {
     __device__ End find_end(bool counting, u64 count, double share, u64 whole, float floor) {
         End e = {};
         // first digit
+        const bool odd = threadIdx.x & 1;  // (of a pair)
+        uint32_t* const counts = reinterpret_cast<uint32_t*>(hist) + threadIdx.x;  // a column to every thread
+        u64* const sums = hist + (kPairs ? threadIdx.x >> 1 : threadIdx.x);
+        auto bin_of = [&](float x) { return (int)key(x) >> kB2; };
+        auto in = [&](float x) { return has_mass(x) && x >= floor; };
+        if (counting) {
 #pragma unroll
-        for (int i = 0; i < kBins1; i++) hist[i * T + threadIdx.x] = 0;
-        masses(counting, [&](float x) { return has_mass(x) && x >= floor; },
-               [&](float x, u64 w, int) { hist[((int)key(x) >> kB2) * T + threadIdx.x] += w; });
+            for (int i = 0; i < kBins1; i++) counts[i * T] = 0;
+            masses(true, in, [&](float x, u64, int) { counts[bin_of(x) * T]++; });
+        } else {
+            if (!kPairs || !odd)
+#pragma unroll
+                for (int i = 0; i < kBins1; i++) sums[i * kCols] = 0;
+            if constexpr (!kPairs) {
+                masses(false, in, [&](float x, u64 w, int) { sums[bin_of(x) * kCols] += w; });
+            } else {
+                for (int i = 0; i < run; i += 6) {  // (all lanes alike)
+                    float x[6];
+                    u64 w[6];
+#pragma unroll
+                    for (int j = 0; j < 6; j++) {
+                        x[j] = a + i + j < b ? at(a + i + j) : -INFINITY;
+                        w[j] = mass(x[j]);
+                    }
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        __syncwarp();
+                        if (odd == (half == 1))
+#pragma unroll
+                            for (int j = 0; j < 6; j++)
+                                if (in(x[j])) sums[bin_of(x[j]) * kCols] += w[j];
+                    }
+                }
+            }
+        }
         for (int i = threadIdx.x; i < 3 * kBins2; i += T) sh.part[0][i] = 0;
         __syncthreads();
         const int lane = threadIdx.x & 31;
         for (int i = threadIdx.x >> 5; i < kBins1; i += T / 32) {
             u64 v = 0;
+            if (counting)
 #pragma unroll
-            for (int j = 0; j < T / 32; j++) v += hist[i * T + j * 32 + lane];
+                for (int j = 0; j < T / 32; j++) v += reinterpret_cast<uint32_t*>(hist)[i * T + j * 32 + lane];
+            else
+#pragma unroll
+                for (int j = 0; j < kCols / 32; j++) v += hist[i * kCols + j * 32 + lane];
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
             if (lane < nr) st_cluster_u64(map_to_rank(smem_u32(&sh.all1[turn][rank][i]), lane), v);
@@ -290,16 +389,18 @@ struct SampleRow {
         }
         const int bin1 = find_bin<kBins1>(sh.all1[turn], 0, target, before, here);
         turn ^= 1;
-        if (!counting)
-            for (int i = 0; i < bin1; i++) e.mine += hist[i * T + threadIdx.x];
+        if (!counting && (!kPairs || !odd))
+            for (int i = 0; i < bin1; i++) e.mine += sums[i * kCols];
         // second digit, of the entries that have the first
         const float k_lo = (float)(bin1 << kB2), k_hi = (float)((bin1 + 1) << kB2);
-        masses(counting,
-               [&](float x) {
-                   const float k = key(x);
-                   return k >= k_lo && k < k_hi && x >= floor;
-               },
+        const bool all_few = counting && before + here <= kSrFew;  // all down to that digit are few: they are chosen
+        const Chosen chosen = choose([&](float x) {
+            const float k = key(x);
+            return (all_few || k >= k_lo) && k < k_hi && x >= floor;
+        });
+        masses_of(chosen, counting,
                [&](float x, u64 w, int) {
+                   if (all_few && key(x) < k_lo) return;
                    const int i = (int)key(x) & (kBins2 - 1);
                    atomicAdd(&sh.part[0][i], (uint32_t)w & 0x7fffu);
                    if (!counting) {
@@ -324,25 +425,23 @@ struct SampleRow {
         // the entries of the last step; or, where top-k ends early, all down to it
         const bool few = counting && before + here <= kSrFew;
         e.i0 = e.i1 = 0;
-        const float k_from = few ? 0.0f : counting ? (float)e.step : k_lo, k_end = (float)(e.step + 1);
-        masses(counting,
-               [&](float x) {
-                   const float k = key(x);
-                   return k >= k_from && k < k_end && x >= floor;
-               },
-               [&](float x, u64 w, int i) {
-                   if (!few && (int)key(x) < e.step) {
-                       e.mine += w;
-                       return;
-                   }
-                   if (e.i1 == 0) e.i0 = i;
-                   e.i1 = i + 1;
-                   const uint32_t place = atomicAdd(&sh.n_list, 1);
-                   if (place < kSrList) {
-                       sh.key[rank][place] = order_bits(x + 0.0f);  // -0 counts as 0
-                       sh.idx[rank][place] = lo + i;
-                   }
-               });
+        const float k_end = (float)(e.step + 1);
+        auto take = [&](float x, u64 w, int i) {
+            if (!(key(x) < k_end)) return;
+            if (!few && (int)key(x) < e.step) {
+                e.mine += w;
+                return;
+            }
+            if (e.i1 == 0) e.i0 = i;
+            e.i1 = i + 1;
+            const uint32_t place = atomicAdd(&sh.n_list, 1);
+            if (place < kSrList) {
+                sh.key[rank][place] = order_bits(x + 0.0f);  // -0 counts as 0
+                sh.idx[rank][place] = lo + i;
+            }
+        };
+        if (few && !all_few) masses(true, [&](float x) { return key(x) < k_end && x >= floor; }, take);
+        else masses_of(chosen, counting, take);
         if (counting) e.mine = 0;
         __syncthreads();
         const uint32_t n_mine = sh.n_list;
@@ -447,8 +546,8 @@ __device__ __forceinline__ float log_prob(float x, const Row& s, double oct, u64
     return (float)(-((double)s.top - (double)x) * oct * 0.6931471805599453094 - log((double)total / (double)s.mass(s.top)));
 }
 
-template <class E, int T, int B1>
-__global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p) {
+template <class E, int T, int B1, int kCols>
+__global__ void __launch_bounds__(T, 512 / T) sample_rows_kernel(const SampleRowsParams p) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ SampleRowsShared<T, B1> sh;
     pdl_launch_dependents();
@@ -460,7 +559,7 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
     const E* src = static_cast<const E*>(p.x) + (long long)row * p.stride + lo;
     constexpr int kV = 16 / sizeof(E);
     const int off = (int)((uintptr_t)src & 15) / (int)sizeof(E);  // the slice keeps the row's alignment
-    E* xs = reinterpret_cast<E*>(smem + sizeof(u64) * (1 << B1) * T) + off;
+    E* xs = reinterpret_cast<E*>(smem + sr_hist_bytes(kCols, B1)) + off;
 
     // ---- the slice, all copies in flight at once ---------------------------------
     const int head = min(cnt, (kV - off) % kV), vecs = (cnt - head) / kV;
@@ -478,7 +577,7 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
 
     // ---- its largest entry, the first of its equals; NaN ---------------------------
     const int run = ((cnt + T - 1) / T) | 1;  // entries of a thread: odd, which spreads a warp over the banks
-    SampleRow<E, T, B1> s{sh, reinterpret_cast<u64*>(smem), xs, lo, min(cnt, (int)threadIdx.x * run), 0, rank, nr,
+    SampleRow<E, T, B1, kCols> s{sh, reinterpret_cast<u64*>(smem), xs, lo, min(cnt, (int)threadIdx.x * run), 0, run, rank, nr,
                           0, 0, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0};
     s.b = min(cnt, s.a + run);
     uint32_t best = 0, first = 0x7fffffffu;  // order bits (of a NaN: all ones), index in the row
@@ -539,7 +638,7 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
     float floor = -INFINITY;  // entries below are out
     int ties = 0x7fffffff;    // of the entries equal to tie, how many stay
     float tie = 0.0f;
-    typename SampleRow<E, T, B1>::End e = {};
+    typename SampleRow<E, T, B1, kCols>::End e = {};
     bool summed = false;      // e.mine holds the thread's mass above e.step
     const float p_end = min_p > 0.0f ? min_p_end(min_p, top, oct) : -INFINITY;
     if (top_k > 0 && top_k < p.n) {
@@ -639,6 +738,12 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
             const float x = s.at(i);
             if (s.has_mass(x) && (int)s.key(x) == e.step && stays(x)) mine += s.mass(x);
         }
+        if constexpr (kCols < T) {  // a column is two threads': the first draws for both runs
+            const u64 other = __shfl_xor_sync(0xffffffffu, mine, 1);
+            const int end = __shfl_xor_sync(0xffffffffu, s.b, 1);
+            mine = threadIdx.x & 1 ? 0 : mine + other;
+            if (!(threadIdx.x & 1)) s.b = end;
+        }
     }
     u64 lower;
     const u64 total = s.cluster_sum(mine, &lower);
@@ -658,9 +763,9 @@ __global__ void __launch_bounds__(T) sample_rows_kernel(const SampleRowsParams p
     }
 }
 
-template <class E, int T, int B1>
+template <class E, int T, int B1, int kCols>
 static int launch_sample_rows(const SampleRowsParams& p, int rows, int cluster, size_t smem, cudaStream_t st) {
-    auto kern = sample_rows_kernel<E, T, B1>;
+    auto kern = sample_rows_kernel<E, T, B1, kCols>;
     static PerDeviceOnce once;
     if (smem_opt_in(once, kern, (int)sr_smem_max(B1)) != cudaSuccess) return HQ4_ERR_LAUNCH;
     cudaLaunchAttribute attr[2];
@@ -680,27 +785,36 @@ static int launch_sample_rows(const SampleRowsParams& p, int rows, int cluster, 
     return cudaLaunchKernelEx(&lc, kern, p) == cudaSuccess ? HQ4_OK : HQ4_ERR_LAUNCH;
 }
 
-// How a row is divided: CTAs, their threads, bits of the first digit.
+// How a row is divided: CTAs, their threads, bits of the first digit, columns
+// of its mass sums.  A wave of rows costs its entries, at a rate that grows
+// with an SM's warps (two CTAs also fill each other's barriers), and barriers
+// and fixed steps.  Measured with top-p 0.9 (top-k 50): 1 row of 152064 fp32,
+// 8 CTAs of 512 threads 20.5 us (15.8), 4 of 512 39 (19), 4 of 256 59; 64 such
+// rows, 4 CTAs of 512 with a column to two threads 117 (42), 4 of 256 150 (56),
+// 8 of 512 with one each 117 (74); 256 rows of 32003 bf16, 2 CTAs of 256 63
+// (38), 1 of 512 66 (37), 4 of 256 97.
 struct SrShape {
-    int cluster, threads, bits;
+    int cluster, threads, bits, cols;
     size_t smem;
 };
 
 template <class E>
 static int sample_rows(SampleRowsParams p, int rows, int sms, cudaStream_t st) {
-    SrShape best = {0, 0, 0, 0};
+    SrShape best = {0, 0, 0, 0, 0};
     double best_cost = 0.0;
     for (int cluster = kSrMaxCluster; cluster >= 1; cluster >>= 1) {
         if (cluster > 1 && p.n / cluster < 2048) continue;
-        for (int small = 0; small < 2; small++) {
-            SrShape s = {cluster, small ? 256 : 512, small ? 4 : 5, 0};
-            s.smem = (size_t)((p.n + cluster - 1) / cluster + 16) * sizeof(E) + (sizeof(u64) << s.bits) * s.threads;
+        static const SrShape shapes[3] = {{0, 512, 5, 512, 0}, {0, 512, 4, 256, 0}, {0, 256, 4, 256, 0}};
+        for (SrShape s : shapes) {
+            s.cluster = cluster;
+            s.smem = (size_t)((p.n + cluster - 1) / cluster + 16) * sizeof(E) + sr_hist_bytes(s.cols, s.bits);
             if (s.smem > sr_smem_max(s.bits)) continue;
-            const int per_sm = std::min<int>(small ? 4 : 2, (int)((size_t)227 * 1024 / (s.smem + 24 * 1024)));
-            const int at_once = std::max(1, sms * std::max(1, per_sm) / cluster);
+            const int per_sm = std::max(1, std::min<int>(512 / s.threads, (int)((size_t)227 * 1024 / (s.smem + 32 * 1024))));
+            const int at_once = std::max(1, sms * per_sm / cluster);
             const int waves = (rows + at_once - 1) / at_once;
-            const int sharing = std::min(std::max(1, per_sm), (rows * cluster + sms - 1) / sms);  // CTAs of an SM
-            const double cost = waves * ((double)p.n / cluster / 512.0 * std::max(1.0, sharing * s.threads / 512.0) + 40.0 + 4.0 * cluster);
+            const int sharing = std::min(per_sm, (rows * cluster + sms - 1) / sms);  // CTAs of an SM
+            const double rate = sharing > 1 ? 1.8 : s.threads > 256 ? 1.6 : 1.0;
+            const double cost = waves * ((double)p.n / cluster / 512.0 * sharing / rate + 20.0 + 2.0 * cluster);
             if (!best.cluster || cost < best_cost) {
                 best_cost = cost;
                 best = s;
@@ -709,8 +823,9 @@ static int sample_rows(SampleRowsParams p, int rows, int sms, cudaStream_t st) {
     }
     if (!best.cluster) return HQ4_ERR_SHAPE;
     p.chunk = (p.n + best.cluster - 1) / best.cluster;
-    return best.threads == 512 ? launch_sample_rows<E, 512, 5>(p, rows, best.cluster, best.smem, st)
-                               : launch_sample_rows<E, 256, 4>(p, rows, best.cluster, best.smem, st);
+    return best.bits == 5      ? launch_sample_rows<E, 512, 5, 512>(p, rows, best.cluster, best.smem, st)
+         : best.threads == 512 ? launch_sample_rows<E, 512, 4, 256>(p, rows, best.cluster, best.smem, st)
+                               : launch_sample_rows<E, 256, 4, 256>(p, rows, best.cluster, best.smem, st);
 }
 
 }  // namespace hq4

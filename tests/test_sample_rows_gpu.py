@@ -225,3 +225,17 @@ def test_refusals(cuda):
         with pytest.raises(RuntimeError):
             ops.sample_rows(*a, **kw)
     assert ops.sample_rows(x[:0], u[:0]).shape == (0,)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n,kind", [(40, 150001, "f32"), (33, 100000, "bf16"), (150, 40003, "f16")])
+def test_many_long_rows(cuda, rows, n, kind):
+    """Rows enough to fill the device, so that each has few CTAs and long slices."""
+    import torch
+    dt = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[kind]
+    rng = np.random.default_rng(n)
+    t = rng.choice([0.0, 0.6, 1.0, 1.7], rows)
+    k = rng.choice([0, 0, 1, 60, 1000, 50000], rows)
+    p = rng.choice([1.0, 0.9, 0.99, 0.5], rows)
+    m = rng.choice([0.0, 0.0, 0.02], rows)
+    check(logits(rng, rows, n), rng.random(rows), dt, temperature=t, top_k=k, top_p=p, min_p=m)
