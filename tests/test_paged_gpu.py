@@ -700,3 +700,21 @@ def test_outputs_over_inputs_refused(cuda):
     both = torch.zeros(5, 4, 64, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(RuntimeError):
         ops.paged_attention(both[:3], b.kc, b.vc, *b.batch(), out=both[2:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,KV,D,act,cache", [(300, 1, 32, "bf16", "bf16"), (40, 1, 64, "f32", "f16"), (66, 2, 256, "f16", "f16")])
+def test_many_heads_to_one(cuda, H, KV, D, act, cache):
+    """More query heads to a key/value head than a tile has rows."""
+    b = Batch([1, 2, 1], [20, 700, 0], H, KV, D, 8, act, cache, seed=H)
+    check_attention(b)
+    check_append(b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [256, 4096])
+@pytest.mark.parametrize("rows,act", [([3, 60], "bf16"), ([1, 1], "f32")])
+def test_large_pages(cuda, page, rows, act):
+    b = Batch(rows, [100, 900], 4, 2, 64, page, act, "bf16", seed=page)
+    check_attention(b)
+    check_append(b)
