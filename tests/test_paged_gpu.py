@@ -718,3 +718,22 @@ def test_large_pages(cuda, page, rows, act):
     b = Batch(rows, [100, 900], 4, 2, 64, page, act, "bf16", seed=page)
     check_attention(b)
     check_append(b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,act,cache", [([2, 1], "bf16", "bf16"), ([70, 9], "f16", "f16"), ([1, 4], "f32", "f16")])
+def test_outputs_beside_inputs(cuda, rows, act, cache):
+    """An output that begins where q's rows end, and one that ends where they begin."""
+    import torch
+    from hetero_infer_b200 import ops
+    b = Batch(rows, [600, 30], 4, 2, 64, 16, act, cache, seed=77)
+    want = ops.paged_attention(b.q, b.kc, b.vc, *b.batch())
+    cos, sin = tables(700, 64)
+    turned = ops.paged_append(b.q, b.k, b.v, b.kc.clone(), b.vc.clone(), *b.batch(), cos, sin)
+    for first in (0, 1):
+        both = torch.full((2 * b.n, 4, 64), 77.0, dtype=b.q.dtype, device="cuda")
+        q, out = both[first * b.n:][:b.n], both[(1 - first) * b.n:][:b.n]
+        q.copy_(b.q)
+        assert torch.equal(ops.paged_attention(q, b.kc, b.vc, *b.batch(), out=out), want)
+        assert torch.equal(ops.paged_append(q, b.k, b.v, b.kc.clone(), b.vc.clone(), *b.batch(), cos, sin, out=out), turned)
+        assert torch.equal(q, b.q)
