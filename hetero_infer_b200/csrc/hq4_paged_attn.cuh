@@ -243,13 +243,15 @@ __device__ __forceinline__ bool paged_sees(const PagedAttnParams& p, const Paged
 // One output row, entry by entry (one warp).  The tiled kernels multiply
 // masked probabilities of zero by values that they do not look at; where such
 // a value is an infinity or a NaN, the row comes out as NaN and is computed
-// here again, from the entries that it sees alone.
+// here again, from the entries that it sees alone.  So is a row whose sum is 0:
+// one that sees nothing is zeros, one whose scores are all -inf is NaN (0 / 0).
 template <class A, class C>
 __device__ __noinline__ void paged_slow_row(const PagedAttnParams& p, const PagedItem& it, int r) {
     const int lane = threadIdx.x & 31, D = p.head_dim;
     const int tok = r / p.group, head = it.h * p.group + r % p.group;
     const A* q = static_cast<const A*>(p.q) + (long long)(it.row0 + tok) * p.q_stride + (long long)head * D;
     float qv[8], acc[8], m = -INFINITY, l = 0.0f;
+    bool any = false;
     const int nd = D >> 5;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
@@ -271,9 +273,10 @@ __device__ __noinline__ void paged_slow_row(const PagedAttnParams& p, const Page
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
         z *= p.scale_log2;
-        const float m1 = (z > m || z != z) ? z : m;
-        const float keep = m == m1 ? 1.0f : exp2f(m - m1), w = exp2f(z - m1);
+        const float m1 = (z > m || z != z) ? z : m, mu = m1 == -INFINITY ? 0.0f : m1;  // (scores of -inf alone so far)
+        const float keep = m == m1 ? 1.0f : exp2f(m - mu), w = exp2f(z - mu);
         m = m1;
+        any = true;
         l = l * keep + w;
 #pragma unroll
         for (int i = 0; i < 8; i++)
@@ -282,7 +285,7 @@ __device__ __noinline__ void paged_slow_row(const PagedAttnParams& p, const Page
     A* out = static_cast<A*>(p.out) + ((long long)(it.row0 + tok) * p.n_heads + head) * D;
 #pragma unroll
     for (int i = 0; i < 8; i++)
-        if (i < nd) out[lane + 32 * i] = Elem<A>::from(l == 0.0f ? 0.0f : acc[i] / l);
+        if (i < nd) out[lane + 32 * i] = Elem<A>::from(any ? acc[i] / l : 0.0f);
 }
 
 // The pieces of split items in the workspace: CTA c's first piece is 2c, its
@@ -407,7 +410,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
         const int row = it.rt * kRows + r, tok = row / p.group, head = it.h * p.group + row % p.group;
         A* out = static_cast<A*>(p.out) + ((long long)(it.row0 + tok) * p.n_heads + head) * D;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        bool bad = false;
+        bool bad = l == 0.0f;
 #pragma unroll
         for (int j = 0; j < kPer; j++)
             if (lane * 4 + 128 * j < D) {

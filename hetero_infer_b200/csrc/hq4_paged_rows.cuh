@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(W * 32) paged_attn_kernel(const __grid_constan
                 for (int i = 0; i < W; i++) w[i] = ll == 0.0f ? 0.0f : w[i] / ll;
             A* out = static_cast<A*>(p.out) + ((long long)(it.row0 + row / p.group) * p.n_heads + it.h * p.group + row % p.group) * D;
             float* part = ws.o + ((size_t)piece * kRows + r) * kDim;
-            bool bad = false;
+            bool bad = ll == 0.0f;
             for (int d = lane; d < D; d += 32) {
                 float y = 0.0f;
 #pragma unroll

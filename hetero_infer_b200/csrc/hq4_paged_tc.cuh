@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                 C* out = static_cast<C*>(p.out) +
                          ((long long)(mine->row0 + tok) * p.n_heads + mine->h * p.group + row % p.group) * D;
                 const size_t at = (size_t)piece_no * kRows + r;
-                bool bad = false;
+                bool bad = on && whole && l == 0.0f;
                 for (int c = 0; c < D; c += 32) {
                     uint32_t o[32];
                     tmem_ld32(o_col + c, o);

@@ -327,7 +327,8 @@ int hq4_paged_append(const void* q, const void* k, const void* v, int act_type, 
 /* Grouped-query attention of the batch's rows over the cache: row i of
  * sequence s attends to entries [0, lens[s] + i], its own among them
  * (hq4_paged_append first).  out [n_rows][n_heads][head_dim] must not overlap
- * q; a row that sees nothing is zeros.  What lies in entries that a row does
+ * q; a row that sees nothing is zeros (one whose scores are all -inf is NaN).
+ * What lies in entries that a row does
  * not see (stale pages, NaN, infinities) does not reach it.  The workspace
  * (hq4_paged_attention_workspace_bytes, 128-byte aligned; may be NULL where
  * that is 0) is written and read by one call: calls that can run at the same

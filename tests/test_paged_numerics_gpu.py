@@ -1,0 +1,65 @@
+"""Attention over a paged cache where the numbers are not ordinary: keys and
+queries that are not finite, scores far apart, lengths at the ends of their type.
+
+Tolerances are those of test_paged_gpu.py; what a test adds is derived in it.
+"""
+import numpy as np
+import pytest
+
+from oracle import paged as op
+from tests.test_paged_gpu import U, Batch, compare_attention, f64, tree
+
+
+def widen(b, entries):
+    """More columns of pages than any sequence needs: so many entries may be, and the work is split."""
+    import torch
+    more = -(-entries // b.page) - b.pages.shape[1]
+    b.pages = torch.cat((b.pages, torch.full((len(b.rows), more), -1, dtype=torch.int32, device="cuda")), 1).contiguous()
+
+
+def compare_nonfinite(b, got, m=None):
+    """The same values are finite as by the definition, and those are right."""
+    with np.errstate(all="ignore"):
+        want, size, _ = op.attention(f64(b.q), f64(b.kc), f64(b.vc), *b.host(), b.D ** -0.5, m)
+    score = op.attention(np.nan_to_num(f64(b.q), posinf=0, neginf=0), np.nan_to_num(f64(b.kc), posinf=0, neginf=0), f64(b.vc),
+                         *b.host(), b.D ** -0.5, m)[2]
+    g = f64(got)
+    wrong = np.argwhere((np.isfinite(g) != np.isfinite(want)).any(-1))
+    assert not len(wrong), f"(row, head) {wrong[:8].tolist()}"
+    compare_attention(b, np.nan_to_num(g), np.nan_to_num(want), np.nan_to_num(size), score)
+
+
+# rows of each of 32 sequences: the warp-level kernel, the tcgen05 kernel
+KERNELS = [(1, 64, "bf16", "bf16"), (1, 128, "f16", "f16"), (2, 64, "f32", "f16"), (1, 128, "f32", "bf16"),
+           (10, 64, "bf16", "bf16"), (10, 64, "f16", "f16"), (7, 128, "bf16", "bf16"), (7, 128, "f16", "f16"),
+           (6, 192, "f16", "f16")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("rows,D,act,cache", KERNELS)
+def test_scores_that_are_all_minus_infinity(cuda, rows, D, act, cache, split):
+    """A row whose entries all score -inf has no distribution: NaN.  Behind such
+    entries at its beginning, an entry that scores more has all the mass, also
+    where an unseen value is NaN and the row is computed entry by entry."""
+    from hetero_infer_b200 import ops
+    n = max(rows, 3)
+    b = Batch([n] * 4, [0, 1, 2, 30], 4, 2, D, 16, act, cache, seed=D + 1)
+    if split:
+        widen(b, 1100)
+    b.q[:, :, 3] = 1.0 + b.q[:, :, 3].abs()
+    host = b.pages.cpu().numpy()
+    for s in range(4):
+        for e in range(2):
+            page, at = op.place(host, b.n_pages, b.page, s, e)
+            b.kc[page, :, at, 3] = -float("inf")
+    compare_nonfinite(b, ops.paged_attention(b.q, b.kc, b.vc, *b.batch()))
+    m = tree(b.rows, 2)
+    for s in range(4):  # the first sequence's node 2 sees itself alone; the last node is NaN and seen by none
+        m[s * n:(s + 1) * n, 0] &= ~(1 << n - 1)
+        page, at = op.place(host, b.n_pages, b.page, s, b.ctx[s] + n - 1)
+        b.vc[page, :, at] = float("nan")
+    with np.errstate(all="ignore"):
+        got = ops.tree_attention(b.q, b.kc, b.vc, *b.batch(), m)
+        b.vc.nan_to_num_(0.0)
+        compare_nonfinite(b, got, m.cpu().numpy().astype(np.int64) & 0xFFFFFFFF)
