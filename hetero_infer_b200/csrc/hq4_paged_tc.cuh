@@ -150,6 +150,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN where either is (fmaxf drops it)
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 __device__ __forceinline__ u64 pt_ex2_both(u64 z) {
     const float2 f = unpair(z);
     return pair(pt_ex2(f.x), pt_ex2(f.y));
@@ -159,11 +164,12 @@ __device__ __forceinline__ u64 pt_ex2_both(u64 z) {
 // [-1/2, 1/2] is a polynomial (least relative error, fitted for this: 7.5e-5 for
 // bf16 probabilities, whose half step is 2e-3, 2.6e-6 for fp16 ones), and the
 // factor 2^n is built from its bits: 0 for n = -127, which is what -inf gives.
+// NaN stays NaN (the polynomial's; a NaN or infinite key that a row sees).
 template <class C>
 __device__ __forceinline__ u64 pt_ex2_series(u64 z) {
     const u64 magic = pair(12582912.0f, 12582912.0f), back = pair(-12582912.0f, -12582912.0f);
     float2 v = unpair(z);
-    z = pair(fmaxf(v.x, -127.0f), fmaxf(v.y, -127.0f));
+    z = pair(max_nan(v.x, -127.0f), max_nan(v.y, -127.0f));
     const u64 r = add2(z, magic);
     const u64 f = fma2(add2(r, back), pair(-1.0f, -1.0f), z);
     u64 s;

@@ -37,6 +37,38 @@ KERNELS = [(1, 64, "bf16", "bf16"), (1, 128, "f16", "f16"), (2, 64, "f32", "f16"
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("rows,D,act,cache", KERNELS)
+def test_keys_that_are_not_finite(cuda, rows, D, act, cache, bad, split):
+    """One value of one key that every row sees, at each place of a tile (a sequence each); the values are finite."""
+    from hetero_infer_b200 import ops
+    b = Batch([rows] * 32, [40 + 3 * s for s in range(32)], 4, 2, D, 16, act, cache, seed=D + rows)
+    if split:
+        widen(b, 1100)
+    for s in range(32):
+        page, at = op.place(b.pages.cpu().numpy(), b.n_pages, b.page, s, s)
+        b.kc[page, :, at, 3] = bad
+    compare_nonfinite(b, ops.paged_attention(b.q, b.kc, b.vc, *b.batch()))
+    m = tree(b.rows, 7)
+    compare_nonfinite(b, ops.tree_attention(b.q, b.kc, b.vc, *b.batch(), m), m.cpu().numpy().astype(np.int64) & 0xFFFFFFFF)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,D,act,cache", KERNELS)
+def test_queries_that_are_not_finite(cuda, rows, D, act, cache):
+    """A NaN in the first row of a prompt, which sees one entry: that row alone, one head of it."""
+    from hetero_infer_b200 import ops
+    b = Batch([rows] * 3, [0, 1, 2], 4, 2, D, 16, act, cache, seed=D)
+    for s in range(3):
+        b.q[s * rows, 1, 5] = float("nan")
+    got = ops.paged_attention(b.q, b.kc, b.vc, *b.batch())
+    compare_nonfinite(b, got)
+    bad = ~np.isfinite(f64(got)).all(-1)
+    assert bad.sum() == 3 and bad[::rows, 1].all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [False, True])
 @pytest.mark.parametrize("rows,D,act,cache", KERNELS)
 def test_scores_that_are_all_minus_infinity(cuda, rows, D, act, cache, split):
     """A row whose entries all score -inf has no distribution: NaN.  Behind such
