@@ -330,15 +330,16 @@ __global__ void __launch_bounds__(W * 32) paged_attn_kernel(const __grid_constan
                         for (int i = 0; i < 4; i++) acc[d][n][i] *= keep[n][i & 1];
                 }
             }
-            // the probabilities as 16-bit terms (of fp16: scaled by 2^14, which the epilogue takes back, so that
-            // those of 2^-28 of the largest are still normal numbers), transposed
+            // the probabilities as 16-bit terms, transposed (of fp16: scaled by 2^14, which the epilogue takes back,
+            // so that those of 2^-28 of the largest are still normal numbers: unscaled, 10^5 entries 25 octaves
+            // below one would add to the sum and nothing to the output)
             uint32_t pb[NT][kTerms][2];
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int hh = 0; hh < 2; hh++) {
                     float a = sc[n][2 * hh], b = sc[n][2 * hh + 1];
-                    if constexpr (kTerms == 2) {
+                    if constexpr (Elem<C>::code == HQ4_F16) {
                         a *= 16384.0f;
                         b *= 16384.0f;
                     }
@@ -372,7 +373,7 @@ __global__ void __launch_bounds__(W * 32) paged_attn_kernel(const __grid_constan
             if (++stage == kStages) stage = 0;
         }
         // ---- the next item's first tiles; the warps' results, joined ----------
-        const float back = kTerms == 2 ? 1.0f / 16384.0f : 1.0f;
+        const float back = Elem<C>::code == HQ4_F16 ? 1.0f / 16384.0f : 1.0f;
         __syncwarp();  // the ring is the warp's own: its lanes have read their last tile
         int os_at = warp * kRing;
         if constexpr (kAhead) {

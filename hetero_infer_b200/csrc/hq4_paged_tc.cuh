@@ -16,9 +16,11 @@
 // The running maximum m only follows a row's true maximum when that passes it
 // by 2^8, so O is rarely rescaled; P stays below 2^8 and the sums are fp32.
 // P V is complete when S of the next tile is (matrix instructions complete in
-// order), so whoever sees S may touch O.  P is rounded to the cache's type,
-// at most half a step of each probability: the same size as the rounding of
-// the 16-bit output.
+// order), so whoever sees S may touch O.  P is rounded to the cache's type, at
+// most half a step of each probability: the same size as the rounding of the
+// 16-bit output.  fp16 has few steps below 1, so its P (and the sums with it)
+// are scaled by 2^7, to at most 2^15: a probability is a normal number down to
+// 2^-21 of 2^m, and below that off by at most 2^-32 of it.
 //
 // 4 chunks of 1025 to 2048 tokens after up to 4096, 28 heads of 128: 317 us,
 // 1.04 PFLOP/s.  What bounds it is each group's own chain: a tile's softmax
@@ -421,7 +423,8 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                             }
                         }
                         const float mu = m == -INFINITY ? 0.0f : m;
-                        const u64 cc = pair(c2, c2), mm = pair(-mu, -mu);
+                        constexpr float kUp = Elem<C>::code == HQ4_F16 ? 7.0f : 0.0f;
+                        const u64 cc = pair(c2, c2), mm = pair(kUp - mu, kUp - mu);
                         u64 add[2] = {0, 0};
 #pragma unroll
                         for (int i = 0; i < kParts; i++) {

@@ -95,3 +95,46 @@ def test_scores_that_are_all_minus_infinity(cuda, rows, D, act, cache, split):
         got = ops.tree_attention(b.q, b.kc, b.vc, *b.batch(), m)
         b.vc.nan_to_num_(0.0)
         compare_nonfinite(b, got, m.cpu().numpy().astype(np.int64) & 0xFFFFFFFF)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("weight", [0.49, 1.49, 30.0])
+@pytest.mark.parametrize("seqs,H,rows,D", [(600, 1, 1, 64), (600, 7, 1, 128), (300, 8, 4, 64), (300, 8, 4, 128), (200, 4, 5, 256)])
+def test_one_strong_entry_and_many_weak_ones(cuda, seqs, H, rows, D, weight):
+    """fp16: 400000 entries of `weight` 2^-24 of one entry's mass each, seen by
+    so many sequences that a CTA walks all of them for one (a part of them that
+    is walked by itself has a maximum of its own).
+
+    A probability is rounded by 2^-11 of itself, or by half of fp16's smallest
+    step, 2^-25 of a scaled value: 2^-32 of the largest, and the maximum that it
+    is relative to may lag it by 2^8, which makes that less.  The matrix unit cuts
+    a sum of 16 entries off below 2^-23 of the running one; of the warp-level
+    kernel's four warps each has a quarter of them."""
+    import torch
+    from hetero_infer_b200 import ops
+    n, page = 400000, 64
+    b = Batch([rows] * seqs, [3] * seqs, H, 1, D, page, "f16", "f16")
+    per = -(-(n + rows) // page)
+    b.lens.fill_(n)
+    b.pages = torch.arange(per, dtype=torch.int32, device="cuda")[None].expand(seqs, per).contiguous()
+    g = torch.Generator(device="cuda").manual_seed(H)
+    b.kc = torch.zeros(per, 1, page, D, dtype=torch.float16, device="cuda")
+    b.vc = -1 - 0.25 * torch.rand(per, 1, page, D, generator=g, device="cuda").half()
+    b.q = torch.ones(rows * seqs, H, D, dtype=torch.float16, device="cuda")
+    at = 77
+    b.kc[at // page, 0, at % page] = 1.0
+    b.vc[at // page, 0, at % page] = 1.0
+    scale = float(np.float32(np.log(2.0 ** 24 / weight) / D))
+    got = f64(ops.paged_attention(b.q, b.kc, b.vc, *b.batch(), scale=scale)).reshape(seqs, rows * H, D)
+    v = f64(b.vc)[:, 0].reshape(-1, D)
+    w = np.exp(-scale * D)
+    steps = n / 16 / (4 if rows == 1 else 1) + 300
+    for i in range(rows):  # the definition: every score is 0 but the one
+        seen = v[:n + i + 1]
+        total = 1 + w * (n + i)
+        want = (w * (seen.sum(0) - 1) + 1) / total
+        size = (w * (abs(seen).sum(0) - 1) + 1) / total
+        e = (U["f16"] + 2.0 ** -17 + 2.0 ** -23 * steps) * size + n * 2.0 ** -32 * 1.25
+        tol = U["f16"] * (abs(want) + e) + e
+        d = abs(got[:, i * H:(i + 1) * H] - want)
+        assert (d <= tol).all(), float((d / tol).max())
