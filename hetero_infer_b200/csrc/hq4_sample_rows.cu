@@ -32,6 +32,7 @@
 #include <algorithm>
 
 #include "hq4_host.cuh"
+#include "hq4_min_p.cuh"
 #include "hq4_paged.cuh"
 
 namespace hq4 {
@@ -76,15 +77,6 @@ __device__ __forceinline__ void st_cluster_u64(uint32_t addr, u64 v) {
 __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
-// Bits that order as the floats do, and back.
-__device__ __forceinline__ uint32_t order_bits(float x) {
-    const uint32_t b = __float_as_uint(x);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float order_value(uint32_t k) {
-    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
-}
-
 // B1: bits of the first digit.
 template <int T, int B1>
 struct SampleRowsShared {
@@ -524,17 +516,6 @@ struct SampleRow {
     }
 };
 
-// The smallest value that min_p keeps (above -inf; at most the maximum).
-__device__ __forceinline__ float min_p_end(float min_p, float top, double oct) {
-    const double most = -log2((double)fminf(min_p, 1.0f));
-    auto stays = [&](float x) { return ((double)top - (double)x) * oct <= most; };
-    const float guess = (float)((double)top - most / oct);
-    uint32_t k = order_bits(fminf(guess == guess ? guess : top, top) + 0.0f);
-    const uint32_t last = order_bits(top);
-    while (k < last && !stays(order_value(k))) k++;  // a rounding or two
-    while (k > 0x00800000u && stays(order_value(k - 1))) k--;
-    return order_value(k) + 0.0f;
-}
 // The place in [0, total) that u falls on.
 __device__ __forceinline__ u64 draw_place(double u, u64 total) {
     const double want = (u > 0.0 ? u : 0.0) * (double)total;

@@ -239,3 +239,28 @@ def test_many_long_rows(cuda, rows, n, kind):
     p = rng.choice([1.0, 0.9, 0.99, 0.5], rows)
     m = rng.choice([0.0, 0.0, 0.02], rows)
     check(logits(rng, rows, n), rng.random(rows), dt, temperature=t, top_k=k, top_p=p, min_p=m)
+
+
+@pytest.mark.gpu
+def test_infinite_temperatures(cuda):
+    """All finite entries are equally likely, whatever min_p is; the filters by value still hold."""
+    rng = np.random.default_rng(8)
+    n, inf = 5000, float("inf")
+    x = logits(rng, 12, n)
+    check(x, rng.random(12), temperature=[inf] * 12, min_p=[0.0, 0.3, 1.0, 7.0] * 3, top_k=[0] * 4 + [40] * 4 + [900] * 4,
+          top_p=[1.0, 1.0, 1.0, 1.0, 0.5, 0.5, 1.0, 0.9, 1.0, 0.3, 0.3, 1.0])
+    # finite ones: only the largest has at least its own probability.  (The oracle cannot say so: 1 - 3e-38, the
+    # next one's share of it, is 1 in 64 bits.)
+    _, tok, lp = run(x, rng.random(12), temperature=[3e38, 1e30] * 6, min_p=[1.0] * 12)
+    assert (tok == x.argmax(1)).all() and (lp == 0).all()
+
+
+@pytest.mark.gpu
+def test_min_p_that_ends_at_zero(cuda):
+    """Floats are densest around 0: a border there."""
+    rng = np.random.default_rng(9)
+    x = logits(rng, 6, 4000) - 30.0
+    x[:, 17] = 20.0
+    for i, v in enumerate([0.0, 1e-16, -1e-16, 1e-40, -1e-7, 1e-7]):
+        x[i, 2900 + i] = v
+    check(x, rng.random(6), min_p=[2.0611537e-9, 2.0611536e-9, 2.0611538e-9] * 2)
