@@ -46,7 +46,10 @@ constexpr double kSrOctaves = 43.9;      // that have mass (at least 1)
 constexpr int kSrList = 128;             // entries of a CTA that are compared directly
 constexpr int kSrFew = 384;              // entries of a row that top-k may leave for that
 constexpr int kSrMaxCluster = 8;
-constexpr int kSrMaxSlice = 36864;       // entries of a CTA
+constexpr int kSrMaxSlice = 36864;       // entries of a CTA of the longest row
+constexpr int kSrMaxRun = 192;           // entries of a thread at most: a bit each (SampleRow::Chosen)
+// Entries of a thread: odd, which spreads a warp over the banks.
+__host__ __device__ constexpr int sr_run(int slice, int threads) { return ((slice + threads - 1) / threads) | 1; }
 // Bytes of the first digit's sums, and of the lists that take their place.
 constexpr size_t sr_hist_bytes(int cols, int bits) {
     const size_t sums = (sizeof(unsigned long long) << bits) * cols;
@@ -232,14 +235,13 @@ struct SampleRow {
     // entries alone, where masses() works them out for all six whenever any
     // lane has chosen one.
     struct Chosen {
-        u64 bits[3];
+        u64 bits[kSrMaxRun / 64];
     };
-    static_assert((kSrMaxSlice + 255) / 256 + 1 <= 192, "the bits hold a run");
     template <class Pick>
     __device__ __forceinline__ Chosen choose(Pick pick) const {
         Chosen c;
 #pragma unroll
-        for (int w = 0; w < 6; w++) {
+        for (int w = 0; w < kSrMaxRun / 32; w++) {
             uint32_t m = 0;
             const int i0 = a + 32 * w, n = min(32, b - i0);
             for (int t = 0; t < n; t += 4)
@@ -253,7 +255,7 @@ struct SampleRow {
     template <class Use>
     __device__ __forceinline__ void masses_of(const Chosen& c, bool counting, Use use) const {
 #pragma unroll
-        for (int k = 0; k < 3; k++)
+        for (int k = 0; k < kSrMaxRun / 64; k++)
             for (u64 m = c.bits[k]; m;) {
                 int i[4];
                 float x[4];
@@ -557,7 +559,7 @@ __global__ void __launch_bounds__(T, 512 / T) sample_rows_kernel(const SampleRow
     cluster_sync();  // the slice is there, and the cluster's other CTAs run: their shared memory can be written
 
     // ---- its largest entry, the first of its equals; NaN ---------------------------
-    const int run = ((cnt + T - 1) / T) | 1;  // entries of a thread: odd, which spreads a warp over the banks
+    const int run = sr_run(cnt, T);
     SampleRow<E, T, B1, kCols> s{sh, reinterpret_cast<u64*>(smem), xs, lo, min(cnt, (int)threadIdx.x * run), 0, run, rank, nr,
                           0, 0, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0};
     s.b = min(cnt, s.a + run);
@@ -789,7 +791,8 @@ static int sample_rows(SampleRowsParams p, int rows, int sms, cudaStream_t st) {
         for (SrShape s : shapes) {
             s.cluster = cluster;
             s.smem = (size_t)((p.n + cluster - 1) / cluster + 16) * sizeof(E) + sr_hist_bytes(s.cols, s.bits);
-            if (s.smem > sr_smem_max(s.bits)) continue;
+            // (a slice of 16-bit entries that fits can be too long for 256 threads: 289 entries each of 73728)
+            if (s.smem > sr_smem_max(s.bits) || sr_run((p.n + cluster - 1) / cluster, s.threads) > kSrMaxRun) continue;
             const int per_sm = std::max(1, std::min<int>(512 / s.threads, (int)((size_t)227 * 1024 / (s.smem + 32 * 1024))));
             const int at_once = std::max(1, sms * per_sm / cluster);
             const int waves = (rows + at_once - 1) / at_once;

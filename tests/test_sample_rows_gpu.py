@@ -264,3 +264,16 @@ def test_min_p_that_ends_at_zero(cuda):
     for i, v in enumerate([0.0, 1e-16, -1e-16, 1e-40, -1e-7, 1e-7]):
         x[i, 2900 + i] = v
     check(x, rng.random(6), min_p=[2.0611537e-9, 2.0611536e-9, 2.0611538e-9] * 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,seed", [(1, 101), (20, 120), (90, 191)])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_long_rows_of_16_bits(cuda, rows, seed, kind):
+    """The longest rows in clusters of 8 and of fewer CTAs, every filter: a thread's run is long, and all of it counts."""
+    import torch
+    n = 8 * 36864
+    rng = np.random.default_rng(seed)
+    x = (rng.standard_normal((rows, n)) * 2).astype(np.float32)
+    check(x, rng.random(rows), {"bf16": torch.bfloat16, "f16": torch.float16}[kind], temperature=rng.choice([0.5, 1.0, 3.0], rows),
+          top_k=rng.choice([0, 0, 30, 5000, 200000], rows), top_p=rng.choice([1.0, 0.5, 0.95], rows))
