@@ -70,7 +70,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 4) paged_append_kernel(cons
     }
     const int s = find_seq(p.b.cu_rows, p.b.n_seqs, t);
     if (s < 0) return;
-    const int e = __ldg(p.b.lens + s) + (t - __ldg(p.b.cu_rows + s));
+    const long long far = (long long)__ldg(p.b.lens + s) + (t - __ldg(p.b.cu_rows + s));
+    const int e = far > 0x7fffffff ? -1 : (int)far;
     const int page = find_page(p.b, s, e), pos = p.positions ? __ldg(p.positions + t) : e;
     if (page < 0 || pos < 0 || pos >= p.max_pos) {
         if (part == 0 && lane == 0) atomicOr(p.b.status, kStatusPaged);

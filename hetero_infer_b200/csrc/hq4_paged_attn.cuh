@@ -50,13 +50,14 @@ struct PagedStart {
     long long total;  // units of the whole batch
 };
 
-// Rows and lengths of a sequence, clamped to what exists.
+// Rows and lengths of a sequence, clamped to what exists: entries beyond all
+// pages are not there, and sums with a length stay within 32 bits.
 __device__ __forceinline__ void paged_seq(const PagedAttnParams& p, int s, PagedItem& it) {
     const int a = max(__ldg(p.b.cu_rows + s), 0), e = min(__ldg(p.b.cu_rows + s + 1), p.b.n_rows);
     it.s = s;
     it.row0 = a;
     it.n_tok = max(e - a, 0);
-    it.len = __ldg(p.b.lens + s);
+    it.len = min(max(__ldg(p.b.lens + s), -(1 << 30)), p.b.pages_per_seq << p.b.page_shift);
 }
 template <int kRows>
 __device__ __forceinline__ int paged_row_tiles(const PagedAttnParams& p, const PagedItem& it) {

@@ -138,3 +138,50 @@ def test_one_strong_entry_and_many_weak_ones(cuda, seqs, H, rows, D, weight):
         tol = U["f16"] * (abs(want) + e) + e
         d = abs(got[:, i * H:(i + 1) * H] - want)
         assert (d <= tol).all(), float((d / tol).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,D,act,cache", [(1, 64, "bf16", "bf16"), (2, 64, "f32", "f16"), (20, 64, "f16", "f16"), (9, 128, "bf16", "bf16")])
+def test_lengths_at_the_ends_of_their_type(cuda, rows, D, act, cache):
+    """A length beyond all pages is one that ends with them; one far below 0 leaves nothing."""
+    import torch
+    from hetero_infer_b200 import ops
+    b = Batch([rows] * 3, [50, 90, 5], 4, 2, D, 16, act, cache, seed=3, stale=False)
+    m = tree(b.rows, 1)
+    cap = b.pages.shape[1] * b.page
+    calls = [lambda: ops.paged_attention(b.q, b.kc, b.vc, *b.batch()), lambda: ops.tree_attention(b.q, b.kc, b.vc, *b.batch(), m)]
+    b.lens[1] = cap
+    want = [c() for c in calls]
+    for far in (2 ** 31 - 1, 2 ** 31 - 2 - rows, 2 ** 31 - 60):
+        b.lens[1] = far
+        assert all(torch.equal(c(), w) for c, w in zip(calls, want)), far
+    for far in (-2 ** 31, -2 ** 31 + 7):
+        b.lens[1] = far
+        for c, w in zip(calls, want):
+            got = c()
+            assert (got[rows:2 * rows] == 0).all()
+            assert torch.equal(got[:rows], w[:rows]) and torch.equal(got[2 * rows:], w[2 * rows:])
+
+
+@pytest.mark.gpu
+def test_append_at_the_ends_of_lengths(cuda):
+    """Rows whose entries lie beyond all pages, or before the first, write nothing."""
+    import torch
+    from hetero_infer_b200 import _lib, ops
+    lib = _lib.load()
+    b = Batch([4] * 4, [50, 90, 5, 7], 4, 2, 64, 16, "bf16", "bf16", seed=3, stale=False)
+    b.lens[:3] = torch.tensor([2 ** 31 - 1, 2 ** 31 - 3, -2 ** 31], device="cuda")
+    pos = torch.arange(16, dtype=torch.int32, device="cuda")
+    cos, sin = torch.ones(16, 32, device="cuda"), torch.zeros(16, 32, device="cuda")
+    k0, v0 = b.kc.clone(), b.vc.clone()
+    lib.hq4_device_status(1)
+    out = torch.full((16, 4, 64), 77.0, dtype=torch.bfloat16, device="cuda")
+    ops.paged_append(b.q, b.k, b.v, b.kc, b.vc, *b.batch(), cos, sin, positions=pos, out=out)
+    assert lib.hq4_device_status(1) & 16
+    assert (out[:12] == 77.0).all() and torch.equal(out[12:], b.q[12:])
+    for now, was, new in ((b.kc, k0, b.k), (b.vc, v0, b.v)):
+        for i in range(4):
+            page, at = op.place(b.pages.cpu().numpy(), b.n_pages, 16, 3, 7 + i)
+            assert torch.equal(now[page, :, at], new[12 + i])
+            was[page, :, at] = now[page, :, at]
+        assert torch.equal(now, was)
