@@ -207,6 +207,17 @@ extern "C" int hq4_paged_append(const void* q, const void* k, const void* v, int
         rows_overlap(k, n_rows, k_stride, k_row, elem, q_out, out_bytes) ||
         rows_overlap(v, n_rows, v_stride, k_row, elem, q_out, out_bytes))
         return HQ4_ERR_SHAPE;
+    // what is written is not read: neither the rows nor the queries lie in the caches, nor the one cache in the other
+    const long long page = (long long)n_kv * page_size * head_dim;
+    const __int128 cache_bytes = ((__int128)(n_pages - 1) * page_stride + page) * 2;
+    const void* const caches[2] = {k_cache, v_cache};
+    for (const void* cache : caches)
+        if (rows_overlap(q_out, n_rows, q_row, q_row, elem, cache, cache_bytes) ||
+            rows_overlap(q, n_rows, q_stride, q_row, elem, cache, cache_bytes) ||
+            rows_overlap(k, n_rows, k_stride, k_row, elem, cache, cache_bytes) ||
+            rows_overlap(v, n_rows, v_stride, k_row, elem, cache, cache_bytes))
+            return HQ4_ERR_SHAPE;
+    if (pages_overlap(k_cache, v_cache, n_pages, page_stride, page, 2)) return HQ4_ERR_SHAPE;
     if (int rc = check_device_cap()) return rc;
     p.b.status = status_word();
     if (!p.b.status) return HQ4_ERR_LAUNCH;

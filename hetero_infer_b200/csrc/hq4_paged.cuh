@@ -54,9 +54,17 @@ __device__ __forceinline__ int find_page(const PagedBatch& b, int s, int e) {
 
 // Whether `rows` rows of `row` elements, `stride` apart, reach into the n_bytes at b (host).
 static inline bool rows_overlap(const void* a, long long rows, long long stride, long long row, int elem_bytes,
-                                const void* b, long long n_bytes) {
+                                const void* b, __int128 n_bytes) {
     const __int128 from = (intptr_t)a, to = from + ((__int128)(rows - 1) * stride + row) * elem_bytes;
-    return from < (__int128)(intptr_t)b + n_bytes && (intptr_t)b < to;
+    return from < (intptr_t)b + n_bytes && (intptr_t)b < to;
+}
+
+// Whether one of n pages of `page` elements, `stride` apart, from a on reaches into one of those from b on (host).
+static inline bool pages_overlap(const void* a, const void* b, long long n, long long stride, long long page, int elem_bytes) {
+    const intptr_t x = (intptr_t)a, y = (intptr_t)b;
+    const unsigned long long d = x < y ? (unsigned long long)y - x : (unsigned long long)x - y, step = (unsigned long long)stride * elem_bytes;
+    const unsigned long long apart = d / step, rest = d % step, bytes = (unsigned long long)page * elem_bytes;
+    return (apart < (unsigned long long)n && rest < bytes) || (apart + 1 < (unsigned long long)n && step - rest < bytes);
 }
 
 template <class T>

@@ -81,7 +81,13 @@ static int paged_attention(const void* q, int act_type, int n_rows, int n_heads,
         return HQ4_ERR_ALIGN;
     const long long q_row = (long long)n_heads * head_dim;
     const int elem = act_type == HQ4_F32 ? 4 : 2;
-    if (rows_overlap(q, n_rows, q_stride, q_row, elem, out, n_rows * q_row * elem)) return HQ4_ERR_SHAPE;
+    const long long page = (long long)n_kv * page_size * head_dim;
+    auto overlaps_inputs = [&](const void* to, long long bytes) {
+        return rows_overlap(q, n_rows, q_stride, q_row, elem, to, bytes) ||
+               rows_overlap(k_cache, n_pages, page_stride, page, 2, to, bytes) ||
+               rows_overlap(v_cache, n_pages, page_stride, page, 2, to, bytes);
+    };
+    if (overlaps_inputs(out, n_rows * q_row * elem)) return HQ4_ERR_SHAPE;
     if (int rc = check_device_cap()) return rc;
     p.b.status = status_word();
     const int sms = device_sms();
@@ -90,6 +96,8 @@ static int paged_attention(const void* q, int act_type, int n_rows, int n_heads,
     if (pl.ws) {
         if (!workspace || workspace_bytes < pl.ws) return HQ4_ERR_SHAPE;
         if ((uintptr_t)workspace & 127) return HQ4_ERR_ALIGN;
+        if (overlaps_inputs(workspace, pl.ws) || rows_overlap(workspace, 1, pl.ws, pl.ws, 1, out, n_rows * q_row * elem))
+            return HQ4_ERR_SHAPE;
     }
     p.q = q;
     p.k = k_cache;

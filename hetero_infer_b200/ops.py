@@ -235,7 +235,8 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: tor
     caches' type, views of one projection if need be; rope_cos, rope_sin:
     float32 [max_pos, head_dim / 2].  A row's position is its entry's number or
     positions[row] (int32); q_norm, k_norm: float32 [head_dim], an RMS norm of
-    each head before the rotation.  out must not overlap q, k or v."""
+    each head before the rotation.  out must not overlap q, k, v or the caches,
+    nor the caches q, k or v."""
     return _lib.torch_calls().paged_append(q, k, v, k_cache, v_cache, pages, cu_rows, lens, rope_cos, rope_sin,
                                            positions, q_norm, k_norm, eps, out)
 
@@ -252,7 +253,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """Causal grouped-query attention of a ragged batch over the paged cache
     (hq4_paged_attention): row i of sequence s sees entries 0 .. lens[s] + i.
     q: [rows, n_heads, head_dim] as paged_append returns it; scale defaults to
-    head_dim ** -0.5, out must not overlap q.  Decode, prompt chunks and
+    head_dim ** -0.5, out must not overlap q or the caches.  Decode, prompt chunks and
     mixtures of them alike."""
     return _lib.torch_calls().attend(q, k_cache, v_cache, pages, cu_rows, lens, None, scale, out, workspace)
 

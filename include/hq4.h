@@ -309,8 +309,9 @@ int hq4_advance_position(int* pos, int delta, void* stream);
 #define HQ4_F16 2
 
 /* Appends the rows of k (rotated) and v to their pages and writes the rotated
- * queries to q_out [n_rows][n_heads][head_dim] (which must not overlap q, k or
- * v).  Rotation as hq4_qkv_rope: half-split, cos/sin tables
+ * queries to q_out [n_rows][n_heads][head_dim].  q_out must not overlap q, k, v
+ * or the caches, nor the caches q, k or v, nor a page of one cache a page of the
+ * other (-1).  Rotation as hq4_qkv_rope: half-split, cos/sin tables
  * [max_pos][head_dim/2]; a row's position is its entry's number, or positions[row] where positions
  * is not NULL (the nodes of a drafted tree: entries one after another,
  * positions by depth).  q_norm / k_norm ([head_dim], each may be NULL): an RMS
@@ -326,13 +327,13 @@ int hq4_paged_append(const void* q, const void* k, const void* v, int act_type, 
 
 /* Grouped-query attention of the batch's rows over the cache: row i of
  * sequence s attends to entries [0, lens[s] + i], its own among them
- * (hq4_paged_append first).  out [n_rows][n_heads][head_dim] must not overlap
- * q; a row that sees nothing is zeros (one whose scores are all -inf is NaN).
- * What lies in entries that a row does
- * not see (stale pages, NaN, infinities) does not reach it.  The workspace
- * (hq4_paged_attention_workspace_bytes, 128-byte aligned; may be NULL where
- * that is 0) is written and read by one call: calls that can run at the same
- * time must not share it.  Deterministic; allocates nothing. */
+ * (hq4_paged_append first).  out [n_rows][n_heads][head_dim] and the workspace
+ * must overlap neither q, the caches nor one another (-1); a row that sees
+ * nothing is zeros (one whose scores are all -inf is NaN).  What lies in entries
+ * that a row does not see (stale pages, NaN, infinities) does not reach it.  The
+ * workspace (hq4_paged_attention_workspace_bytes, 128-byte aligned; may be NULL
+ * where that is 0) is written and read by one call: calls that can run at the
+ * same time must not share it.  Deterministic; allocates nothing. */
 int hq4_paged_attention(const void* q, int act_type, int n_rows, int n_heads, int n_kv, int head_dim,
                         long long q_stride, const int* cu_rows, const int* lens, int n_seqs, const int* pages,
                         int pages_per_seq, const void* k_cache, const void* v_cache, int cache_type, int n_pages,

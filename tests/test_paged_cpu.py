@@ -143,3 +143,30 @@ def test_outputs_over_inputs_refused(at, rc):
     assert append(q=P * 8, k=far, v=far, out=P * 8 + at) == rc
     assert append(q=far, k=P * 8, v=far, ks=512, out=P * 8 + min(at, 3 * 512 * 2 + 128 * 2 - 16)) == rc
     assert append(q=far, k=far, v=P * 8, vs=512, out=P * 8 + min(at, 3 * 512 * 2 + 128 * 2 - 16)) == rc
+
+
+KB = 2 * 16 * 64 * 2  # bytes of a page of one cache
+FAR = 1 << 30
+
+
+@pytest.mark.parametrize("out", [FAR, FAR + 20 * KB - 16, FAR - 4 * 512 * 2 + 16, 2 * FAR + 7 * KB])
+def test_outputs_over_the_caches_refused(out):
+    """20 pages of keys and of values: an output that begins or ends in them."""
+    a = dict(q=P, kc=FAR, vc=2 * FAR, out=out)
+    assert attention(**a) == -1 and attention(tree=True, **a) == -1
+    assert append(k=P + (1 << 16), v=P + (1 << 17), **a) == -1
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v"])
+@pytest.mark.parametrize("at", [FAR, FAR + 20 * KB - 16, 2 * FAR + 5 * KB])
+def test_rows_in_the_caches_refused(name, at):
+    """Rows that the append reads while it writes the pages that they lie in."""
+    a = dict(q=P, k=P + (1 << 16), v=P + (1 << 17), kc=FAR, vc=2 * FAR, out=P * 8)
+    assert append(**{**a, name: at}) == -1
+
+
+@pytest.mark.parametrize("stride,at", [(KB, 0), (KB, 16), (KB, 19 * KB + 16), (KB, -19 * KB - 16), (3 * KB, KB - 16), (3 * KB, 2 * KB + 16),
+                                       (3 * KB, 19 * 3 * KB), (3 * KB, -2 * 3 * KB)])
+def test_caches_in_one_another_refused(stride, at):
+    a = dict(q=P, k=P + (1 << 16), v=P + (1 << 17), out=P * 8, stride=stride // 2)
+    assert append(kc=FAR, vc=FAR + at, **a) == -1

@@ -737,3 +737,35 @@ def test_outputs_beside_inputs(cuda, rows, act, cache):
         assert torch.equal(ops.paged_attention(q, b.kc, b.vc, *b.batch(), out=out), want)
         assert torch.equal(ops.paged_append(q, b.k, b.v, b.kc.clone(), b.vc.clone(), *b.batch(), cos, sin, out=out), turned)
         assert torch.equal(q, b.q)
+
+
+@pytest.mark.gpu
+def test_buffers_over_one_another_refused(cuda):
+    """What a call writes must not be what it reads; caches that lie between one another's pages are accepted."""
+    import torch
+    from hetero_infer_b200 import ops
+    b = Batch([2, 40], [700, 1500], 4, 2, 64, 16, "bf16", "bf16", interleave=True, stale=False)
+    cos, sin = tables(1600, 64)
+    q, rows = b.q.contiguous(), b.n * 4 * 64
+    pool = torch.zeros(max(2 * rows, ops.paged_attention_workspace(q, b.kc, b.pages).numel() + 4 * rows), dtype=torch.uint8, device="cuda")
+    in_ws = pool[256:256 + 2 * rows].view(torch.bfloat16).view(b.n, 4, 64)
+    in_ws.copy_(q)
+    whole = b.kc.contiguous()
+    in_cache = whole.view(-1)[512:512 + rows].view(b.n, 4, 64)
+    k_in_cache = whole.view(-1)[512:512 + rows // 2].view(b.n, 2, 64)
+    want = ops.paged_attention(q, b.kc, b.vc, *b.batch())
+    for call in (lambda: ops.paged_attention(q, b.kc, b.vc, *b.batch(), out=in_ws, workspace=pool),
+                 lambda: ops.paged_attention(in_ws, b.kc, b.vc, *b.batch(), workspace=pool),
+                 lambda: ops.paged_attention(q, whole, b.vc.contiguous(), *b.batch(), out=in_cache),
+                 lambda: ops.paged_append(q, k_in_cache, b.v, whole, b.vc.contiguous(), *b.batch(), cos, sin),
+                 lambda: ops.paged_append(q, b.k, b.v, whole, whole, *b.batch(), cos, sin)):
+        with pytest.raises(RuntimeError):
+            call()
+    ops.paged_append(q, b.k, b.v, b.kc.clone(), b.vc.clone(), *b.batch(), cos, sin)
+    both = torch.stack((b.kc, b.vc), 1)  # pages of keys and values by turns
+    ops.paged_append(q, b.k, b.v, both[:, 0], both[:, 1], *b.batch(), cos, sin)
+    k, v = b.kc.clone(), b.vc.clone()
+    ops.paged_append(q, b.k, b.v, k, v, *b.batch(), cos, sin)
+    assert torch.equal(both[:, 0], k) and torch.equal(both[:, 1], v)
+    assert torch.equal(ops.paged_attention(q, whole, whole, *b.batch()), ops.paged_attention(q, whole, whole.clone(), *b.batch()))
+    assert torch.equal(want, ops.paged_attention(q, b.kc, b.vc, *b.batch()))
