@@ -827,6 +827,19 @@ extern "C" int hq4_sample_rows(const void* logits, int act_type, int n_rows, int
         (((uintptr_t)temperature | (uintptr_t)top_k | (uintptr_t)top_p | (uintptr_t)min_p | (uintptr_t)tok |
           (uintptr_t)logprob) & 3))
         return HQ4_ERR_ALIGN;
+    // what a row's clusters write, those of other rows do not read (a row's own parameter may lie where its result goes)
+    const int elem = act_type == HQ4_F32 ? 4 : 2;
+    const void* const outs[2] = {tok, logprob};
+    const void* const params[5] = {temperature, top_k, top_p, min_p, tok};
+    for (const void* out : outs) {
+        if (!out) continue;
+        const long long bytes = 4ll * n_rows;
+        if (rows_overlap(logits, n_rows, row_stride, n, elem, out, bytes) || rows_overlap(u, n_rows, 1, 1, 8, out, bytes))
+            return HQ4_ERR_SHAPE;
+        for (const void* x : params)
+            if (x && (x != out || (x == tok && out == logprob)) && rows_overlap(x, n_rows, 1, 1, 4, out, bytes))
+                return HQ4_ERR_SHAPE;
+    }
     if (int rc = check_device_cap()) return rc;
     SampleRowsParams p = {};
     p.x = logits;

@@ -374,7 +374,8 @@ long long hq4_paged_attention_workspace_bytes(int act_type, int n_rows, int n_he
  * those that stay (0 for a greedy one).  Masses are 44-bit fixed point, so the
  * draw does not depend on an order of summation.  -inf logits have no mass; a
  * row with a NaN, a +inf or -inf alone gets token n - 1 and log probability
- * NaN, and sets status bit 3.  n up to 8 x 36864. */
+ * NaN, and sets status bit 3.  n up to 8 x 36864.  tok and logprob must not
+ * overlap logits, u, one another or, but for the same address, a parameter (-1). */
 int hq4_sample_rows(const void* logits, int act_type, int n_rows, int n, long long row_stride,
                     const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                     const double* u, int* tok, float* logprob, void* stream);

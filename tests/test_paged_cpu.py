@@ -170,3 +170,14 @@ def test_rows_in_the_caches_refused(name, at):
 def test_caches_in_one_another_refused(stride, at):
     a = dict(q=P, k=P + (1 << 16), v=P + (1 << 17), out=P * 8, stride=stride // 2)
     assert append(kc=FAR, vc=FAR + at, **a) == -1
+
+
+@pytest.mark.parametrize("kw", [dict(tok=FAR), dict(tok=FAR + 3 * 4096 + 1600 - 4), dict(logprob=FAR + 40), dict(tok=FAR - 12), dict(tok=2 * FAR + 28),
+                                dict(logprob=2 * FAR - 4), dict(tok=P, logprob=P), dict(tok=P, logprob=P + 12), dict(tok=P, top_k=P + 4),
+                                dict(tok=P, logprob=P + 64, top_p=P + 60), dict(tok=P + 12, min_p=P, temperature=P)])
+def test_samples_over_inputs_refused(kw):
+    """4 rows of 400 fp32 logits, 4096 bytes apart, at FAR, their u at 2 FAR."""
+    a = dict(x=FAR, kind=0, rows=4, n=400, stride=1024, temperature=None, top_k=None, top_p=None, min_p=None, u=2 * FAR, tok=P,
+             logprob=None, stream=None)
+    a.update(kw)
+    assert _lib.load().hq4_sample_rows(*a.values()) == -1

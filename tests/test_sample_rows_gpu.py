@@ -277,3 +277,21 @@ def test_long_rows_of_16_bits(cuda, rows, seed, kind):
     x = (rng.standard_normal((rows, n)) * 2).astype(np.float32)
     check(x, rng.random(rows), {"bf16": torch.bfloat16, "f16": torch.float16}[kind], temperature=rng.choice([0.5, 1.0, 3.0], rows),
           top_k=rng.choice([0, 0, 30, 5000, 200000], rows), top_p=rng.choice([1.0, 0.5, 0.95], rows))
+
+
+@pytest.mark.gpu
+def test_results_in_place_of_parameters(cuda):
+    """A row's token may go where its top_k was; results over other rows' inputs are refused."""
+    import torch
+    from hetero_infer_b200 import ops
+    rng = np.random.default_rng(10)
+    x = torch.from_numpy(logits(rng, 8, 70000)).cuda()
+    u = torch.from_numpy(rng.random(8)).cuda()
+    k = torch.arange(0, 400, 50, dtype=torch.int32, device="cuda")
+    want = ops.sample_rows(x, u, top_k=k.clone())
+    assert torch.equal(ops.sample_rows(x, u, top_k=k, out=k), want) and torch.equal(k, want)
+    pool = torch.zeros(9, dtype=torch.int32, device="cuda")
+    for a, kw in (((x, u), dict(out=x.view(torch.int32)[0, :8])), ((x, u), dict(out=u.view(torch.int32)[:8])),
+                  ((x, u), dict(top_k=pool[:8], out=pool[1:]))):
+        with pytest.raises(RuntimeError):
+            ops.sample_rows(*a, **kw)
