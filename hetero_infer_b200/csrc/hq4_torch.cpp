@@ -274,6 +274,8 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!count(n, 8)) return nullptr;
     return guarded([&]() -> PyObject* {
         const at::Tensor& x = tensor(a[0], "logits");
+        const int want = PyObject_IsTrue(a[7]);
+        if (want < 0) throw PyError{};
         if (x.dim() != 2 || !x.is_cuda() || type_code(x.scalar_type()) < 0)
             refuse("logits must be a CUDA float32, bfloat16 or float16 tensor [rows, vocab]");
         const int64_t rows = x.size(0), vocab = x.size(1);
@@ -289,7 +291,7 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
             need(t[i], names[i], types[i], x.device());
             if (t[i].dim() != 1 || t[i].size(0) != rows) refuse(names[i], " must be [rows], got ", t[i].sizes());
         }
-        const bool given = t[5].defined(), want = PyObject_IsTrue(a[7]) == 1;
+        const bool given = t[5].defined();
         if (!given) t[5] = at::detail::empty_cuda({rows}, at::kInt, x.device(), std::nullopt);
         at::Tensor lp;
         if (want) lp = at::detail::empty_cuda({rows}, at::kFloat, x.device(), std::nullopt);

@@ -181,3 +181,11 @@ def test_samples_over_inputs_refused(kw):
              logprob=None, stream=None)
     a.update(kw)
     assert _lib.load().hq4_sample_rows(*a.values()) == -1
+
+
+def test_logprob_without_a_truth_value():
+    """Its error is raised, and not left behind under a result."""
+    import torch
+    from hetero_infer_b200 import ops
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        ops.sample_rows(torch.zeros(2, 4), torch.zeros(2, dtype=torch.float64), logprob=torch.zeros(2))
