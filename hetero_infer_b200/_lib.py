@@ -127,7 +127,8 @@ def torch_calls():
         return _torch_calls
     path = _build.TORCH_LIB
     if not os.path.exists(path):
-        raise RuntimeError(f"{path} is missing: build it with `python -m hetero_infer_b200.build`")
+        raise RuntimeError(f"{path} is missing: build it with `python -m hetero_infer_b200.build`, which says why where "
+                           "it cannot (it needs PyTorch's headers and a host compiler)")
     import importlib.util
 
     import torch  # noqa: F401  (its libraries)

@@ -2,7 +2,8 @@
 
 The library is plain C ABI (``include/hq4.h``) over hand-written CUDA, without
 torch headers.  Beside it, ``_hq4_torch`` (host code only, one file over torch's
-headers) makes the paged operators' calls from tensors.  Both build without a GPU.
+headers) makes the paged operators' calls from tensors; the library builds and
+works without it.  Both build without a GPU.
 """
 from __future__ import annotations
 
@@ -63,7 +64,11 @@ def torch_command():
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile every csrc/*.cu into libhq4.so, and _hq4_torch.so (each skipped when up to date)."""
+    """Compile every csrc/*.cu into libhq4.so, and _hq4_torch.so (each skipped when up to date).
+
+    libhq4.so needs nvcc alone.  Where _hq4_torch cannot be built (no torch, none of
+    its headers, no host compiler) the reason goes to stderr, and the calls that
+    need it (_lib.torch_calls) say that it is missing."""
     todo = [lib for lib in (LIB, TORCH_LIB) if force or not up_to_date(lib)]
     if not todo:
         return LIB
@@ -76,19 +81,24 @@ def build(force: bool = False, verbose: bool = False) -> str:
             raise RuntimeError("the build failed:\n" + " ".join(cmd) + "\n" + out.stdout + out.stderr)
         return out.stderr
 
-    with tempfile.TemporaryDirectory() as tmp:  # the files side by side, then one link
-        files = sources() if LIB in todo else []
-        objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in files]
-        cmds = [[nvcc(), *ARCH_FLAGS, *NVCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", s, "-o", o]
-                for s, o in zip(files, objs)]
-        if TORCH_LIB in todo:
-            cmds.append(torch_command())
-        with concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
-            logs = list(pool.map(run, cmds))
-        if files:
+    logs = []
+    with tempfile.TemporaryDirectory() as tmp, \
+            concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        binding = pool.submit(lambda: run(torch_command())) if TORCH_LIB in todo else None
+        if LIB in todo:  # the files side by side, then one link
+            objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in sources()]
+            logs += pool.map(run, ([nvcc(), *ARCH_FLAGS, *NVCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", s, "-o", o]
+                                   for s, o in zip(sources(), objs)))
             run([nvcc(), *ARCH_FLAGS, "-shared", "-o", LIB + ".tmp", *objs])
-    for lib in todo:
-        os.replace(lib + ".tmp", lib)
+            os.replace(LIB + ".tmp", LIB)
+        if binding:
+            try:
+                logs.append(binding.result())
+                os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+            except (ImportError, OSError, RuntimeError) as e:
+                if os.path.exists(TORCH_LIB):  # it does not fit these sources
+                    os.remove(TORCH_LIB)
+                sys.stderr.write(f"{TORCH_LIB} was not built (libhq4.so is there without it): {e}\n")
     if verbose:
         sys.stdout.write("".join(logs))
     return LIB
