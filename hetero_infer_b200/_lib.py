@@ -132,6 +132,10 @@ def torch_calls():
     import importlib.util
 
     import torch  # noqa: F401  (its libraries)
+    had, have = _build.built_for(), _build.torch_version()
+    if had and had != have:
+        raise RuntimeError(f"{path} was built for torch {had}, torch {have} is installed: build it again with "
+                           "`python -m hetero_infer_b200.build`")
     lib = load()
     spec = importlib.util.spec_from_file_location("hetero_infer_b200._hq4_torch", path)
     mod = importlib.util.module_from_spec(spec)

@@ -40,8 +40,28 @@ def headers():
     return sorted(glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h")))
 
 
+def torch_version() -> str:
+    """The installed torch's version, without importing it ('' where there is none)."""
+    import importlib.metadata
+    try:
+        return importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        return ""
+
+
+def built_for() -> str:
+    """The torch version that _hq4_torch.so was built against, from the file beside it ('' for none)."""
+    try:
+        with open(TORCH_LIB + ".torch") as f:
+            return f.read().strip()
+    except OSError:
+        return ""
+
+
 def up_to_date(lib: str = LIB) -> bool:
     if not os.path.exists(lib):
+        return False
+    if lib == TORCH_LIB and built_for() != torch_version():  # torch's ABI is that of a version
         return False
     t = os.path.getmtime(lib)
     deps = [TORCH_SRC] if lib == TORCH_LIB else sources()
@@ -95,6 +115,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
             try:
                 logs.append(binding.result())
                 os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+                with open(TORCH_LIB + ".torch", "w") as f:
+                    f.write(torch_version() + "\n")
             except (ImportError, OSError, RuntimeError) as e:
                 if os.path.exists(TORCH_LIB):  # it does not fit these sources
                     os.remove(TORCH_LIB)

@@ -46,3 +46,19 @@ def test_a_missing_binding_is_named(tmp_path, monkeypatch):
     monkeypatch.setattr(_lib, "_torch_calls", None)
     with pytest.raises(RuntimeError, match="_hq4_torch.so is missing"):
         _lib.torch_calls()
+
+
+def test_a_binding_for_another_torch(tmp_path, monkeypatch):
+    """It is neither taken for up to date nor loaded."""
+    import shutil
+    from hetero_infer_b200 import _lib, build
+    path = str(tmp_path / "_hq4_torch.so")
+    shutil.copy(build.TORCH_LIB, path)
+    monkeypatch.setattr(build, "TORCH_LIB", path)
+    monkeypatch.setattr(_lib, "_torch_calls", None)
+    (tmp_path / "_hq4_torch.so.torch").write_text(build.torch_version() + "\n")
+    assert build.up_to_date(path) and build.torch_version()
+    (tmp_path / "_hq4_torch.so.torch").write_text("1.0.0\n")
+    assert not build.up_to_date(path)
+    with pytest.raises(RuntimeError, match="built for torch 1.0.0"):
+        _lib.torch_calls()
