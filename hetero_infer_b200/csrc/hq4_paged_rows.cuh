@@ -33,8 +33,16 @@ struct PaShape {
     static constexpr int kTile = kPaKeys * kDim * 2;                  // bytes of a tile of keys or of values
     static constexpr int kRing = kStages * 2 * kTile;                 // of a warp
 };
+// 16-bit terms of a query.
 template <class A, class C>
 constexpr int pa_terms() { return sizeof(A) == 2 ? 1 : Elem<C>::code == HQ4_BF16 ? 3 : 2; }
+// 16-bit terms of a probability.  Of 16-bit calls two, so that the output's own
+// rounding is the only one to 16 bits (with one, errors against 64 bits are 1.13
+// times as large): 64 streams of 100 to 8200 entries, 28 heads of 128: 131 us
+// with one, 135 with two (flushed caches).  Wide heads keep one, which is off by
+// at most half a step of each probability: two would cost 279 -> 298 us there.
+template <class A, class C, int kDim>
+constexpr int pa_p_terms() { return sizeof(A) == 4 ? pa_terms<A, C>() : kDim <= 128 ? 2 : 1; }
 template <int kDim, int kRows, int kTerms, int W>
 constexpr int pa_smem() { return W * PaShape<kDim>::kRing + kTerms * kRows * kDim * 2; }
 
@@ -75,7 +83,7 @@ __device__ __forceinline__ int tile_at(int r, int c) { return r * (kDim * 2) + (
 // NT: 8-row tiles; W: warps.
 template <class A, class C, int kDim, int NT, int W>
 __global__ void __launch_bounds__(W * 32) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
-    constexpr int kRows = 8 * NT, kTerms = pa_terms<A, C>(), kStages = PaShape<kDim>::kStages;
+    constexpr int kRows = 8 * NT, kTerms = pa_terms<A, C>(), kPTerms = pa_p_terms<A, C, kDim>(), kStages = PaShape<kDim>::kStages;
     constexpr int kTile = PaShape<kDim>::kTile, kRing = PaShape<kDim>::kRing;
     constexpr int kChunks = kDim / 8, kOs = kDim + 4;
     static_assert(kRows * kOs * 4 <= kRing, "a warp's outputs fit its ring");
@@ -333,7 +341,7 @@ __global__ void __launch_bounds__(W * 32) paged_attn_kernel(const __grid_constan
             // the probabilities as 16-bit terms, transposed (of fp16: scaled by 2^14, which the epilogue takes back,
             // so that those of 2^-28 of the largest are still normal numbers: unscaled, 10^5 entries 25 octaves
             // below one would add to the sum and nothing to the output)
-            uint32_t pb[NT][kTerms][2];
+            uint32_t pb[NT][kPTerms][2];
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -344,7 +352,7 @@ __global__ void __launch_bounds__(W * 32) paged_attn_kernel(const __grid_constan
                         b *= 16384.0f;
                     }
 #pragma unroll
-                    for (int term = 0; term < kTerms; term++) {
+                    for (int term = 0; term < kPTerms; term++) {
                         const uint32_t w = pack2<C>(a, b);
                         pb[n][term][hh] = transpose8(w);
                         const float2 f = unpack2<C>(w);
@@ -360,11 +368,12 @@ __global__ void __launch_bounds__(W * 32) paged_attn_kernel(const __grid_constan
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     if constexpr (kTerms == 1) {
-                        mma16<C>(acc[d][n], a, pb[n][0][0], pb[n][0][1]);
+#pragma unroll
+                        for (int term = kPTerms - 1; term >= 0; term--) mma16<C>(acc[d][n], a, pb[n][term][0], pb[n][term][1]);
                     } else {  // fp32's precision: a tile's sum by itself, then rounded to nearest into the whole
                         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                        for (int term = kTerms - 1; term >= 0; term--) mma16<C>(sum, a, pb[n][term][0], pb[n][term][1]);
+                        for (int term = kPTerms - 1; term >= 0; term--) mma16<C>(sum, a, pb[n][term][0], pb[n][term][1]);
 #pragma unroll
                         for (int i = 0; i < 4; i++) acc[d][n][i] = fmaf(acc[d][n][i], keep[n][i & 1], sum[i]);
                     }

@@ -18,7 +18,9 @@
 // P V is complete when S of the next tile is (matrix instructions complete in
 // order), so whoever sees S may touch O.  P is rounded to the cache's type, at
 // most half a step of each probability: the same size as the rounding of the
-// 16-bit output.  fp16 has few steps below 1, so its P (and the sums with it)
+// 16-bit output (errors against 64 bits are up to 1.4 times that rounding's
+// alone; a caller who wants them smaller passes fp32 queries, which the
+// warp-level kernel takes).  fp16 has few steps below 1, so its P (and the sums with it)
 // are scaled by 2^7, to at most 2^15: a probability is a normal number down to
 // 2^-21 of 2^m, and below that off by at most 2^-32 of it.
 //

@@ -333,7 +333,10 @@ int hq4_paged_append(const void* q, const void* k, const void* v, int act_type, 
  * that a row does not see (stale pages, NaN, infinities) does not reach it.  The
  * workspace (hq4_paged_attention_workspace_bytes, 128-byte aligned; may be NULL
  * where that is 0) is written and read by one call: calls that can run at the
- * same time must not share it.  Deterministic; allocates nothing. */
+ * same time must not share it.  Deterministic; allocates nothing.
+ * With fp32 queries results are good to fp32.  With 16-bit ones each probability
+ * may be rounded to the cache's type (half a step of it, as the outputs are):
+ * heads above 128, and prompts and trees. */
 int hq4_paged_attention(const void* q, int act_type, int n_rows, int n_heads, int n_kv, int head_dim,
                         long long q_stride, const int* cu_rows, const int* lens, int n_seqs, const int* pages,
                         int pages_per_seq, const void* k_cache, const void* v_cache, int cache_type, int n_pages,

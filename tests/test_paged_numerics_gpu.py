@@ -185,3 +185,20 @@ def test_append_at_the_ends_of_lengths(cuda):
             assert torch.equal(now[page, :, at], new[12 + i])
             was[page, :, at] = now[page, :, at]
         assert torch.equal(now, was)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,KV,D,kind", [(7, 1, 128, "bf16"), (28, 4, 128, "f16"), (8, 2, 64, "bf16"), (4, 4, 32, "f16"), (6, 2, 96, "bf16")])
+@pytest.mark.parametrize("ctx", [[159], [9, 700, 2000]])
+def test_decode_rounds_its_outputs_alone(cuda, H, KV, D, kind, ctx):
+    """A probability as two terms is off by 2^-17 of itself (bf16: 16 bits) or
+    2^-21 (fp16, down to its smallest step); the rest as test_paged_gpu.py has it."""
+    from hetero_infer_b200 import ops
+    b = Batch([1] * len(ctx), ctx, H, KV, D, 16, kind, kind, seed=D)
+    want, size, score = op.attention(f64(b.q), f64(b.kc), f64(b.vc), *b.host(), D ** -0.5)
+    n = max(ctx) + 1
+    s_err = ((D + 8) * 2.0 ** -23 + 2.0 ** -21) * score[..., None]
+    e = (2 * s_err + 2.0 ** -20 + (2.0 ** -17 if kind == "bf16" else 2.0 ** -21) + (n / 16 + 16) * 2.0 ** -22) * size
+    tol = U[kind] * (abs(want) + e) + e + (2.0 ** -25 if kind == "f16" else 0)
+    d = abs(f64(ops.paged_attention(b.q, b.kc, b.vc, *b.batch())) - want)
+    assert (d <= tol).all(), float((d / tol).max())
