@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 from oracle import paged as op
-from tests.test_paged_gpu import U, Batch, compare_attention, f64, tree
+from tests.test_paged_gpu import U, Batch, check_attention, compare_attention, f64, tree
 
 
 def widen(b, entries):
@@ -202,3 +202,15 @@ def test_decode_rounds_its_outputs_alone(cuda, H, KV, D, kind, ctx):
     tol = U[kind] * (abs(want) + e) + e + (2.0 ** -25 if kind == "f16" else 0)
     d = abs(f64(ops.paged_attention(b.q, b.kc, b.vc, *b.batch())) - want)
     assert (d <= tol).all(), float((d / tol).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,KV,D,act,cache", [(7, 1, 128, "bf16", "bf16"), (2, 2, 64, "bf16", "bf16"), (4, 2, 64, "f32", "f16"), (2, 2, 256, "f16", "f16")])
+@pytest.mark.parametrize("decode", [60, 500])
+def test_decode_rows_beside_a_prompt_chunk(cuda, H, KV, D, act, cache, decode):
+    """A step of many streams that decode and one prompt chunk, in any order: one kernel takes all of them."""
+    rows, ctx = [1] * decode, [(i * 53) % 90 for i in range(decode)]
+    rows[decode // 3], ctx[decode // 3] = 230, 410
+    ctx[decode // 2] = 1300
+    b = Batch(rows, ctx, H, KV, D, 16, act, cache, seed=decode + D)
+    check_attention(b)
