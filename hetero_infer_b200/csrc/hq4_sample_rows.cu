@@ -21,10 +21,11 @@
 // 42 with top-k 50, 45 without filters and 119 with top-p 0.9; one row 5, 16,
 // 11 and 21.
 //
-// Masses are integers of 2^-44 of the maximum's or so, and 0 below that, each
-// good to 2e-9 of itself (see mass()).  Their sums are exact, so the token does not depend on how the work is divided, and
-// rounding errors of fp32 sums over 1.5e5 entries, 1e-6 of the whole, which
-// would move tokens, do not arise.
+// Masses are integers of 2^-44 of the maximum's or so, and 0 below that: each is
+// good to 3e-9 of itself (see mass()) and cut off to such an integer, which is
+// much of a mass of a few.  Their sums are exact, so the token does not depend on
+// how the work is divided, and rounding errors of fp32 sums over 1.5e5 entries,
+// 1e-6 of the whole, which would move tokens, do not arise.
 //
 // A thread owns a run of consecutive entries, so its columns above the end that
 // is found add up to what its run (or its pair's) contributes to the draw, and
@@ -191,10 +192,13 @@ struct SampleRow {
     // arithmetic (fp64 is several times slower).  x * oct is Q / 64 + g: its
     // product as a sum of two floats (a fused multiply-add gives the rounding
     // error), Q the nearest integer (left in the low bits by adding 1.5 * 2^23),
-    // |g| <= 2^-7; 2^g - 1 is three terms of its series (the fourth is below
-    // 4e-11), at most 5.5e-3, as an integer of 2^-29 (9e-10); 2^(Q/64) comes
-    // from a table and a shift.  The maximum's own g is left in all masses
-    // alike, which changes no ratio: they are up to 2^(1/64) times 2^44.
+    // |g| <= 9.3e-3 (2^-7, and of |x * oct| < 16000 what z does not hold: 5e-4,
+    // and x * oct_lo: 1e-3); 2^g - 1 is three terms of its series (the fourth is
+    // below 8e-11), at most 6.5e-3, as an integer of 2^-29 (9e-10; it fits the
+    // 22 bits that the addition rounds to, up to 7.8e-3); 2^(Q/64) comes from a
+    // table and a shift.  With their roundings a mass is good to 3e-9 (2.8e-9
+    // over 8 million values).  The maximum's own g is left in all masses alike,
+    // which changes no ratio: they are up to 2^(1/64) times 2^44.
     __device__ __forceinline__ u64 mass(float x) const {
         x -= shift;
         const float z = x * oct;
@@ -612,8 +616,9 @@ __global__ void __launch_bounds__(T, 512 / T) sample_rows_kernel(const SampleRow
     s.top = top;
     s.oct = (float)fmin(oct, 1e30);
     s.oct_lo = (float)(fmin(oct, 1e30) - (double)s.oct);
-    // a maximum of so many octaves: the entries within 44 of it are so near that their distance to it is exact
-    s.shift = fabs((double)top * oct) < 60000.0 ? 0.0f : top;
+    // a maximum of so many octaves (mass() says why): the entries within 44 of it are so near that their distance to it
+    // is exact
+    s.shift = fabs((double)top * oct) < 16000.0 ? 0.0f : top;
     s.top_q = (int)__float_as_uint(fmaf((top - s.shift) * s.oct, 64.0f, 12582912.0f));
     s.steps = fminf((float)(oct * (kSrSteps / kSrOctaves)), 1e30f);
 

@@ -295,3 +295,19 @@ def test_results_in_place_of_parameters(cuda):
                   ((x, u), dict(top_k=pool[:8], out=pool[1:]))):
         with pytest.raises(RuntimeError):
             ops.sample_rows(*a, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("octaves", [300, 9000, 15990, 16010, 24000, 33000, 41000, 52000, 59000, 61000, 500000])
+def test_maxima_of_many_octaves(cuda, octaves):
+    """Temperatures so low that the maximum is thousands of octaves: the entries with mass lie within few floats of it."""
+    rng = np.random.default_rng(octaves)
+    n, tops = 3000, np.array([20.0, -20.0, 31.5, -0.37, 900.0, -16.5], np.float32)
+    temps = (abs(tops) / (octaves * np.log(2))).astype(np.float32)
+    x = np.full((len(tops), n), -1e4, np.float32)
+    for i, top in enumerate(tops):
+        near = top - rng.uniform(0, 12, 60) * np.log(2) * temps[i]
+        x[i, rng.choice(n, 60, replace=False)] = near.astype(np.float32)
+        x[i, 7] = top
+    check(x, rng.random(len(tops)), temperature=temps)
+    check(x, rng.random(len(tops)), temperature=temps, top_p=[0.9] * len(tops))
