@@ -15,7 +15,7 @@
 // 16-bit terms (three bf16 terms hold 24 bits; two fp16 terms of a row scaled
 // by a power of two hold 22).
 //
-// 64 streams of 100 to 8200 entries, 28 heads of 128 over 4: 120 us, 5.1 TB/s;
+// 64 streams of 100 to 8200 entries, 28 heads of 128 over 4: 125 us, 4.9 TB/s;
 // the main loop reads at 6.2 to 6.9 TB/s, the rest is starts, ends and the
 // join.  One stream of 131072 with fp32 queries: 66 us, of them 45 in the main
 // loop.

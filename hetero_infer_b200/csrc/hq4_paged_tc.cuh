@@ -24,8 +24,8 @@
 // are scaled by 2^7, to at most 2^15: a probability is a normal number down to
 // 2^-21 of 2^m, and below that off by at most 2^-32 of it.
 //
-// 4 chunks of 1025 to 2048 tokens after up to 4096, 28 heads of 128: 317 us,
-// 1.04 PFLOP/s.  What bounds it is each group's own chain: a tile's softmax
+// 4 chunks of 1025 to 2048 tokens after up to 4096, 28 heads of 128: 360 us in
+// turn with other work, 0.91 PFLOP/s, and 324 replayed by itself.  What bounds it is each group's own chain: a tile's softmax
 // takes its threads about 2000 cycles and the tensor cores 1024 for its two
 // products, and the two groups of an SM cover for one another only in part;
 // then the join of split items, 8 to 20 us.  (Half a tile at a time, with the

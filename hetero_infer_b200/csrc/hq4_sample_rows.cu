@@ -15,11 +15,10 @@
 // the rest of the work is theirs.
 //
 // What bounds it is neither memory (64 rows of 152064 fp32 are 6 us of it) nor
-// the issue rate, but how few warps an SM has beside the slices: each issues
-// about every fourth cycle (46% of the slots with 8 warps), with a cluster
-// barrier of about 0.8 us between the steps.  64 such rows take 13 us greedy,
-// 42 with top-k 50, 45 without filters and 119 with top-p 0.9; one row 5, 16,
-// 11 and 21.
+// the issue rate, but how few warps an SM has beside the slices (16, which fill
+// 47% of the slots), with a cluster barrier of about 0.8 us between the steps.
+// 64 such rows take 14 us greedy, 43 with top-k 50, 51 without filters, 33 with
+// min-p 0.05 and 113 with top-p 0.9; one row 6, 19, 15, 10 and 23.
 //
 // Masses are integers of 2^-44 of the maximum's or so, and 0 below that: each is
 // good to 3e-9 of itself (see mass()) and cut off to such an integer, which is
