@@ -277,9 +277,6 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
         __syncwarp();
     }
     pdl_launch_dependents();
-    auto fewer_registers = [] {
-        if constexpr (kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    };
     const int D = p.head_dim, ksteps = D >> 4;
     bool fail = false;
     // A warp's wait, which ends: after so many tries (each may sleep up to a millisecond; reading a
@@ -499,141 +496,142 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
             }
             tc_fence_before();
         }
-    } else if (busy && warp == 4 * kGroups) {
-        // ---- matrix instructions -------------------------------------------------------
-        fewer_registers();
-        constexpr uint32_t kType = Elem<C>::code == HQ4_BF16 ? 1u : 0u;
-        const uint32_t id_s = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(kKeys >> 3) << 17) | (8u << 24);
-        const uint32_t id_o = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
-        uint32_t n_slot = 0, n_q[kGroups], n_p[kGroups];
-        for (int g = 0; g < kGroups; g++) n_q[g] = n_p[g] = 0;
-        auto slot_at = [&](uint32_t n) { return ring + (n % S::kSlots) * S::kSlot; };
-        auto full = [&](uint32_t n) { return wait(full_bar(n % S::kSlots), n / S::kSlots); };
-        auto scores = [&](int g, uint32_t slot) {
-            const uint64_t a = sw128_desc(base + g * S::kQBytes), b = sw128_desc(slot);
-            const uint32_t d = tmem + g * kKeys;
-            if (pt_elect()) {
-#pragma unroll
-                for (int k = 0; k < kDim / 16; k++) {
-                    if (k >= ksteps) break;
-                    // 16 dims: 32 bytes on within a 128-byte row, then the next block of 64 dims
-                    pt_mma_ss(d, a + ((k >> 2) * (128 * 128 / 16) + 2 * (k & 3)),
-                              b + ((k >> 2) * (kKeys * 128 / 16) + 2 * (k & 3)), id_s, k ? 1u : 0u);
-                }
-                umma_commit(s_bar(g));
-            }
-            __syncwarp();
-        };
-        while (left > 0 && !fail) {
-            int t0, t1;
-            const int units = piece(t0, t1);
-            if (t1 == 0) break;  // the part ends before the item's first tile
-            const int ng = groups_of();
-            if (!full(n_slot)) break;
-            for (int g = 0; g < ng && !fail; g++) {
-                if (!wait(q_bar(g), n_q[g])) break;
-                n_q[g]++;
-                tc_fence_after();
-                scores(g, slot_at(n_slot));
-            }
-            if (fail) break;
-            if (pt_elect()) umma_commit(empty_bar(n_slot % S::kSlots));
-            __syncwarp();
-            for (int t = t0; t < t1 && !fail; t++) {
-                const uint32_t nv = n_slot + 1, nk = n_slot + 2;  // this tile's values, the next one's keys
-                const bool more = t + 1 < t1;
-                if (!full(nv)) break;
-                const int past = it->keys - t * kKeys;  // values that no row sees may be anything: zeros instead
-                if (past < kKeys) {
-                    for (int i = lane; i < (kKeys - max(past, 0)) * (kDim / 8); i += 32) {
-                        const int r = max(past, 0) + i / (kDim / 8), c = i % (kDim / 8);
-                        *reinterpret_cast<uint4*>(sm + (slot_at(nv) - base) + (c >> 3) * (kKeys * 128) +
-                                                  sw128_off(r, c & 7)) = make_uint4(0, 0, 0, 0);
+    } else if (busy) {
+        // (one instruction for all warps of the warpgroup)
+        if constexpr (kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp == 4 * kGroups) {
+            // ---- matrix instructions -------------------------------------------------------
+            constexpr uint32_t kType = Elem<C>::code == HQ4_BF16 ? 1u : 0u;
+            const uint32_t id_s = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(kKeys >> 3) << 17) | (8u << 24);
+            const uint32_t id_o = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
+            uint32_t n_slot = 0, n_q[kGroups], n_p[kGroups];
+            for (int g = 0; g < kGroups; g++) n_q[g] = n_p[g] = 0;
+            auto slot_at = [&](uint32_t n) { return ring + (n % S::kSlots) * S::kSlot; };
+            auto full = [&](uint32_t n) { return wait(full_bar(n % S::kSlots), n / S::kSlots); };
+            auto scores = [&](int g, uint32_t slot) {
+                const uint64_t a = sw128_desc(base + g * S::kQBytes), b = sw128_desc(slot);
+                const uint32_t d = tmem + g * kKeys;
+                if (pt_elect()) {
+    #pragma unroll
+                    for (int k = 0; k < kDim / 16; k++) {
+                        if (k >= ksteps) break;
+                        // 16 dims: 32 bytes on within a 128-byte row, then the next block of 64 dims
+                        pt_mma_ss(d, a + ((k >> 2) * (128 * 128 / 16) + 2 * (k & 3)),
+                                  b + ((k >> 2) * (kKeys * 128 / 16) + 2 * (k & 3)), id_s, k ? 1u : 0u);
                     }
-                    fence_proxy_async_smem();
-                    __syncwarp();
+                    umma_commit(s_bar(g));
                 }
+                __syncwarp();
+            };
+            while (left > 0 && !fail) {
+                int t0, t1;
+                const int units = piece(t0, t1);
+                if (t1 == 0) break;  // the part ends before the item's first tile
+                const int ng = groups_of();
+                if (!full(n_slot)) break;
                 for (int g = 0; g < ng && !fail; g++) {
-                    if (!wait(p_bar(g), n_p[g])) break;
-                    n_p[g]++;
+                    if (!wait(q_bar(g), n_q[g])) break;
+                    n_q[g]++;
                     tc_fence_after();
-                    const uint64_t b = sw128_mn_desc(slot_at(nv), kKeys * 128);
-                    const uint32_t d = tmem + S::kOCol + g * kDim, a = tmem + g * kKeys;
-                    if (pt_elect()) {
-#pragma unroll
-                        for (int k = 0; k < kKeys / 16; k++)  // 16 keys: 2048 bytes on
-                            pt_mma_ts(d, a + 8 * k, b + k * (2048 / 16), id_o, k || t > t0 ? 1u : 0u);
-                        if (!more) umma_commit(o_bar(g));
-                    }
-                    __syncwarp();
-                    if (more) {
-                        if (g == 0 && !full(nk)) break;
-                        tc_fence_after();
-                        scores(g, slot_at(nk));
-                    }
+                    scores(g, slot_at(n_slot));
                 }
                 if (fail) break;
-                if (pt_elect()) {
-                    umma_commit(empty_bar(nv % S::kSlots));
-                    if (more) umma_commit(empty_bar(nk % S::kSlots));
-                }
+                if (pt_elect()) umma_commit(empty_bar(n_slot % S::kSlots));
                 __syncwarp();
-                n_slot += 2;
-            }
-            next(units);
-        }
-        if (pt_elect()) umma_commit(end_bar);
-        __syncwarp();
-        // all products are done before the memory goes (a limit of its own: the others may have failed)
-        mbar_wait_ns(end_bar, 0, kPtWaitNs);
-    } else if (busy && warp == 4 * kGroups + 1) {
-        // ---- keys and values -------------------------------------------------------------
-        fewer_registers();
-        const uint64_t policy = l2_policy_evict_last();
-        const int box = min(1 << p.b.page_shift, kKeys), boxes = kKeys / box;
-        uint32_t n = 0, tile_no = 0;
-        while (left > 0 && !fail) {
-            int t0, t1;
-            const int units = piece(t0, t1);
-            if (t1 == 0) break;  // the part ends before the item's first tile
-            if (lane == 0 && (it->len < 0 || (long long)it->len + it->n_tok > (long long)p.b.pages_per_seq << p.b.page_shift))
-                atomicOr(p.b.status, kStatusPaged);  // rows whose entries have no place
-            for (int t = t0; t < t1 && !fail; t++, tile_no++) {
-                const int e = t * kKeys + lane * box;
-                int page = -1;
-                if (lane < boxes && e < it->keys) {
-                    page = find_page(p.b, it->s, e);
-                    if (page < 0) atomicOr(p.b.status, kStatusPaged);
-                }
-                const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
-                if (lane < kKeys / 32) {
-                    uint32_t v = 0;
-                    for (int b = 0; b < 32; b += min(box, 32))
-                        if (ok >> ((lane * 32 + b) / box) & 1) v |= (box >= 32 ? 0xffffffffu : (1u << box) - 1u) << b;
-                    s_valid[tile_no & 7][lane] = v;
-                }
-                __syncwarp();
-                for (int kv = 0; kv < 2; kv++, n++) {
-                    const int slot = n % S::kSlots;
-                    if (n >= S::kSlots && !wait(empty_bar(slot), n / S::kSlots - 1)) break;
-                    if (lane == 0) mbar_arrive_expect_tx(full_bar(slot), S::kSlot);
+                for (int t = t0; t < t1 && !fail; t++) {
+                    const uint32_t nv = n_slot + 1, nk = n_slot + 2;  // this tile's values, the next one's keys
+                    const bool more = t + 1 < t1;
+                    if (!full(nv)) break;
+                    const int past = it->keys - t * kKeys;  // values that no row sees may be anything: zeros instead
+                    if (past < kKeys) {
+                        for (int i = lane; i < (kKeys - max(past, 0)) * (kDim / 8); i += 32) {
+                            const int r = max(past, 0) + i / (kDim / 8), c = i % (kDim / 8);
+                            *reinterpret_cast<uint4*>(sm + (slot_at(nv) - base) + (c >> 3) * (kKeys * 128) +
+                                                      sw128_off(r, c & 7)) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    for (int g = 0; g < ng && !fail; g++) {
+                        if (!wait(p_bar(g), n_p[g])) break;
+                        n_p[g]++;
+                        tc_fence_after();
+                        const uint64_t b = sw128_mn_desc(slot_at(nv), kKeys * 128);
+                        const uint32_t d = tmem + S::kOCol + g * kDim, a = tmem + g * kKeys;
+                        if (pt_elect()) {
+    #pragma unroll
+                            for (int k = 0; k < kKeys / 16; k++)  // 16 keys: 2048 bytes on
+                                pt_mma_ts(d, a + 8 * k, b + k * (2048 / 16), id_o, k || t > t0 ? 1u : 0u);
+                            if (!more) umma_commit(o_bar(g));
+                        }
+                        __syncwarp();
+                        if (more) {
+                            if (g == 0 && !full(nk)) break;
+                            tc_fence_after();
+                            scores(g, slot_at(nk));
+                        }
+                    }
+                    if (fail) break;
+                    if (pt_elect()) {
+                        umma_commit(empty_bar(nv % S::kSlots));
+                        if (more) umma_commit(empty_bar(nk % S::kSlots));
+                    }
                     __syncwarp();
-                    if (lane < boxes) {
-                        // without a page: a place past the last page, which reads as zeros
-                        const int y = e & ((1 << p.b.page_shift) - 1), w = page >= 0 ? page : p.b.n_pages;
-                        for (int b = 0; b < S::kBlocks; b++)
-                            tma_load_4d(ring + slot * S::kSlot + b * (kKeys * 128) + lane * box * 128,
-                                        kv ? &tm_v : &tm_k, b * 64, y, it->h, w, full_bar(slot), policy);
+                    n_slot += 2;
+                }
+                next(units);
+            }
+            if (pt_elect()) umma_commit(end_bar);
+            __syncwarp();
+            // all products are done before the memory goes (a limit of its own: the others may have failed)
+            mbar_wait_ns(end_bar, 0, kPtWaitNs);
+        } else if (warp == 4 * kGroups + 1) {
+            // ---- keys and values -------------------------------------------------------------
+            const uint64_t policy = l2_policy_evict_last();
+            const int box = min(1 << p.b.page_shift, kKeys), boxes = kKeys / box;
+            uint32_t n = 0, tile_no = 0;
+            while (left > 0 && !fail) {
+                int t0, t1;
+                const int units = piece(t0, t1);
+                if (t1 == 0) break;  // the part ends before the item's first tile
+                if (lane == 0 && (it->len < 0 || (long long)it->len + it->n_tok > (long long)p.b.pages_per_seq << p.b.page_shift))
+                    atomicOr(p.b.status, kStatusPaged);  // rows whose entries have no place
+                for (int t = t0; t < t1 && !fail; t++, tile_no++) {
+                    const int e = t * kKeys + lane * box;
+                    int page = -1;
+                    if (lane < boxes && e < it->keys) {
+                        page = find_page(p.b, it->s, e);
+                        if (page < 0) atomicOr(p.b.status, kStatusPaged);
+                    }
+                    const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
+                    if (lane < kKeys / 32) {
+                        uint32_t v = 0;
+                        for (int b = 0; b < 32; b += min(box, 32))
+                            if (ok >> ((lane * 32 + b) / box) & 1) v |= (box >= 32 ? 0xffffffffu : (1u << box) - 1u) << b;
+                        s_valid[tile_no & 7][lane] = v;
+                    }
+                    __syncwarp();
+                    for (int kv = 0; kv < 2; kv++, n++) {
+                        const int slot = n % S::kSlots;
+                        if (n >= S::kSlots && !wait(empty_bar(slot), n / S::kSlots - 1)) break;
+                        if (lane == 0) mbar_arrive_expect_tx(full_bar(slot), S::kSlot);
+                        __syncwarp();
+                        if (lane < boxes) {
+                            // without a page: a place past the last page, which reads as zeros
+                            const int y = e & ((1 << p.b.page_shift) - 1), w = page >= 0 ? page : p.b.n_pages;
+                            for (int b = 0; b < S::kBlocks; b++)
+                                tma_load_4d(ring + slot * S::kSlot + b * (kKeys * 128) + lane * box * 128,
+                                            kv ? &tm_v : &tm_k, b * 64, y, it->h, w, full_bar(slot), policy);
+                        }
                     }
                 }
+                next(units);
             }
-            next(units);
+            // no copy is left behind: each slot's last one has arrived
+            for (uint32_t i = n > S::kSlots ? n - S::kSlots : 0; i < n; i++)
+                mbar_wait_ns(full_bar(i % S::kSlots), (i / S::kSlots) & 1u, kPtWaitNs);
         }
-        // no copy is left behind: each slot's last one has arrived
-        for (uint32_t i = n > S::kSlots ? n - S::kSlots : 0; i < n; i++)
-            mbar_wait_ns(full_bar(i % S::kSlots), (i / S::kSlots) & 1u, kPtWaitNs);
     }
-    if (busy && warp > 4 * kGroups + 1) fewer_registers();  // the rest of the third warpgroup
     if (fail && lane == 0) atomicOr(p.b.status, 1);
     __syncwarp();
     tc_fence_before();
