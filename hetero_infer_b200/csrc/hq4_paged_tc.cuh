@@ -20,17 +20,18 @@
 // most half a step of each probability: the same size as the rounding of the
 // 16-bit output (errors against 64 bits are up to 1.4 times that rounding's
 // alone; a caller who wants them smaller passes fp32 queries, which the
-// warp-level kernel takes).  fp16 has few steps below 1, so its P (and the sums with it)
-// are scaled by 2^7, to at most 2^15: a probability is a normal number down to
-// 2^-21 of 2^m, and below that off by at most 2^-32 of it.
+// warp-level kernel takes).  fp16 has few steps below 1, so its P (and the sums
+// with it) are scaled by 2^7, to at most 2^15: a probability is a normal number
+// down to 2^-21 of 2^m, and below that off by at most 2^-32 of it.
 //
-// 4 chunks of 1025 to 2048 tokens after up to 4096, 28 heads of 128: 360 us in
-// turn with other work, 0.91 PFLOP/s, and 324 replayed by itself.  What bounds it is each group's own chain: a tile's softmax
-// takes its threads about 2000 cycles and the tensor cores 1024 for its two
-// products, and the two groups of an SM cover for one another only in part;
-// then the join of split items, 8 to 20 us.  (Half a tile at a time, with the
-// other half's products under way: 521 us; two threads to a row: slower; the
-// groups sharing the rows and splitting the keys: 391.)
+// 4 chunks of 1025 to 2048 tokens after up to 4096, 28 heads of 128: 367 us in
+// turn with other work, 0.90 PFLOP/s, and 328 replayed by itself.  What bounds it
+// is each group's own chain: a tile's softmax takes its threads about 2000 cycles
+// and the tensor cores 1024 for its two products, and the two groups of an SM
+// cover for one another only in part; then the join of split items, 8 to 20 us.
+// (Half a tile at a time, with the other half's products under way: 521 us; two
+// threads to a row: slower; the groups sharing the rows and splitting the keys:
+// 391.)
 #pragma once
 #include <algorithm>
 
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                 const uint64_t a = sw128_desc(base + g * S::kQBytes), b = sw128_desc(slot);
                 const uint32_t d = tmem + g * kKeys;
                 if (pt_elect()) {
-    #pragma unroll
+#pragma unroll
                     for (int k = 0; k < kDim / 16; k++) {
                         if (k >= ksteps) break;
                         // 16 dims: 32 bytes on within a 128-byte row, then the next block of 64 dims
@@ -559,7 +560,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                         const uint64_t b = sw128_mn_desc(slot_at(nv), kKeys * 128);
                         const uint32_t d = tmem + S::kOCol + g * kDim, a = tmem + g * kKeys;
                         if (pt_elect()) {
-    #pragma unroll
+#pragma unroll
                             for (int k = 0; k < kKeys / 16; k++)  // 16 keys: 2048 bytes on
                                 pt_mma_ts(d, a + 8 * k, b + k * (2048 / 16), id_o, k || t > t0 ? 1u : 0u);
                             if (!more) umma_commit(o_bar(g));
