@@ -244,8 +244,9 @@ __device__ __forceinline__ bool paged_sees(const PagedAttnParams& p, const Paged
 // One output row, entry by entry (one warp).  The tiled kernels multiply
 // masked probabilities of zero by values that they do not look at; where such
 // a value is an infinity or a NaN, the row comes out as NaN and is computed
-// here again, from the entries that it sees alone.  So is a row whose sum is 0:
-// one that sees nothing is zeros, one whose scores are all -inf is NaN (0 / 0).
+// here again, from the entries that it sees alone.  So is a row whose sum is 0,
+// unless none of the entries has a page: one that sees nothing is zeros, one whose
+// scores are all -inf is NaN (0 / 0).
 template <class A, class C>
 __device__ __noinline__ void paged_slow_row(const PagedAttnParams& p, const PagedItem& it, int r) {
     const int lane = threadIdx.x & 31, D = p.head_dim;
@@ -259,10 +260,22 @@ __device__ __noinline__ void paged_slow_row(const PagedAttnParams& p, const Page
         qv[i] = i < nd ? Elem<A>::to(q[lane + 32 * i]) : 0.0f;
         acc[i] = 0.0f;
     }
+    // 32 entries are looked up at once: a padded sequence that still has a length, but no pages, is passed quickly
+    // (a lane's entry, and its page where the row sees it)
+    int mine = -1;
+    uint32_t left = 0;
     for (int e = 0; e < it.keys; e++) {
-        if (!paged_sees(p, it, tok, e)) continue;
-        const int page = find_page(p.b, it.s, e);
-        if (page < 0) continue;
+        if ((e & 31) == 0) {
+            mine = e + lane < it.keys && paged_sees(p, it, tok, e + lane) ? find_page(p.b, it.s, e + lane) : -1;
+            left = __ballot_sync(0xffffffffu, mine >= 0);
+        }
+        if (!left) {
+            e |= 31;
+            continue;
+        }
+        if (!(left >> (e & 31) & 1)) continue;
+        left &= ~(1u << (e & 31));
+        const int page = __shfl_sync(0xffffffffu, mine, e & 31);
         const long long at = (long long)page * p.b.page_stride +
                              (((long long)it.h << p.b.page_shift) + (e & ((1 << p.b.page_shift) - 1))) * D;
         const C* k = static_cast<const C*>(p.k) + at;
@@ -294,7 +307,7 @@ __device__ __noinline__ void paged_slow_row(const PagedAttnParams& p, const Page
 template <int kRows, int kDim>
 struct PagedWs {
     PagedStart* info;  // of each CTA's part; without any work at all, of CTA 0 alone
-    float2* ml;       // [pieces][kRows]: running maximum (of log2 scores) and sum
+    float2* ml;       // [pieces][kRows]: running maximum (of log2 scores) and sum (1 for 0 where an entry had a page)
     float* o;         // [pieces][kRows][kDim], not divided
     __host__ __device__ PagedWs(void* ws, int ctas) {
         unsigned char* p = static_cast<unsigned char*>(ws);
@@ -358,7 +371,12 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
         };
         ask(mine);  // (before the weights are known)
         float m = -INFINITY;
-        for (int i = lane; i < n; i += 32) m = fmaxf(m, ws.ml[at(i)].x);
+        bool any = false;  // an entry has a page
+        for (int i = lane; i < n; i += 32) {
+            const float2 ml = ws.ml[at(i)];
+            m = fmaxf(m, ml.x);
+            any |= ml.y != 0.0f;
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         const float mu = m == -INFINITY ? 0.0f : m;
@@ -411,7 +429,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) paged_combine_kernel(const
         const int row = it.rt * kRows + r, tok = row / p.group, head = it.h * p.group + row % p.group;
         A* out = static_cast<A*>(p.out) + ((long long)(it.row0 + tok) * p.n_heads + head) * D;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        bool bad = l == 0.0f;
+        bool bad = l == 0.0f && any;
 #pragma unroll
         for (int j = 0; j < kPer; j++)
             if (lane * 4 + 128 * j < D) {

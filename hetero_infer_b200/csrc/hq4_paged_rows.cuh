@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(W * 32) paged_attn_kernel(const __grid_constan
     __shared__ PagedScan scan;
     __shared__ float s_m[W][kRows], s_l[W][kRows], s_qs[kRows];
     __shared__ int s_os[W];  // where in shared memory each warp has left its outputs
+    __shared__ uint32_t s_any[W];  // whether any of its entries had a page
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int D = p.head_dim, ksteps = D >> 4;
@@ -261,6 +262,7 @@ __global__ void __launch_bounds__(W * 32) paged_attn_kernel(const __grid_constan
             }
         }
         const int first_tok = it.rt * kRows / p.group;
+        uint32_t any = 0;
         for (int t = t0 + warp; t < t1; t += W) {
             int ahead = stage + kStages - 1;
             if (ahead >= kStages) ahead -= kStages;
@@ -268,6 +270,7 @@ __global__ void __launch_bounds__(W * 32) paged_attn_kernel(const __grid_constan
             const uint32_t more = load_tile(it, t + (kStages - 1) * W, t1, page_next, ahead);
             page_next = look_up(it, t + kStages * W, t1);
             const uint32_t ok = (uint32_t)oks & 0xffffu;
+            any |= ok;
             oks = (oks >> 16) | (unsigned long long)more << (16 * (kStages - 2));
             cp_async_wait<kStages - 1>();
             __syncwarp();
@@ -393,7 +396,10 @@ __global__ void __launch_bounds__(W * 32) paged_attn_kernel(const __grid_constan
             __syncwarp();
         }
         float* os = reinterpret_cast<float*>(smem + os_at);
-        if (lane == 0) s_os[warp] = os_at;
+        if (lane == 0) {
+            s_os[warp] = os_at;
+            s_any[warp] = any;
+        }
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -433,7 +439,13 @@ __global__ void __launch_bounds__(W * 32) paged_attn_kernel(const __grid_constan
                 for (int i = 0; i < W; i++) w[i] = ll == 0.0f ? 0.0f : w[i] / ll;
             A* out = static_cast<A*>(p.out) + ((long long)(it.row0 + row / p.group) * p.n_heads + it.h * p.group + row % p.group) * D;
             float* part = ws.o + ((size_t)piece * kRows + r) * kDim;
-            bool bad = ll == 0.0f;
+            if (ll == 0.0f) {
+                any = 0;
+#pragma unroll
+                for (int i = 0; i < W; i++) any |= s_any[i];
+                if (!whole && any) ll = 1.0f;  // (of weight 0: its maximum is -inf)
+            }
+            bool bad = ll == 0.0f && any;
             for (int d = lane; d < D; d += 32) {
                 float y = 0.0f;
 #pragma unroll

@@ -366,6 +366,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
             const bool warp_on = in && it->rt * kRows + g * 128 + (warp & 3) * 32 < rows;
             const int tok = on ? row / p.group : 0;
             float m = -INFINITY, l = 0.0f;  // of scaled scores (log2), and the row's sum
+            uint32_t any = 0;               // an entry has a page
             const int t_plain = (it->len + (p.tree_mask ? 0 : it->rt * kRows / p.group + 1)) / kKeys;  // before: all seen
             const float c2 = fmaxf(fabsf(p.scale_log2), 1e-30f);  // not 0: masked scores stay -inf
             if (in) {
@@ -383,9 +384,12 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                         bool plain = t < t_plain;
 #pragma unroll
                         for (int i = 0; i < kParts; i++) plain = plain && valid[i] == 0xffffffffu;
-                        if (!__all_sync(0xffffffffu, plain)) {
+                        if (__all_sync(0xffffffffu, plain)) {
+                            any = 1;
+                        } else {
 #pragma unroll
                             for (int i = 0; i < kParts; i++) {
+                                any |= valid[i];
                                 const uint32_t see = on ? valid[i] & paged_sees32(p, *it, tok, t * kKeys + i * 32) : 0u;
 #pragma unroll
                                 for (int j = 0; j < 32; j++)
@@ -466,7 +470,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                 C* out = static_cast<C*>(p.out) +
                          ((long long)(mine->row0 + tok) * p.n_heads + mine->h * p.group + row % p.group) * D;
                 const size_t at = (size_t)piece_no * kRows + r;
-                bool bad = on && whole && l == 0.0f;
+                bool bad = on && whole && l == 0.0f && any;
                 for (int c = 0; c < D; c += 32) {
                     uint32_t o[32];
                     tmem_ld32(o_col + c, o);
@@ -487,7 +491,7 @@ __global__ void __launch_bounds__(PtShape<kDim>::kThreads, 1)
                     }
                     __syncwarp();
                 }
-                if (on && !whole) ws.ml[at] = make_float2(m, l);
+                if (on && !whole) ws.ml[at] = make_float2(m, l == 0.0f && any ? 1.0f : l);
                 uint32_t again = __ballot_sync(0xffffffffu, bad);
                 while (again) {
                     const int i = __ffs(again) - 1;

@@ -214,3 +214,17 @@ def test_decode_rows_beside_a_prompt_chunk(cuda, H, KV, D, act, cache, decode):
     ctx[decode // 2] = 1300
     b = Batch(rows, ctx, H, KV, D, 16, act, cache, seed=decode + D)
     check_attention(b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,D,act,cache", KERNELS)
+def test_padded_sequences_without_pages(cuda, rows, D, act, cache):
+    """Sequences that still have a length but no pages see nothing: zeros, beside others that are right."""
+    b = Batch([rows] * 6, [3000, 40, 2999, 100, 2000, 1], 4, 2, D, 16, act, cache, seed=D + 5)
+    b.pages[::2] = -1
+    got = check_attention(b)
+    for s in (0, 2, 4):
+        assert (got[s * rows:(s + 1) * rows] == 0).all()
+    m = tree(b.rows, 3)
+    got = check_attention(b, tree_mask=m)
+    assert (got[:rows] == 0).all()
